@@ -20,6 +20,9 @@ OBJ = os.path.join(CSRC, "build")
 SO = os.path.join(HERE, "libcpfn_hip.so")
 ARCH = "gfx950"
 
+# no packed fp32 instructions at all (v_pk_{add,mul,fma}_f32 have given wrong results on this hardware now and then)
+_NO_PK = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
 # file -> extra flags
 SOURCES = {
     "abi.hip": [],
@@ -43,7 +46,11 @@ SOURCES = {
     "losses.hip": [],
     "merging.hip": [],
     "metrics.hip": [],
-    "optim.hip": [],
+    "optim.hip": _NO_PK,
+    "rownorm_fwd.hip": _NO_PK,
+    "rownorm_bwd.hip": _NO_PK,
+    "route.hip": _NO_PK,
+    "gradnorm.hip": _NO_PK,
 }
 COMMON = ["--offload-arch=" + ARCH, "-O3", "-fPIC", "-std=c++17", "-fvisibility=hidden",
           "-Wall", "-Wno-unused-function"]

@@ -5,6 +5,7 @@
 // torch/optim/adam.py, non-amsgrad, maximize=False), capturable: learning rate, step count and the
 // "skip this step" flag live in device memory.
 #include "common.h"
+#include "gradnorm.h"
 
 namespace {
 
@@ -22,12 +23,29 @@ namespace {
 // it needs the BatchNorm coefficients of the last finalize launch of the pass, so as a reduction it was a launch of its own
 // (12 workgroups, 5.7 us + a kernel boundary) between that finalize and this kernel.
 struct AdamXw { const float *S, *coef; int C; float *out; };
+// CLIP (cpfn_adam_flat_clip): the gradients' squares have been summed by cpfn_grad_sumsq; this wave adds the partial sums (fp64, a fixed
+// order), forms the clipping factor — coef[3], applied by the streaming kernel as it loads the gradients, which stay as they are in
+// memory — and skips the step if the norm is not finite, i.e. if any gradient is not: the scan for NaN / inf comes with the norm.
+struct AdamClip { const double *parts; int count; double max_norm; float *norm; };
+template <bool CLIP>
 __global__ __launch_bounds__(64) void adam_prepare_kernel(const float *__restrict__ lr, float beta1, float beta2,
                                                          float *__restrict__ step, double *__restrict__ pows,
                                                          const float *__restrict__ found_inf, float *__restrict__ coef,
                                                          unsigned *__restrict__ nf_partial, int nf_count,
-                                                         float *__restrict__ skipped, int n_sticky, const AdamXw xw) {
+                                                         float *__restrict__ skipped, int n_sticky, const AdamXw xw, const AdamClip cl) {
   unsigned bad = 0;
+  if (CLIP) {
+    double s = 0.0;
+    for (int i = threadIdx.x; i < cl.count; i += 64) s += cl.parts[i];
+#pragma unroll
+    for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d, 64);
+    const double total = sqrt(s);
+    bad = !(total <= 1.7976931348623157e308);
+    if (threadIdx.x == 0) {
+      coef[3] = grad_clip_factor(total, cl.max_norm);
+      if (cl.norm) *cl.norm = (float)total;
+    }
+  }
   if (xw.out) {
     const int C = xw.C;
     for (int e = threadIdx.x; e < 3 * C; e += 64) {
@@ -51,6 +69,7 @@ __global__ __launch_bounds__(64) void adam_prepare_kernel(const float *__restric
   else if (skipped) *skipped += 1.f;
 }
 
+template <bool CLIP>
 __global__ __launch_bounds__(256) void adam_flat_kernel(float *__restrict__ p, const float *__restrict__ g,
                                                         float *__restrict__ m, float *__restrict__ v, long long n,
                                                         float beta1, float beta2, float eps, float weight_decay,
@@ -70,6 +89,10 @@ __global__ __launch_bounds__(256) void adam_flat_kernel(float *__restrict__ p, c
     g4 = make_float4(g[i0], i1 < n ? g[i1] : 0.f, i2 < n ? g[i2] : 0.f, 0.f);
     m4 = make_float4(m[i0], i1 < n ? m[i1] : 0.f, i2 < n ? m[i2] : 0.f, 0.f);
     v4 = make_float4(v[i0], i1 < n ? v[i1] : 0.f, i2 < n ? v[i2] : 0.f, 0.f);
+  }
+  if (CLIP) {
+    const float f = coef[3];
+    g4.x *= f; g4.y *= f; g4.z *= f; g4.w *= f;
   }
   float pv[4] = {p4.x, p4.y, p4.z, p4.w}, gv[4] = {g4.x, g4.y, g4.z, g4.w}, mv[4] = {m4.x, m4.y, m4.z, m4.w},
         vv[4] = {v4.x, v4.y, v4.z, v4.w};
@@ -155,8 +178,28 @@ extern "C" int cpfn_adam_flat_xw(float *p, const float *g, float *m, float *v, l
   if (((uintptr_t)p | (uintptr_t)g | (uintptr_t)m | (uintptr_t)v) & 15) return CPFN_EINVAL;
   if (n == 0) return 0;
   hipStream_t st = (hipStream_t)stream;
-  adam_prepare_kernel<<<1, 64, 0, st>>>(lr, beta1, beta2, step, pows, found_inf, coef3, nf_partial, nf_count, skipped, n_sticky, xw);
-  adam_flat_kernel<<<cpfn_cdiv(cpfn_cdiv(n, 4), 256), 256, 0, st>>>(p, g, m, v, n, beta1, beta2, eps, weight_decay, coef3);
+  adam_prepare_kernel<false><<<1, 64, 0, st>>>(lr, beta1, beta2, step, pows, found_inf, coef3, nf_partial, nf_count, skipped, n_sticky, xw,
+                                               AdamClip{});
+  adam_flat_kernel<false><<<cpfn_cdiv(cpfn_cdiv(n, 4), 256), 256, 0, st>>>(p, g, m, v, n, beta1, beta2, eps, weight_decay, coef3);
+  return cpfn_launch_status();
+}
+
+extern "C" int cpfn_adam_flat_clip(float *p, const float *g, float *m, float *v, long long n, const float *lr, float beta1,
+                                   float beta2, float eps, float weight_decay, float *step, double *pows,
+                                   const float *found_inf, float *coef4, unsigned *nf_partial, int nf_count, int n_sticky,
+                                   float *skipped, double max_norm, double *parts, float *norm, void *stream) {
+  if (n < 0 || !p || !g || !m || !v || !lr || !step || !pows || !coef4 || nf_count < 0 || (nf_count > 0 && !nf_partial) ||
+      n_sticky < 0 || n_sticky > nf_count || !(max_norm >= 0.0) || !parts || !norm)
+    return CPFN_EINVAL;
+  if ((((uintptr_t)p | (uintptr_t)g | (uintptr_t)m | (uintptr_t)v) & 15) || ((uintptr_t)parts & 7)) return CPFN_EINVAL;
+  if (n == 0) return 0;
+  hipStream_t st = (hipStream_t)stream;
+  const int rc = cpfn_grad_sumsq(g, n, parts, stream);
+  if (rc) return rc;
+  const AdamClip cl = {parts, cpfn_grad_sumsq_blocks(n), max_norm, norm};
+  adam_prepare_kernel<true><<<1, 64, 0, st>>>(lr, beta1, beta2, step, pows, found_inf, coef4, nf_partial, nf_count, skipped, n_sticky,
+                                              AdamXw{}, cl);
+  adam_flat_kernel<true><<<cpfn_cdiv(cpfn_cdiv(n, 4), 256), 256, 0, st>>>(p, g, m, v, n, beta1, beta2, eps, weight_decay, coef4);
   return cpfn_launch_status();
 }
 

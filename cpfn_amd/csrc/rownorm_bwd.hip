@@ -1,0 +1,334 @@
+// Backward pass of the residual block's norms, gate and residual scale (rownorm.h), in one pass over the rows.
+//
+// Nothing of the forward pass is kept but its inputs: out and both norms' statistics are formed again from x, y and the gate, which
+// the gradients need anyway (out in fp32, as the forward pass had it).  With D = d loss / d out (its own gradient and the one through
+// the next norm), hats for normalised values and means over the channels:
+//   dh = d_normed next_weight,  D = d_out + r1 (dh - [mean dh] - hat1 mean(dh hat1)),   d_x = D
+//   du = D scale a,  e = du weight,  d_y = r2 (e - [mean e] - hat2 mean(e hat2))   (d_y = du without a post-norm)
+//   d_gate = D scale u  (times a (1 - a) behind a sigmoid), summed over the rows that share it
+// [..] for layer norms only.  The parameters' gradients are column sums of four products:
+//   S1 = sum D a hat2,  S2 = sum D a,  S3 = sum d_normed hat1,  S4 = sum d_normed
+//   d_weight = scale S1,  d_bias = scale S2,  d_scale = weight S1 + bias S2,  d_next_weight = S3,  d_next_bias = S4
+// (hat2 = y without a post-norm).  A lane owns its eight channels for every row of its workgroup, so a column sum is a register until
+// the workgroup ends; the workgroups' sums are added by a second small launch in a fixed order: no atomics, bit-reproducible.
+#include "rownorm.h"
+
+namespace {
+
+template <typename T> struct NormBwd {
+  const T *x, *y, *gate, *d_out, *d_normed;
+  const float *weight, *bias, *scale, *next_weight;
+  long long P, rows_per_gate;      // rows that share a gate row (1: a gate for every row; P with no gate)
+  long long chunk;                 // rows of a workgroup (blocks_per_group > 1) ...
+  int blocks_per_group;            // ... of which so many cover one gate group,
+  int groups_per_block;            // or whole groups of a workgroup
+  long long groups;
+  int C, layer, sigmoid;
+  float eps;
+  T *d_x, *d_y, *d_gate;
+  float *part;                     // [workgroup][4 (+ 1)][C]
+  int shared_gate, sums12, sums34; // which sums are wanted
+};
+
+// sum over the row slots of a workgroup, element by element; lane `i` order of the registers -> dst[channel]
+template <typename T, int L, typename F> __device__ __forceinline__ void slots_sum(const float *v, float *lds, int C, F store) {
+  constexpr int THREADS = NormShape<T, L>::THREADS, ROWS = NormShape<T, L>::ROWS;
+  const int lane = threadIdx.x & (L - 1), slot = threadIdx.x / L;
+  if (ROWS == 1) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int c = norm_col<T, L>(lane, i);
+      if (c < C) store(c, v[i]);
+    }
+    return;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) lds[slot * (L * 8) + i * L + lane] = v[i];
+  __syncthreads();
+  for (int e = threadIdx.x; e < L * 8; e += THREADS) {
+    float t = 0.f;
+#pragma unroll
+    for (int q = 0; q < ROWS; ++q) t += lds[q * (L * 8) + e];
+    const int c = norm_col<T, L>(e & (L - 1), e / L);
+    if (c < C) store(c, t);
+  }
+}
+
+template <typename T, int L>
+__global__ __launch_bounds__((NormShape<T, L>::THREADS)) void norm_residual_bwd_kernel(const NormBwd<T> a) {
+  constexpr int ROWS = NormShape<T, L>::ROWS, THREADS = NormShape<T, L>::THREADS;
+  __shared__ float2 slots[32];
+  __shared__ float comb[ROWS > 1 ? THREADS * 8 : 1];
+  int turn = 0;
+  const int lane = threadIdx.x & (L - 1), slot = threadIdx.x / L, C = a.C;
+  const float inv_c = 1.f / (float)C;
+  const bool layer = a.layer != 0, post = a.weight != nullptr, has_y = a.y != nullptr, next = a.d_normed != nullptr;
+  float w[8], b[8], s[8], nw[8], s1[8], s2[8], s3[8], s4[8], sg[8];
+  param_load<T, L>(w, a.weight, lane, C, 1.f);
+  param_load<T, L>(b, a.bias, lane, C, 0.f);
+  param_load<T, L>(s, a.scale, lane, C, 1.f);
+  param_load<T, L>(nw, a.next_weight, lane, C, 1.f);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) { s1[i] = s2[i] = s3[i] = s4[i] = sg[i] = 0.f; }
+  const long long g0 = a.blocks_per_group > 1 ? blockIdx.x / a.blocks_per_group : (long long)blockIdx.x * a.groups_per_block;
+  long long g1 = a.blocks_per_group > 1 ? g0 + 1 : g0 + a.groups_per_block;
+  if (g1 > a.groups) g1 = a.groups;
+  const int nsums = 4 + (a.shared_gate && a.blocks_per_group > 1);
+  for (long long g = g0; g < g1; ++g) {
+    long long row0 = g * a.rows_per_gate, row1 = row0 + a.rows_per_gate;
+    if (a.blocks_per_group > 1) {
+      row0 += (long long)(blockIdx.x % a.blocks_per_group) * a.chunk;
+      if (row0 + a.chunk < row1) row1 = row0 + a.chunk;
+    }
+    for (long long base = row0; base < row1; base += ROWS) {
+      const long long r = base + slot;
+      const bool there = r < row1;
+      const float eps = there ? a.eps : 1.f;
+      RowRaw<T, L> rx, ry, rg, rd, rn;
+      row_zero(rx); row_zero(ry); row_zero(rg); row_zero(rd); row_zero(rn);
+      if (there) {
+        if (next) row_load(rx, a.x + r * C, lane, C);
+        if (has_y) row_load(ry, a.y + r * C, lane, C);
+        if (a.gate) row_load(rg, a.gate + (a.shared_gate ? g : r) * C, lane, C);
+        if (a.d_out) row_load(rd, a.d_out + r * C, lane, C);
+        if (next) row_load(rn, a.d_normed + r * C, lane, C);
+      }
+      float hat2[8], ga[8], r2 = 0.f;
+      if (has_y) {
+        row_unpack(ry, hat2);
+        if (post) r2 = row_normalise<T, L>(hat2, lane, C, inv_c, layer, eps, slots, turn);
+        if (a.gate) {
+          row_unpack(rg, ga);
+          if (a.sigmoid) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ga[i] = norm_sigmoid(ga[i]);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) ga[i] = 1.f;
+        }
+      }
+      float D[8];
+      row_unpack(rd, D);
+      if (next) {
+        float h[8], dn[8];
+        row_unpack(rx, h);
+        row_unpack(rn, dn);
+        if (has_y) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) h[i] = fmaf(s[i], ga[i] * fmaf(hat2[i], w[i], b[i]), h[i]);
+        }
+        const float r1 = row_normalise<T, L>(h, lane, C, inv_c, layer, eps, slots, turn);
+        float m1 = 0.f, m2 = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          s3[i] = fmaf(dn[i], h[i], s3[i]);
+          s4[i] += dn[i];
+          dn[i] *= nw[i];
+          m1 += dn[i];
+          m2 = fmaf(dn[i], h[i], m2);
+        }
+        row_sum2<L>(m1, m2, slots, turn);
+        m1 = layer ? m1 * inv_c : 0.f;
+        m2 *= inv_c;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) D[i] = fmaf(r1, dn[i] - m1 - h[i] * m2, D[i]);
+      }
+      if (there && a.d_x) row_store<T, L>(a.d_x + r * C, lane, C, D);
+      if (has_y) {
+        float e[8], m1 = 0.f, m2 = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float da = D[i] * ga[i];
+          s1[i] = fmaf(da, hat2[i], s1[i]);
+          s2[i] += da;
+          e[i] = da * s[i] * w[i];                       // (w = 1 without a post-norm: e = du)
+          m1 += e[i];
+          m2 = fmaf(e[i], hat2[i], m2);
+        }
+        if (a.d_gate) {
+          float dg[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            dg[i] = D[i] * s[i] * fmaf(hat2[i], w[i], b[i]);
+            if (a.sigmoid) dg[i] *= ga[i] * (1.f - ga[i]);
+            sg[i] += dg[i];
+          }
+          if (there && !a.shared_gate) row_store<T, L>(a.d_gate + r * C, lane, C, dg);
+        }
+        if (post) {
+          row_sum2<L>(m1, m2, slots, turn);
+          m1 = layer ? m1 * inv_c : 0.f;
+          m2 *= inv_c;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) e[i] = r2 * (e[i] - m1 - hat2[i] * m2);
+        }
+        if (there && a.d_y) row_store<T, L>(a.d_y + r * C, lane, C, e);
+      }
+    }
+    if (a.shared_gate && a.d_gate && a.blocks_per_group == 1) {        // this workgroup has seen all rows of the gate's row
+      slots_sum<T, L>(sg, comb, C, [&](int c, float v) { a.d_gate[g * C + c] = cpfn_from_f32<T>(v); });
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sg[i] = 0.f;
+    }
+  }
+  float *part = a.part + (size_t)blockIdx.x * nsums * C;
+  if (a.sums12) {
+    slots_sum<T, L>(s1, comb, C, [&](int c, float v) { part[c] = v; });
+    slots_sum<T, L>(s2, comb, C, [&](int c, float v) { part[C + c] = v; });
+  }
+  if (a.sums34) {
+    slots_sum<T, L>(s3, comb, C, [&](int c, float v) { part[2 * C + c] = v; });
+    slots_sum<T, L>(s4, comb, C, [&](int c, float v) { part[3 * C + c] = v; });
+  }
+  if (nsums == 5) slots_sum<T, L>(sg, comb, C, [&](int c, float v) { part[4 * C + c] = v; });
+}
+
+// The workgroups' sums -> gradients of the parameters (grid.y 0: S1, S2; 1: S3, S4) and of a shared gate (grid.y 2 + group).
+// 16 channels x 64 subsets of workgroups: subset q adds workgroups q, q + 64, ... in fp64, then the subsets are added in order.
+struct NormReduce {
+  const float *part;
+  int nblk, nsums, C, blocks_per_group;
+  const float *weight, *bias, *scale;
+  float *d_weight, *d_bias, *d_scale, *d_next_weight, *d_next_bias;
+  void *d_gate;
+  int wants12, wants34;
+};
+template <typename T> __global__ __launch_bounds__(1024) void norm_residual_reduce_kernel(const NormReduce a) {
+  __shared__ double acc[64][16][2];
+  const int c = blockIdx.x * 16 + (threadIdx.x & 15), q = threadIdx.x >> 4;
+  const bool gate = blockIdx.y >= 2;
+  if ((blockIdx.y == 0 && !a.wants12) || (blockIdx.y == 1 && !a.wants34)) return;
+  const int first = gate ? (int)(blockIdx.y - 2) * a.blocks_per_group : 0, last = gate ? first + a.blocks_per_group : a.nblk;
+  const int k = gate ? 4 : blockIdx.y * 2;
+  double t1 = 0.0, t2 = 0.0;
+  if (c < a.C) {
+#pragma unroll 4
+    for (int i = first + q; i < last; i += 64) {
+      const float *p = a.part + ((size_t)i * a.nsums + k) * a.C + c;
+      t1 += (double)p[0];
+      if (!gate) t2 += (double)p[a.C];
+    }
+  }
+  acc[q][threadIdx.x & 15][0] = t1;
+  acc[q][threadIdx.x & 15][1] = t2;
+  __syncthreads();
+  if (q != 0 || c >= a.C) return;
+  t1 = t2 = 0.0;
+#pragma unroll 8
+  for (int i = 0; i < 64; ++i) { t1 += acc[i][threadIdx.x][0]; t2 += acc[i][threadIdx.x][1]; }
+  if (gate) {
+    ((T *)a.d_gate)[(size_t)(blockIdx.y - 2) * a.C + c] = cpfn_from_f32<T>((float)t1);
+  } else if (blockIdx.y == 0) {
+    const double sc = a.scale ? (double)a.scale[c] : 1.0;
+    if (a.d_weight) a.d_weight[c] = (float)(sc * t1);
+    if (a.d_bias) a.d_bias[c] = (float)(sc * t2);
+    if (a.d_scale) a.d_scale[c] = (float)((a.weight ? (double)a.weight[c] : 1.0) * t1 + (a.bias ? (double)a.bias[c] * t2 : 0.0));
+  } else {
+    if (a.d_next_weight) a.d_next_weight[c] = (float)t1;
+    if (a.d_next_bias) a.d_next_bias[c] = (float)t2;
+  }
+}
+
+// How the rows are split over workgroups.
+struct NormSplit { long long groups, rows_per_gate, chunk; int nblk, blocks_per_group, groups_per_block; };
+NormSplit norm_split(long long P, int C, long long gate_rows) {
+  const int L = norm_lanes(C), threads = L <= 256 ? 256 : L, rows = threads / L;
+  const bool shared = gate_rows > 0 && gate_rows < P;
+  NormSplit s;
+  s.groups = shared ? gate_rows : 1;
+  s.rows_per_gate = P / s.groups;
+  const long long sets = (s.rows_per_gate + rows - 1) / rows;             // row sets of a group
+  const long long want = 768 * 256 / threads;                             // workgroups that are resident together
+  long long bpg = (want + s.groups - 1) / s.groups;
+  if (bpg > (sets + 3) / 4) bpg = (sets + 3) / 4;                         // (at least four row sets each: the sums have to be paid for)
+  if (bpg < 1) bpg = 1;
+  s.chunk = (sets + bpg - 1) / bpg * rows;
+  bpg = (s.rows_per_gate + s.chunk - 1) / s.chunk;
+  s.blocks_per_group = (int)bpg;
+  s.groups_per_block = 1;
+  if (bpg == 1) {
+    const long long per = (s.groups + want - 1) / want;
+    s.groups_per_block = (int)per;
+    s.nblk = (int)((s.groups + per - 1) / per);
+  } else {
+    s.nblk = (int)(bpg * s.groups);
+  }
+  return s;
+}
+
+template <typename T, int L> void launch(const NormBwd<T> &a, int nblk, hipStream_t st) {
+  norm_residual_bwd_kernel<T, L><<<nblk, NormShape<T, L>::THREADS, 0, st>>>(a);
+}
+
+struct Grads { float *d_weight, *d_bias, *d_scale, *d_next_weight, *d_next_bias; };
+
+template <typename T>
+int backward(const void *x, const void *y, const void *gate, const float *weight, const float *bias, const float *scale,
+             const float *next_weight, const void *d_out, const void *d_normed, long long P, int C, long long gate_rows, int layer,
+             int sigmoid, float eps, void *d_x, void *d_y, void *d_gate, const Grads &d, float *workspace, hipStream_t st) {
+  const NormSplit s = norm_split(P, C, gate_rows);
+  NormBwd<T> a;
+  a.x = (const T *)x; a.y = (const T *)y; a.gate = (const T *)gate; a.d_out = (const T *)d_out; a.d_normed = (const T *)d_normed;
+  a.weight = weight; a.bias = bias; a.scale = scale; a.next_weight = next_weight;
+  a.P = P; a.rows_per_gate = s.rows_per_gate; a.chunk = s.chunk; a.blocks_per_group = s.blocks_per_group;
+  a.groups_per_block = s.groups_per_block; a.groups = s.groups;
+  a.C = C; a.layer = layer; a.sigmoid = sigmoid; a.eps = eps;
+  a.d_x = (T *)d_x; a.d_y = (T *)d_y; a.d_gate = (T *)d_gate;
+  a.part = workspace;
+  a.shared_gate = gate && gate_rows < P;
+  a.sums12 = d.d_weight || d.d_bias || d.d_scale;
+  a.sums34 = d.d_next_weight || d.d_next_bias;
+  switch (norm_lanes(C)) {
+    case 8: launch<T, 8>(a, s.nblk, st); break;
+    case 16: launch<T, 16>(a, s.nblk, st); break;
+    case 32: launch<T, 32>(a, s.nblk, st); break;
+    case 64: launch<T, 64>(a, s.nblk, st); break;
+    case 128: launch<T, 128>(a, s.nblk, st); break;
+    case 256: launch<T, 256>(a, s.nblk, st); break;
+    default: launch<T, 512>(a, s.nblk, st); break;
+  }
+  const bool gate_part = a.shared_gate && d_gate && s.blocks_per_group > 1;
+  if (a.sums12 || a.sums34 || gate_part) {
+    NormReduce r;
+    r.part = workspace; r.nblk = s.nblk; r.nsums = 4 + (a.shared_gate && s.blocks_per_group > 1); r.C = C;
+    r.blocks_per_group = s.blocks_per_group;
+    r.weight = weight; r.bias = bias; r.scale = scale;
+    r.d_weight = d.d_weight; r.d_bias = d.d_bias; r.d_scale = d.d_scale; r.d_next_weight = d.d_next_weight; r.d_next_bias = d.d_next_bias;
+    r.d_gate = d_gate; r.wants12 = a.sums12; r.wants34 = a.sums34;
+    norm_residual_reduce_kernel<T><<<dim3(cpfn_cdiv(C, 16), 2 + (gate_part ? (unsigned)s.groups : 0)), 1024, 0, st>>>(r);
+  }
+  return cpfn_launch_status();
+}
+
+}  // namespace
+
+extern "C" long long cpfn_norm_residual_workspace(long long P, int C, long long gate_rows) {
+  if (P < 0 || C < 1 || C > CPFN_NORM_MAX_C || gate_rows < 0 || (gate_rows > 0 && P % gate_rows != 0)) return -1;
+  if (P == 0) return 0;
+  return (long long)norm_split(P, C, gate_rows).nblk * 5 * C * (long long)sizeof(float);
+}
+
+extern "C" int cpfn_norm_residual_bwd(const void *x, const void *y, const void *gate, const float *weight, const float *bias,
+                                      const float *scale, const float *next_weight, const void *d_out, const void *d_normed,
+                                      long long P, int C, long long gate_rows, int dtype, int layer, int sigmoid, float eps, void *d_x,
+                                      void *d_y, void *d_gate, float *d_weight, float *d_bias, float *d_scale, float *d_next_weight,
+                                      float *d_next_bias, void *workspace, void *stream) {
+  if (P < 0 || C < 1 || C > CPFN_NORM_MAX_C || !(eps >= 0.f) || (d_normed && (!next_weight || !x)) || (bias && !weight) ||
+      (!y && (gate || weight || scale || d_y || d_weight || d_scale)) || (d_weight && !weight) || (d_bias && !weight) ||
+      (d_scale && !scale) || ((d_next_weight || d_next_bias) && !d_normed) || (d_gate && !gate))
+    return CPFN_EINVAL;
+  if (gate && (gate_rows < 1 || P % gate_rows != 0)) return CPFN_EINVAL;
+  if (P == 0 || (!d_out && !d_normed) || !workspace) return CPFN_EINVAL;
+  const Grads d = {d_weight, d_bias, d_scale, d_next_weight, d_next_bias};
+  if (!gate) gate_rows = 0;
+  hipStream_t st = (hipStream_t)stream;
+  float *ws = (float *)workspace;
+  switch (dtype) {
+    case CPFN_F32: return backward<float>(x, y, gate, weight, bias, scale, next_weight, d_out, d_normed, P, C, gate_rows, layer, sigmoid, eps, d_x, d_y, d_gate, d, ws, st);
+    case CPFN_BF16: return backward<cpfn_bf16>(x, y, gate, weight, bias, scale, next_weight, d_out, d_normed, P, C, gate_rows, layer, sigmoid, eps, d_x, d_y, d_gate, d, ws, st);
+    case CPFN_F16: return backward<cpfn_f16>(x, y, gate, weight, bias, scale, next_weight, d_out, d_normed, P, C, gate_rows, layer, sigmoid, eps, d_x, d_y, d_gate, d, ws, st);
+  }
+  return CPFN_EINVAL;
+}

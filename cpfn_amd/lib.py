@@ -12,7 +12,7 @@ SO_PATH = os.path.join(_HERE, "libcpfn_hip.so")
 ABI_VERSION = 3          # = CPFN_ABI_VERSION of include/cpfn_hip.h; bumped whenever an exported signature changes
 
 _vp, _i, _f, _i64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_int64
-_ll = ctypes.c_longlong
+_ll, _d = ctypes.c_longlong, ctypes.c_double
 
 # name -> argtypes (restype is int unless listed in _RESTYPES); mirrors include/cpfn_hip.h
 SIGNATURES = {
@@ -152,9 +152,24 @@ SIGNATURES = {
     "cpfn_seg_stats_bwd": [_vp, _vp, _i, _i, _i, _vp, _vp],
     "cpfn_residue_fwd": [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp],
     "cpfn_residue_bwd": [_vp, _vp, _vp, _vp, _i, _i, _vp, _vp, _vp],
+    "cpfn_norm_residual_fwd": [_vp] * 8 + [_ll, _i, _ll, _i, _i, _i, _f, _vp, _vp, _vp],
+    "cpfn_norm_residual_workspace": [_ll, _i, _ll],
+    "cpfn_norm_residual_bwd": [_vp] * 9 + [_ll, _i, _ll, _i, _i, _i, _f] + [_vp] * 10,
+    "cpfn_route_workspace": [_ll, _i],
+    "cpfn_route_plan": [_vp, _i, _ll, _i, _vp, _vp, _vp, _vp],
+    "cpfn_route_gather": [_vp, _vp, _vp, _ll, _i, _i, _i, _i, _vp, _vp],
+    "cpfn_route_combine": [_vp, _vp, _vp, _ll, _i, _i, _i, _vp, _vp],
+    "cpfn_route_combine_bwd": [_vp, _vp, _vp, _vp, _vp, _ll, _i, _i, _i, _i, _vp, _vp, _vp],
+    "cpfn_grad_norm_workspace": [_vp, _i],
+    "cpfn_grad_norm": [_vp, _vp, _vp, _i, _i, _vp, _vp, _vp],
+    "cpfn_grad_clip": [_vp, _vp, _vp, _vp, _vp, _i, _i, _d, _vp, _vp, _vp],
+    "cpfn_grad_sumsq_blocks": [_ll],
+    "cpfn_grad_sumsq": [_vp, _ll, _vp, _vp],
+    "cpfn_adam_flat_clip": [_vp, _vp, _vp, _vp, _ll, _vp, _f, _f, _f, _f, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _d, _vp, _vp, _vp],
 }
 _RESTYPES = {"cpfn_build_info": ctypes.c_char_p, "cpfn_similarity_soft_workspace": ctypes.c_longlong,
-             "cpfn_metrics_workspace": ctypes.c_longlong}
+             "cpfn_metrics_workspace": ctypes.c_longlong, "cpfn_norm_residual_workspace": ctypes.c_longlong,
+             "cpfn_route_workspace": ctypes.c_longlong, "cpfn_grad_norm_workspace": ctypes.c_longlong}
 
 _lib = None
 _raw = None

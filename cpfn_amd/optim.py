@@ -5,11 +5,128 @@ builds `optim.Adam(spfn_module.parameters(), lr=...)`, training_SPFN.py; torch/o
 every parameter at a view of ONE contiguous fp32 buffer and reads the gradients from the trainer's
 FlatGradBucket, so a step is a single launch over 1.4 M elements instead of a multi-tensor launch over ~100
 tensors.  Capturable: learning rate, step count and `found_inf` (set it before `step()` to skip on non-finite
-gradients) are device scalars.  GPU only — on CPU the trainer keeps torch.optim.Adam."""
+gradients) are device scalars.  GPU only — on CPU the trainer keeps torch.optim.Adam.
+
+`grad_norm`, `clip_grads_` and `clip_grad_norm_` take any list of gradients (csrc/gradnorm.hip): the norm over all of them and their
+clipping, in two launches for up to 128 tensors; `FlatAdam.step(max_grad_norm=...)` clips what it reads from the flat buffer."""
+import ctypes
+
 import torch
 
 from . import lib as _l
-from .ops import _ptr, _stream
+from .ops import ROW_DTYPES, _ptr, _stream
+
+_NORMS = {1.0: 1, 2.0: 2, float("inf"): 0}
+
+
+def _dense(t):
+    """Do t's elements fill one stretch of memory, in whatever order of the dimensions?"""
+    if t.is_contiguous():
+        return True
+    expected = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
+        if stride != expected:
+            return False
+        expected *= size
+    return True
+
+
+def _gradient_table(grads, name="grads"):
+    """Checks a list of gradients -> (pointers, lengths, types) as ctypes arrays."""
+    dev = grads[0].device
+    for t in grads:
+        if not isinstance(t, torch.Tensor):
+            raise RuntimeError("%s must be tensors" % name)
+        if not t.is_cuda:
+            raise RuntimeError("%s must be CUDA(HIP) tensors: CPU not supported" % name)
+        if t.device != dev:
+            raise RuntimeError("%s must be on one device (got %s and %s)" % (name, dev, t.device))
+        if t.dtype not in ROW_DTYPES:
+            raise RuntimeError("%s must be float32, bfloat16 or float16 tensors (got %s)" % (name, t.dtype))
+        if t.layout != torch.strided or not _dense(t):
+            raise RuntimeError("%s must be dense and without overlap (got strides %s for shape %s)" % (name, t.stride(), tuple(t.shape)))
+    k = len(grads)
+    return ((ctypes.c_void_p * k)(*[t.data_ptr() for t in grads]), (ctypes.c_longlong * k)(*[t.numel() for t in grads]),
+            (ctypes.c_int * k)(*[ROW_DTYPES[t.dtype] for t in grads]))
+
+
+def _list_of(grads):
+    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    if any(not isinstance(t, torch.Tensor) for t in grads):
+        raise RuntimeError("gradients must be tensors")
+    return grads
+
+
+def _norm_code(norm_type):
+    p = _NORMS.get(float(norm_type))
+    if p is None:
+        raise RuntimeError("norm_type must be 1, 2 or inf (got %r)" % (norm_type,))
+    return p
+
+
+@torch.no_grad()
+def grad_norm(grads, norm_type=2.0):
+    """The norm over all values of a list of tensors (fp32, bf16 and fp16 together; any lengths) -> 0-dim fp32 tensor on their device,
+    without a host synchronisation.  norm_type 1, 2 or inf; fp64 sums in a fixed order (bit-reproducible); NaN if any value is NaN."""
+    grads, p = _list_of(grads), _norm_code(norm_type)
+    if not grads:
+        return torch.zeros(())
+    ptr, n, types = _gradient_table(grads)
+    h, dev = _l.lib(), grads[0].device
+    with torch.cuda.device(dev):
+        norm = torch.empty((), dtype=torch.float32, device=dev)
+        ws = torch.empty(h.cpfn_grad_norm_workspace(n, len(grads)) // 8, dtype=torch.float64, device=dev)
+        _l.check(h.cpfn_grad_norm(ptr, n, types, len(grads), p, _ptr(norm), _ptr(ws), _stream()), "cpfn_grad_norm")
+    _l.add_bytes("cpfn_grad_norm", sum(t.numel() * t.element_size() for t in grads))
+    return norm
+
+
+@torch.no_grad()
+def clip_grads_(grads, max_norm, norm_type=2.0, out=None):
+    """grads *= min(1, max_norm / (norm + 1e-6)) with the norm of grad_norm -> that norm (before clipping, on the device).  Nothing is
+    synchronised, and in place nothing is written where the factor is 1.  out: tensors of the same shapes, of the gradients' types or
+    fp32 (master gradients), that take the result instead; a gradient listed twice, or memory shared with a tensor that is written, is
+    refused.  An infinite norm gives the factor 0 and a NaN one NaN, as the formula has it."""
+    grads, p, max_norm = _list_of(grads), _norm_code(norm_type), float(max_norm)
+    if not max_norm >= 0.0:
+        raise RuntimeError("max_norm must not be negative (got %r)" % max_norm)
+    outs = None if out is None else _list_of(out)
+    if outs is not None and len(outs) != len(grads):
+        raise RuntimeError("out must have a tensor for each gradient (got %d for %d)" % (len(outs), len(grads)))
+    if not grads:
+        return torch.zeros(())
+    ptr, n, types = _gradient_table(grads)
+    h, dev, optr, otypes = _l.lib(), grads[0].device, None, None
+    if outs is not None:
+        for g, o in zip(grads, outs):
+            if o.shape != g.shape or o.device != dev or (o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous())):
+                raise RuntimeError("out must have the gradients' shapes, order of dimensions and device")
+            if o.dtype != g.dtype and o.dtype != torch.float32:
+                raise RuntimeError("out must be of the gradient's type or float32 (got %s for %s)" % (o.dtype, g.dtype))
+        optr, _, otypes = _gradient_table(outs, "out")
+    with torch.cuda.device(dev):
+        norm = torch.empty((), dtype=torch.float32, device=dev)
+        ws = torch.empty(h.cpfn_grad_norm_workspace(n, len(grads)) // 8, dtype=torch.float64, device=dev)
+        status = h.cpfn_grad_clip(ptr, optr, n, types, otypes, len(grads), p, max_norm, _ptr(norm), _ptr(ws), _stream())
+        if status == -22:
+            raise RuntimeError("a tensor that is written shares memory with another one of the lists (a gradient listed twice?)")
+        _l.check(status, "cpfn_grad_clip")
+    _l.add_bytes("cpfn_grad_clip", sum(t.numel() * t.element_size() for t in grads + (outs or grads)))
+    return norm
+
+
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
+    """torch.nn.utils.clip_grad_norm_ on clip_grads_: clips the .grad of the parameters that have one, in place -> their norm before.
+    error_if_nonfinite reads the norm on the host first (a synchronisation and another pass over the gradients; not inside a capture) and
+    raises before anything is scaled."""
+    grads = [p.grad for p in _list_of(parameters) if p.grad is not None]
+    if error_if_nonfinite and grads:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("error_if_nonfinite reads the norm on the host: not inside a stream capture")
+        norm = float(grad_norm(grads, norm_type))
+        if not norm < float("inf"):
+            raise RuntimeError("the norm of the gradients is %r: not clipped" % norm)
+    return clip_grads_(grads, max_norm, norm_type)
 
 
 class FlatAdam(torch.optim.Optimizer):
@@ -36,17 +153,19 @@ class FlatAdam(torch.optim.Optimizer):
         self.exp_avg_sq = torch.zeros(n, dtype=torch.float32, device=dev)
         self.step_count = torch.zeros((), dtype=torch.float32, device=dev)
         self.lr_dev = torch.zeros((), dtype=torch.float32, device=dev)
-        self._coef = torch.zeros(3, dtype=torch.float32, device=dev)
+        self._coef = torch.zeros(4, dtype=torch.float32, device=dev)
         self.beta_pows = torch.ones(2, dtype=torch.float64, device=dev)      # beta1^step, beta2^step
         self._lr_host = None
         self.found_inf = None
         self._nf_ws = None
+        self.grad_norm = torch.zeros((), dtype=torch.float32, device=dev)     # before clipping, of the last step(max_grad_norm=...)
+        self._parts = torch.empty(max(1, _l.lib().cpfn_grad_sumsq_blocks(n)), dtype=torch.float64, device=dev)
         g = self.param_groups[0]
         g["lr"] = self.lr_dev                      # the trainer's staircase does `group['lr'].fill_(lr)`
         self.lr_dev.fill_(float(lr))
 
     @torch.no_grad()
-    def step(self, closure=None, check_gradients=False, skipped=None, nf_flags=None, combine=None):
+    def step(self, closure=None, check_gradients=False, skipped=None, nf_flags=None, combine=None, max_grad_norm=None):
         """check_gradients: scan the flat gradient for NaN / inf in the same launch sequence and skip the step if any
         is found (the reference's per-parameter isinf/isnan scan, Utils/training_utils.py:151-156) — the scan's final
         reduction and the optional `skipped` device counter (+1 per skipped step) live in the 1-wave prepare kernel.
@@ -54,7 +173,17 @@ class FlatAdam(torch.optim.Optimizer):
         copy of FlatGradBucket.collect); the step is skipped if any of them is set.  The first n_sticky words are OR-ed into by
         the launches that wrote the gradients (fused_mlp.GradSink) and are cleared by this step's prepare kernel.
         combine = (S [7 C], coef [3, C], C, out [C, 3] — a slice of the flat gradient): the pass's last gradient, finished (and
-        checked) by the prepare kernel (fused_mlp.GradSink.combine, cpfn_adam_flat_xw)."""
+        checked) by the prepare kernel (fused_mlp.GradSink.combine, cpfn_adam_flat_xw).
+        max_grad_norm: step on the gradients times min(1, max_grad_norm / (norm + 1e-6)), norm = the 2-norm over the whole bucket (left in
+        `self.grad_norm`, a 0-dim device tensor); the factor is applied as the step reads the gradients, which stay as they are in the
+        bucket.  A norm that is not finite skips the step like check_gradients does.  Not together with `combine` (that gradient is not
+        finished when the norm is taken)."""
+        if max_grad_norm is not None:
+            max_grad_norm = float(max_grad_norm)
+            if not max_grad_norm >= 0.0:
+                raise RuntimeError("max_grad_norm must not be negative (got %r)" % max_grad_norm)
+            if combine is not None:
+                raise RuntimeError("max_grad_norm needs finished gradients: not together with combine")
         g = self.param_groups[0]
         lr = g["lr"]
         if not isinstance(lr, torch.Tensor):       # someone assigned a float: mirror it into the device scalar
@@ -70,11 +199,19 @@ class FlatAdam(torch.optim.Optimizer):
             if nf_flags is not None:
                 nf_ws, nf_count = nf_flags[0], nf_flags[1]
                 n_sticky = nf_flags[2] if len(nf_flags) > 2 else 0       # words OR-ed into by the gradients' writers: cleared here
-            elif check_gradients:
+            elif check_gradients and max_grad_norm is None:
                 if self._nf_ws is None:
                     self._nf_ws = torch.empty(256, dtype=torch.int32, device=self.flat_p.device)
                 nf_ws, nf_count = self._nf_ws, h.cpfn_nonfinite_blocks(grads.numel())
                 _l.check(h.cpfn_nonfinite_partial(_ptr(grads), grads.numel(), _ptr(nf_ws), _stream()), "cpfn_nonfinite_partial")
+            if max_grad_norm is not None:
+                _l.check(h.cpfn_adam_flat_clip(_ptr(self.flat_p), _ptr(grads), _ptr(self.exp_avg), _ptr(self.exp_avg_sq),
+                                               self.flat_p.numel(), _ptr(lr), float(b1), float(b2), float(g["eps"]),
+                                               float(g["weight_decay"]), _ptr(self.step_count), _ptr(self.beta_pows),
+                                               _ptr(self.found_inf), _ptr(self._coef), _ptr(nf_ws), nf_count, n_sticky, _ptr(skipped),
+                                               max_grad_norm, _ptr(self._parts), _ptr(self.grad_norm), _stream()), "cpfn_adam_flat_clip")
+                _l.add_bytes("cpfn_adam_flat_clip", 32 * self.flat_p.numel())
+                return
             xS, xc, xC, xo = combine if combine is not None else (None, None, 0, None)
             _l.check(h.cpfn_adam_flat_xw(_ptr(self.flat_p), _ptr(grads), _ptr(self.exp_avg), _ptr(self.exp_avg_sq),
                                          self.flat_p.numel(), _ptr(lr), float(b1), float(b2), float(g["eps"]),

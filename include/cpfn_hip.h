@@ -829,6 +829,71 @@ CPFN_API int cpfn_similarity_soft(const float *spfn_labels, const float *predict
 CPFN_API int cpfn_label_pool(const float *M, const int64_t *labels, long long N, int C, int G, void *workspace,
                              float *out, void *stream);
 
+/* ------------------------------------------------------------------ norms around a residual block
+ * Rows [P, C] (C <= 4096, contiguous, any alignment of the element type) of `dtype`; parameters fp32; all arithmetic fp32, one rounding
+ * at each store.  No reference counterpart.
+ *   n(v; w, b) = (v - mu) / sqrt(mean((v - mu)^2) + eps) * w + b over the C channels, mu = mean(v) if layer != 0, else 0
+ *   u = n(y; weight, bias), or y if weight is NULL;   a = gate, sigmoid(gate) (sigmoid != 0), or 1 (NULL)
+ *   out = x + scale * a * u (scale NULL: 1);          normed = n(out; next_weight, next_bias), of the unrounded sum
+ * gate: [gate_rows, C], gate_rows dividing P: P / gate_rows consecutive rows share one (a gate for each cloud).  normed NULL: not formed.
+ * y NULL: normed = n(x; next_weight, next_bias) alone (out is not written).  bias / next_bias NULL: 0. */
+#define CPFN_F32 0
+#define CPFN_BF16 1
+#define CPFN_F16 2
+CPFN_API int cpfn_norm_residual_fwd(const void *x, const void *y, const void *gate, const float *weight, const float *bias,
+                                    const float *scale, const float *next_weight, const float *next_bias, long long P, int C,
+                                    long long gate_rows, int dtype, int layer, int sigmoid, float eps, void *out, void *normed,
+                                    void *stream);
+/* The backward pass from the forward pass's inputs: d_out / d_normed (either may be NULL: no gradient) -> d_x, d_y, d_gate (shape of the
+ * gate) and the parameters' fp32 gradients, each optional.  Fixed summation orders.  workspace: cpfn_norm_residual_workspace bytes
+ * (gate_rows 0 without a gate), 8-byte aligned; P >= 1. */
+CPFN_API long long cpfn_norm_residual_workspace(long long P, int C, long long gate_rows);
+CPFN_API int cpfn_norm_residual_bwd(const void *x, const void *y, const void *gate, const float *weight, const float *bias,
+                                    const float *scale, const float *next_weight, const void *d_out, const void *d_normed, long long P,
+                                    int C, long long gate_rows, int dtype, int layer, int sigmoid, float eps, void *d_x, void *d_y,
+                                    void *d_gate, float *d_weight, float *d_bias, float *d_scale, float *d_next_weight,
+                                    float *d_next_bias, void *workspace, void *stream);
+
+/* ------------------------------------------------------------------ rows sorted by expert and back
+ * choice[n] (int32, or int64 if wide != 0): an expert index for each choice, n = R k in row order; E <= 2048.  A stable counting sort:
+ * offsets[E + 1] = first position of each expert, place[n] = position of each choice among all sorted ones, -1 for an index outside
+ * [0, E) (a choice that is not routed).  workspace: cpfn_route_workspace bytes.  No reference counterpart. */
+CPFN_API long long cpfn_route_workspace(long long n, int E);
+CPFN_API int cpfn_route_plan(const void *choice, int wide, long long n, int E, int *offsets, int *place, void *workspace, void *stream);
+/* out[place[r, j]] = rows[r] for every routed choice, out [R k, C]; its rows behind offsets[E] are zero. */
+CPFN_API int cpfn_route_gather(const void *rows, const int *place, const int *offsets, long long R, int k, int E, int C, int dtype,
+                               void *out, void *stream);
+/* out[r] = sum over j of weights[r, j] sorted[place[r, j]] (weights NULL: 1, the adjoint of cpfn_route_gather); a choice that is not
+ * routed adds nothing.  fp32 sums in the order of j. */
+CPFN_API int cpfn_route_combine(const void *sorted, const float *weights, const int *place, long long R, int k, int C, int dtype,
+                                void *out, void *stream);
+/* The adjoint of cpfn_route_combine for the gradient g [R, C]: d_sorted[place[r, j]] = weights[r, j] g[r] (zero behind offsets[E]) and
+ * d_weights[r, j] = <g[r], sorted[place[r, j]]> (zero where not routed); either may be NULL. */
+CPFN_API int cpfn_route_combine_bwd(const void *g, const void *sorted, const float *weights, const int *place, const int *offsets,
+                                    long long R, int k, int E, int C, int dtype, void *d_sorted, float *d_weights, void *stream);
+
+/* ------------------------------------------------------------------ the norm of many gradients, and clipping
+ * HOST arrays of `count` device pointers, lengths and types (CPFN_F32 / BF16 / F16; contiguous, any alignment of the type).
+ * norm[0] (fp32, device) = (sum |g|^p)^(1/p) over all of them, p = 1, 2, or 0 for the largest |g|; fp64 sums in a fixed order.
+ * workspace: cpfn_grad_norm_workspace bytes, 8-byte aligned.  No reference counterpart. */
+CPFN_API long long cpfn_grad_norm_workspace(const long long *n, int count);
+CPFN_API int cpfn_grad_norm(const void *const *grads, const long long *n, const int *type, int count, int p, float *norm, void *workspace,
+                            void *stream);
+/* ... and out[i] = min(1, max_norm / (norm + 1e-6)) grads[i].  out NULL: in place; else tensors of the same type or fp32 (out_type).
+ * A tensor that is written may share memory with no other one of the lists (refused), except that out[i] may be grads[i]. */
+CPFN_API int cpfn_grad_clip(const void *const *grads, void *const *out, const long long *n, const int *type, const int *out_type, int count,
+                            int p, double max_norm, float *norm, void *workspace, void *stream);
+/* The sums of squares of cpfn_grad_sumsq_blocks(n) workgroups over one fp32 tensor. */
+CPFN_API int cpfn_grad_sumsq_blocks(long long n);
+CPFN_API int cpfn_grad_sumsq(const float *g, long long n, double *parts, void *stream);
+/* cpfn_adam_flat_sticky on gradients clipped to max_norm (2-norm over the whole of g; g itself is not changed): parts = scratch for
+ * cpfn_grad_sumsq_blocks(n) doubles, coef4 = 4 floats of scratch, norm[0] = the norm before clipping.  A norm that is not finite skips the
+ * step. */
+CPFN_API int cpfn_adam_flat_clip(float *p, const float *g, float *m, float *v, long long n, const float *lr, float beta1, float beta2,
+                                 float eps, float weight_decay, float *step, double *pows, const float *found_inf, float *coef4,
+                                 unsigned *nf_partial, int nf_count, int n_sticky, float *skipped, double max_norm, double *parts,
+                                 float *norm, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
