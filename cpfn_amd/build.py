@@ -18,6 +18,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(CSRC, "build")
 SO = os.path.join(HERE, "libcpfn_hip.so")
+TABLES = os.path.join(HERE, "_tables.so")
 ARCH = "gfx950"
 
 # no packed fp32 instructions at all (v_pk_{add,mul,fma}_f32 have given wrong results on this hardware now and then)
@@ -140,11 +141,31 @@ def _check_isa(src):
             os.remove(os.path.join(OBJ, f))
 
 
+def _build_tables(force):
+    """_tables.so (csrc/tables.cpp): a CPython extension over torch's own headers; host code only."""
+    import sysconfig
+    src = os.path.join(CSRC, "tables.cpp")
+    if not force and not _stale(TABLES, [src]):
+        return
+    import torch
+    from torch.utils.cpp_extension import include_paths
+    cmd = ["g++", "-O2", "-fPIC", "-shared", "-std=c++17", "-fvisibility=hidden", "-Wall",
+           "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI, "-I" + sysconfig.get_paths()["include"]]
+    for d in include_paths():
+        cmd += ["-isystem", d]
+    cmd += [src, "-o", TABLES, "-L" + os.path.join(os.path.dirname(torch.__file__), "lib"), "-lc10", "-ltorch_cpu", "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("g++ failed for tables.cpp:\n%s" % r.stderr[-4000:])
+
+
 def build(force=False, verbose=False):
     os.makedirs(OBJ, exist_ok=True)
     srcs = {s: f for s, f in SOURCES.items() if os.path.exists(os.path.join(CSRC, s))}
     with ThreadPoolExecutor(max_workers=min(6, len(srcs))) as ex:
+        tables = ex.submit(_build_tables, force)
         res = list(ex.map(lambda kv: _compile(kv[0], kv[1], force), srcs.items()))
+        tables.result()
     objs = [o for o, _ in res]
     if force or any(c for _, c in res) or _stale(SO, objs):
         cmd = [_hipcc(), "--offload-arch=" + ARCH, "-shared", "-fPIC", "-o", SO] + objs

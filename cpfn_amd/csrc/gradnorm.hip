@@ -293,7 +293,7 @@ extern "C" int cpfn_grad_clip(const void *const *grads, void *const *out, const 
   void *const *dst = out ? out : (void *const *)grads;
   const int *to = out ? out_type : type;
   try {
-    if (overlapping(grads, dst, n, type, to, count)) return CPFN_EINVAL;
+    if (overlapping(grads, dst, n, type, to, count)) return CPFN_EOVERLAP;
   } catch (...) {
     return CPFN_EINVAL;
   }

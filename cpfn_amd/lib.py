@@ -205,6 +205,11 @@ def add_bytes(name, nbytes):
         ent[1] += int(nbytes)
 
 
+def counting():
+    """Is anybody counting algorithmic bytes?  (For callers whose sum takes longer than asking.)"""
+    return _census is not None or bool(_bytes)
+
+
 def timed_bytes(name):
     return _bytes.get(name, 0)
 
@@ -290,4 +295,5 @@ def lib():
 def check(status, what):
     if status != 0:
         raise CpfnHipError("%s failed with status %d%s" % (
-            what, status, " (invalid argument)" if status == -22 else " (hipError_t)"))
+            what, status, {-22: " (invalid argument)", -16: " (a tensor that is written shares memory with another one of the lists: "
+                           "a gradient listed twice?)"}.get(status, " (hipError_t)")))

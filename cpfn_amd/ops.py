@@ -407,6 +407,18 @@ _KINDS = {"rms": 0, "layer": 1}
 _GATE_ACTS = {"none": 0, "sigmoid": 1}
 
 
+def _launch(name, device, *args):
+    """One call of a C-ABI entry point on the current stream of the tensors' device."""
+    fn, i = getattr(_l.lib(), name), device.index
+    if i == torch._C._cuda_getDevice():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    else:
+        with torch.cuda.device(i):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    if status:
+        _l.check(status, name)
+
+
 def _chk_rows(t, name, like=None):
     """rows [P, C] of fp32 / bf16 / fp16 (like: of the same type, on the same device)."""
     if not isinstance(t, torch.Tensor):
@@ -470,13 +482,12 @@ def norm_residual_fwd(x, y, weight=None, bias=None, gate=None, gate_act="none", 
     normed = torch.empty_like(x) if next_weight is not None else None
     if P == 0:
         return out, normed
-    with torch.cuda.device(x.device):
-        _l.check(_l.lib().cpfn_norm_residual_fwd(_ptr(x), _ptr(y), _ptr(gate), _ptr(weight), _ptr(bias), _ptr(scale), _ptr(next_weight),
-                                                 _ptr(next_bias), P, C, 0 if gate is None else gate.shape[0], ROW_DTYPES[x.dtype],
-                                                 _KINDS[kind], _GATE_ACTS[gate_act], eps, _ptr(out), _ptr(normed), _stream()),
-                 "cpfn_norm_residual_fwd")
-    _l.add_bytes("cpfn_norm_residual_fwd", x.element_size() * (P * C * (1 + 2 * (y is not None) + (normed is not None))
-                                                               + (0 if gate is None else gate.numel())))
+    _launch("cpfn_norm_residual_fwd", x.device, _ptr(x), _ptr(y), _ptr(gate), _ptr(weight), _ptr(bias), _ptr(scale), _ptr(next_weight),
+            _ptr(next_bias), P, C, 0 if gate is None else gate.shape[0], ROW_DTYPES[x.dtype], _KINDS[kind], _GATE_ACTS[gate_act], eps,
+            _ptr(out), _ptr(normed))
+    if _l.counting():
+        _l.add_bytes("cpfn_norm_residual_fwd", x.element_size() * (P * C * (1 + 2 * (y is not None) + (normed is not None))
+                                                                   + (0 if gate is None else gate.numel())))
     return out, normed
 
 
@@ -508,19 +519,16 @@ def norm_residual_bwd(x, y, weight, bias, gate, gate_act, scale, next_weight, d_
         got.update(zip(vectors, (torch.zeros if P == 0 else torch.empty)(len(vectors), C, dtype=torch.float32, device=dev).unbind(0)))
     if P == 0 or not got:
         return got
-    h = _l.lib()
     G = 0 if gate is None else gate.shape[0]
-    with torch.cuda.device(dev):
-        ws = torch.empty(h.cpfn_norm_residual_workspace(P, C, G) // 4, dtype=torch.float32, device=dev)
-        p = {n: t.data_ptr() for n, t in got.items()}.get
-        _l.check(h.cpfn_norm_residual_bwd(_ptr(x), _ptr(y), _ptr(gate), _ptr(weight), _ptr(bias), _ptr(scale),
-                                          _ptr(next_weight), _ptr(d_out), _ptr(d_normed), P, C, G,
-                                          ROW_DTYPES[x.dtype], _KINDS[kind], _GATE_ACTS[gate_act], eps, p("x"), p("y"), p("gate"),
-                                          p("weight"), p("bias"), p("scale"), p("next_weight"), p("next_bias"), _ptr(ws), _stream()),
-                 "cpfn_norm_residual_bwd")
-    _l.add_bytes("cpfn_norm_residual_bwd", x.element_size() * (P * C * (sum(t is not None for t in (y, d_out)) + 2 * (d_normed is not None)
-                                                                        + ("x" in got) + ("y" in got)) + (0 if gate is None else gate.numel())
-                                                               + (got["gate"].numel() if "gate" in got else 0)))
+    ws = torch.empty(_l.lib().cpfn_norm_residual_workspace(P, C, G) // 4, dtype=torch.float32, device=dev)
+    p = {n: t.data_ptr() for n, t in got.items()}.get
+    _launch("cpfn_norm_residual_bwd", dev, _ptr(x), _ptr(y), _ptr(gate), _ptr(weight), _ptr(bias), _ptr(scale), _ptr(next_weight),
+            _ptr(d_out), _ptr(d_normed), P, C, G, ROW_DTYPES[x.dtype], _KINDS[kind], _GATE_ACTS[gate_act], eps, p("x"), p("y"), p("gate"),
+            p("weight"), p("bias"), p("scale"), p("next_weight"), p("next_bias"), ws.data_ptr())
+    if _l.counting():
+        full = sum(t is not None for t in (y, d_out)) + 2 * (d_normed is not None) + ("x" in got) + ("y" in got)
+        _l.add_bytes("cpfn_norm_residual_bwd", x.element_size() * (P * C * full + (0 if gate is None else gate.numel())
+                                                                   + (got["gate"].numel() if "gate" in got else 0)))
     return got
 
 
@@ -553,12 +561,9 @@ def route_plan(choice, n_experts):
     dev = choice.device
     offsets = torch.empty(E + 1, dtype=torch.int32, device=dev)
     place = torch.empty(choice.shape, dtype=torch.int32, device=dev)
-    h = _l.lib()
-    with torch.cuda.device(dev):
-        nws = h.cpfn_route_workspace(n, E)
-        ws = torch.empty(nws // 4, dtype=torch.int32, device=dev) if nws else None
-        _l.check(h.cpfn_route_plan(_ptr(choice), 1 if choice.dtype == torch.int64 else 0, n, E, _ptr(offsets), _ptr(place), _ptr(ws),
-                                   _stream()), "cpfn_route_plan")
+    nws = _l.lib().cpfn_route_workspace(n, E)
+    ws = torch.empty(nws // 4, dtype=torch.int32, device=dev) if nws else None
+    _launch("cpfn_route_plan", dev, _ptr(choice), 1 if choice.dtype == torch.int64 else 0, n, E, _ptr(offsets), _ptr(place), _ptr(ws))
     _l.add_bytes("cpfn_route_plan", (choice.element_size() + 4) * n + 4 * (E + 1))
     return RoutePlan(offsets, place, E)
 
@@ -590,9 +595,8 @@ def route_gather_fwd(rows, plan):
     out = torch.empty(R * k, C, dtype=rows.dtype, device=rows.device)
     if R == 0:
         return out
-    with torch.cuda.device(rows.device):
-        _l.check(_l.lib().cpfn_route_gather(_ptr(rows), _ptr(plan.place), _ptr(plan.offsets), R, k, plan.n_experts, C,
-                                            ROW_DTYPES[rows.dtype], _ptr(out), _stream()), "cpfn_route_gather")
+    _launch("cpfn_route_gather", rows.device, _ptr(rows), _ptr(plan.place), _ptr(plan.offsets), R, k, plan.n_experts, C,
+            ROW_DTYPES[rows.dtype], _ptr(out))
     _l.add_bytes("cpfn_route_gather", rows.element_size() * (R + R * k) * C + 4 * R * k)
     return out
 
@@ -607,9 +611,8 @@ def route_combine_fwd(sorted_rows, weights, plan):
     out = torch.empty(R, C, dtype=sorted_rows.dtype, device=sorted_rows.device)
     if R == 0:
         return out
-    with torch.cuda.device(sorted_rows.device):
-        _l.check(_l.lib().cpfn_route_combine(_ptr(sorted_rows), _ptr(weights), _ptr(plan.place), R, k, C, ROW_DTYPES[sorted_rows.dtype],
-                                             _ptr(out), _stream()), "cpfn_route_combine")
+    _launch("cpfn_route_combine", sorted_rows.device, _ptr(sorted_rows), _ptr(weights), _ptr(plan.place), R, k, C,
+            ROW_DTYPES[sorted_rows.dtype], _ptr(out))
     _l.add_bytes("cpfn_route_combine", sorted_rows.element_size() * (R + R * k) * C + (4 if weights is None else 8) * R * k)
     return out
 
@@ -632,9 +635,7 @@ def route_combine_bwd(grad_out, sorted_rows, weights, plan, need_rows=True, need
     d_weights = torch.empty(R, k, dtype=torch.float32, device=dev) if need_weights else None
     if R == 0:
         return d_sorted, d_weights
-    with torch.cuda.device(dev):
-        _l.check(_l.lib().cpfn_route_combine_bwd(_ptr(grad_out), _ptr(sorted_rows) if need_weights else None, _ptr(weights), _ptr(plan.place),
-                                                 _ptr(plan.offsets), R, k, plan.n_experts, C, ROW_DTYPES[grad_out.dtype], _ptr(d_sorted),
-                                                 _ptr(d_weights), _stream()), "cpfn_route_combine_bwd")
+    _launch("cpfn_route_combine_bwd", dev, _ptr(grad_out), _ptr(sorted_rows) if need_weights else None, _ptr(weights), _ptr(plan.place),
+            _ptr(plan.offsets), R, k, plan.n_experts, C, ROW_DTYPES[grad_out.dtype], _ptr(d_sorted), _ptr(d_weights))
     _l.add_bytes("cpfn_route_combine_bwd", grad_out.element_size() * (R + R * k * (need_rows + need_weights)) * C + 12 * R * k)
     return d_sorted, d_weights

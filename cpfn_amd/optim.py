@@ -9,52 +9,21 @@ gradients) are device scalars.  GPU only — on CPU the trainer keeps torch.opti
 
 `grad_norm`, `clip_grads_` and `clip_grad_norm_` take any list of gradients (csrc/gradnorm.hip): the norm over all of them and their
 clipping, in two launches for up to 128 tensors; `FlatAdam.step(max_grad_norm=...)` clips what it reads from the flat buffer."""
-import ctypes
-
 import torch
 
 from . import lib as _l
-from .ops import ROW_DTYPES, _ptr, _stream
+from .ops import _launch, _ptr, _stream
+
+try:
+    from . import _tables               # (csrc/tables.cpp)
+except ImportError as e:
+    raise ImportError("cpfn_amd/_tables.so is not built: run `python -m cpfn_amd.build` (%s)" % e) from e
 
 _NORMS = {1.0: 1, 2.0: 2, float("inf"): 0}
 
 
-def _dense(t):
-    """Do t's elements fill one stretch of memory, in whatever order of the dimensions?"""
-    if t.is_contiguous():
-        return True
-    expected = 1
-    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
-        if stride != expected:
-            return False
-        expected *= size
-    return True
-
-
-def _gradient_table(grads, name="grads"):
-    """Checks a list of gradients -> (pointers, lengths, types) as ctypes arrays."""
-    dev = grads[0].device
-    for t in grads:
-        if not isinstance(t, torch.Tensor):
-            raise RuntimeError("%s must be tensors" % name)
-        if not t.is_cuda:
-            raise RuntimeError("%s must be CUDA(HIP) tensors: CPU not supported" % name)
-        if t.device != dev:
-            raise RuntimeError("%s must be on one device (got %s and %s)" % (name, dev, t.device))
-        if t.dtype not in ROW_DTYPES:
-            raise RuntimeError("%s must be float32, bfloat16 or float16 tensors (got %s)" % (name, t.dtype))
-        if t.layout != torch.strided or not _dense(t):
-            raise RuntimeError("%s must be dense and without overlap (got strides %s for shape %s)" % (name, t.stride(), tuple(t.shape)))
-    k = len(grads)
-    return ((ctypes.c_void_p * k)(*[t.data_ptr() for t in grads]), (ctypes.c_longlong * k)(*[t.numel() for t in grads]),
-            (ctypes.c_int * k)(*[ROW_DTYPES[t.dtype] for t in grads]))
-
-
 def _list_of(grads):
-    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
-    if any(not isinstance(t, torch.Tensor) for t in grads):
-        raise RuntimeError("gradients must be tensors")
-    return grads
+    return [grads] if isinstance(grads, torch.Tensor) else list(grads)
 
 
 def _norm_code(norm_type):
@@ -71,13 +40,12 @@ def grad_norm(grads, norm_type=2.0):
     grads, p = _list_of(grads), _norm_code(norm_type)
     if not grads:
         return torch.zeros(())
-    ptr, n, types = _gradient_table(grads)
-    h, dev = _l.lib(), grads[0].device
-    with torch.cuda.device(dev):
-        norm = torch.empty((), dtype=torch.float32, device=dev)
-        ws = torch.empty(h.cpfn_grad_norm_workspace(n, len(grads)) // 8, dtype=torch.float64, device=dev)
-        _l.check(h.cpfn_grad_norm(ptr, n, types, len(grads), p, _ptr(norm), _ptr(ws), _stream()), "cpfn_grad_norm")
-    _l.add_bytes("cpfn_grad_norm", sum(t.numel() * t.element_size() for t in grads))
+    dev, nbytes, ptr, n, types, _, _ = _tables.gradients(grads, None)
+    dev = torch.device("cuda", dev)
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    ws = torch.empty(_l.lib().cpfn_grad_norm_workspace(n, len(grads)) // 8, dtype=torch.float64, device=dev)
+    _launch("cpfn_grad_norm", dev, ptr, n, types, len(grads), p, norm.data_ptr(), ws.data_ptr())
+    _l.add_bytes("cpfn_grad_norm", nbytes)
     return norm
 
 
@@ -91,27 +59,14 @@ def clip_grads_(grads, max_norm, norm_type=2.0, out=None):
     if not max_norm >= 0.0:
         raise RuntimeError("max_norm must not be negative (got %r)" % max_norm)
     outs = None if out is None else _list_of(out)
-    if outs is not None and len(outs) != len(grads):
-        raise RuntimeError("out must have a tensor for each gradient (got %d for %d)" % (len(outs), len(grads)))
-    if not grads:
+    if not grads and not outs:
         return torch.zeros(())
-    ptr, n, types = _gradient_table(grads)
-    h, dev, optr, otypes = _l.lib(), grads[0].device, None, None
-    if outs is not None:
-        for g, o in zip(grads, outs):
-            if o.shape != g.shape or o.device != dev or (o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous())):
-                raise RuntimeError("out must have the gradients' shapes, order of dimensions and device")
-            if o.dtype != g.dtype and o.dtype != torch.float32:
-                raise RuntimeError("out must be of the gradient's type or float32 (got %s for %s)" % (o.dtype, g.dtype))
-        optr, _, otypes = _gradient_table(outs, "out")
-    with torch.cuda.device(dev):
-        norm = torch.empty((), dtype=torch.float32, device=dev)
-        ws = torch.empty(h.cpfn_grad_norm_workspace(n, len(grads)) // 8, dtype=torch.float64, device=dev)
-        status = h.cpfn_grad_clip(ptr, optr, n, types, otypes, len(grads), p, max_norm, _ptr(norm), _ptr(ws), _stream())
-        if status == -22:
-            raise RuntimeError("a tensor that is written shares memory with another one of the lists (a gradient listed twice?)")
-        _l.check(status, "cpfn_grad_clip")
-    _l.add_bytes("cpfn_grad_clip", sum(t.numel() * t.element_size() for t in grads + (outs or grads)))
+    dev, nbytes, ptr, n, types, optr, otypes = _tables.gradients(grads, outs)
+    dev = torch.device("cuda", dev)
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    ws = torch.empty(_l.lib().cpfn_grad_norm_workspace(n, len(grads)) // 8, dtype=torch.float64, device=dev)
+    _launch("cpfn_grad_clip", dev, ptr, optr, n, types, otypes, len(grads), p, max_norm, norm.data_ptr(), ws.data_ptr())
+    _l.add_bytes("cpfn_grad_clip", nbytes if outs else 2 * nbytes)
     return norm
 
 

@@ -34,6 +34,7 @@ extern "C" {
 #endif
 
 #define CPFN_EINVAL (-22)
+#define CPFN_EOVERLAP (-16) /* a tensor that is written shares memory with another one (cpfn_grad_clip) */
 #define CPFN_ABI_VERSION 3
 
 /* Library / build identification (no GPU needed). */
@@ -880,7 +881,7 @@ CPFN_API long long cpfn_grad_norm_workspace(const long long *n, int count);
 CPFN_API int cpfn_grad_norm(const void *const *grads, const long long *n, const int *type, int count, int p, float *norm, void *workspace,
                             void *stream);
 /* ... and out[i] = min(1, max_norm / (norm + 1e-6)) grads[i].  out NULL: in place; else tensors of the same type or fp32 (out_type).
- * A tensor that is written may share memory with no other one of the lists (refused), except that out[i] may be grads[i]. */
+ * A tensor that is written may share memory with no other one of the lists (CPFN_EOVERLAP), except that out[i] may be grads[i]. */
 CPFN_API int cpfn_grad_clip(const void *const *grads, void *const *out, const long long *n, const int *type, const int *out_type, int count,
                             int p, double max_norm, float *norm, void *workspace, void *stream);
 /* The sums of squares of cpfn_grad_sumsq_blocks(n) workgroups over one fp32 tensor. */
