@@ -59,26 +59,22 @@ __device__ __forceinline__ void zero_counters(unsigned short *cnt, int E) {     
   __syncthreads();
 }
 
-// counts[e][tile] (several tiles only)
+// counts[e][tile] (several tiles only): a histogram by LDS additions, whose order does not show in an integer
 template <typename I>
-__global__ __launch_bounds__(RANK_WAVES * 64) void route_count_kernel(const I *__restrict__ choice, long long n, int E, int bits, int tiles,
+__global__ __launch_bounds__(RANK_WAVES * 64) void route_count_kernel(const I *__restrict__ choice, long long n, int E, int tiles,
                                                                       int *__restrict__ counts) {
-  extern __shared__ unsigned lds[];               // [waves][E] 16-bit counters
-  unsigned short *cnt = (unsigned short *)lds;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const long long i0 = (long long)blockIdx.x * RANK_TILE + wave * (RANK_ITEMS * 64) + lane;
-  int e[RANK_ITEMS], rank[RANK_ITEMS];
+  extern __shared__ unsigned lds[];               // [E]
+  for (int x = threadIdx.x; x < E; x += RANK_WAVES * 64) lds[x] = 0u;
+  const long long i0 = (long long)blockIdx.x * RANK_TILE + threadIdx.x;
+  int e[RANK_ITEMS];
 #pragma unroll
-  for (int t = 0; t < RANK_ITEMS; ++t) e[t] = expert_of(choice, i0 + t * 64, n, E);
-  zero_counters(cnt, E);
-  wave_ranks(e, rank, cnt + wave * E, bits, lane);
+  for (int t = 0; t < RANK_ITEMS; ++t) e[t] = expert_of(choice, i0 + t * (RANK_WAVES * 64), n, E);
   __syncthreads();
-  for (int x = threadIdx.x; x < E; x += RANK_WAVES * 64) {
-    int s = 0;
 #pragma unroll
-    for (int w = 0; w < RANK_WAVES; ++w) s += cnt[w * E + x];
-    counts[(long long)x * tiles + blockIdx.x] = s;
-  }
+  for (int t = 0; t < RANK_ITEMS; ++t)
+    if (e[t] >= 0) atomicAdd(&lds[e[t]], 1u);
+  __syncthreads();
+  for (int x = threadIdx.x; x < E; x += RANK_WAVES * 64) counts[(long long)x * tiles + blockIdx.x] = (int)lds[x];
 }
 
 __device__ __forceinline__ int wave_scan(int v, int lane) {                       // inclusive
@@ -341,10 +337,10 @@ int plan(const I *choice, long long n, int E, int *offsets, int *place, int *ws,
   const int tiles = n > RANK_TILE ? (int)((n + RANK_TILE - 1) / RANK_TILE) : 1;
   int bits = 0;
   while ((1 << bits) < E) ++bits;
-  const size_t lds_count = (size_t)RANK_WAVES * E * 2, lds_rank = lds_count + (size_t)E * 4;
+  const size_t lds_rank = (size_t)RANK_WAVES * E * 2 + (size_t)E * 4;
   const int mode = tiles == 1 ? 0 : tiles <= DIRECT_TILES && E <= DIRECT_E ? 1 : 2;
   int *counts = ws, *totals = ws + (size_t)tiles * E;
-  if (mode) route_count_kernel<I><<<tiles, RANK_WAVES * 64, lds_count, st>>>(choice, n, E, bits, tiles, counts);
+  if (mode) route_count_kernel<I><<<tiles, RANK_WAVES * 64, (size_t)E * 4, st>>>(choice, n, E, tiles, counts);
   if (mode == 2) route_scan_kernel<<<cpfn_cdiv(E, 4), 256, 0, st>>>(counts, totals, E, tiles);
   route_rank_kernel<I><<<tiles, RANK_WAVES * 64, lds_rank, st>>>(choice, n, E, bits, tiles, mode, counts, totals, offsets, place);
   return cpfn_launch_status();

@@ -11,8 +11,9 @@
 
 #define CPFN_NORM_MAX_C 4096        // (512 lanes: with 1024 the backward kernel's registers do not fit)
 
+// (rows of several waves have a workgroup of their own: its barriers then wait for nobody else)
 template <typename T, int L> struct NormShape {
-  enum { THREADS = L <= 256 ? 256 : L, ROWS = THREADS / L, VN = cpfn_piece<T>::N, NP = 8 / VN, WAVES = THREADS / 64 };
+  enum { THREADS = L <= 64 ? 256 : L, ROWS = THREADS / L, VN = cpfn_piece<T>::N, NP = 8 / VN, WAVES = THREADS / 64 };
 };
 
 // channel of element i (0..7) of lane `lane` of its row
@@ -23,9 +24,27 @@ template <typename T, int L> __device__ __forceinline__ int norm_col(int lane, i
 
 template <typename T, int L> struct RowRaw { typename cpfn_piece<T>::vec p[8 / cpfn_piece<T>::N]; };
 
-template <typename T, int L> __device__ __forceinline__ void row_load(RowRaw<T, L> &raw, const T *__restrict__ row, int lane, int C) {
+// RAGGED: C is no multiple of a piece; `mask`: what of this lane's pieces lies in the row
+template <typename T, int L, bool RAGGED> __device__ __forceinline__ RowRaw<T, L> row_mask(int lane, int C) {
+  RowRaw<T, L> m;
 #pragma unroll
-  for (int q = 0; q < 8 / cpfn_piece<T>::N; ++q) raw.p[q] = cpfn_load_piece(row, (q * L + lane) * cpfn_piece<T>::N, C);
+  for (int q = 0; q < 8 / cpfn_piece<T>::N; ++q) {
+    if (RAGGED) m.p[q] = cpfn_piece_mask<T>(C - (q * L + lane) * cpfn_piece<T>::N);
+    else m.p[q] = {};
+  }
+  return m;
+}
+// row r of P rows
+template <typename T, int L, bool RAGGED>
+__device__ __forceinline__ void row_load(RowRaw<T, L> &raw, const T *__restrict__ base, long long r, long long P, int lane, int C, const RowRaw<T, L> &mask) {
+  const T *__restrict__ row = base + r * C;
+#pragma unroll
+  for (int q = 0; q < 8 / cpfn_piece<T>::N; ++q) {
+    const int at = (q * L + lane) * cpfn_piece<T>::N;
+    if (RAGGED) raw.p[q] = cpfn_load_ragged(row, at, C, (P - r) * C, mask.p[q]);
+    else if (at < C) raw.p[q] = *(const typename cpfn_piece<T>::vec *)(row + at);
+    else raw.p[q] = {};
+  }
 }
 template <typename T, int L> __device__ __forceinline__ void row_zero(RowRaw<T, L> &raw) {
 #pragma unroll
@@ -35,9 +54,13 @@ template <typename T, int L> __device__ __forceinline__ void row_unpack(const Ro
 #pragma unroll
   for (int q = 0; q < 8 / cpfn_piece<T>::N; ++q) cpfn_unpack(raw.p[q], f + q * cpfn_piece<T>::N, (T *)nullptr);
 }
-template <typename T, int L> __device__ __forceinline__ void row_store(T *__restrict__ row, int lane, int C, const float *f) {
+template <typename T, int L, bool RAGGED> __device__ __forceinline__ void row_store(T *__restrict__ row, int lane, int C, const float *f) {
 #pragma unroll
-  for (int q = 0; q < 8 / cpfn_piece<T>::N; ++q) cpfn_store_piece(row, (q * L + lane) * cpfn_piece<T>::N, C, f + q * cpfn_piece<T>::N);
+  for (int q = 0; q < 8 / cpfn_piece<T>::N; ++q) {
+    const int at = (q * L + lane) * cpfn_piece<T>::N;
+    if (RAGGED) cpfn_store_piece(row, at, C, f + q * cpfn_piece<T>::N);
+    else if (at < C) *(typename cpfn_piece<T>::vec *)(row + at) = cpfn_pack(f + q * cpfn_piece<T>::N, (T *)nullptr);
+  }
 }
 // a parameter vector (fp32, any 4-byte alignment: parameters live inside a flat buffer), `fill` where there is none
 template <typename T, int L> __device__ __forceinline__ void param_load(float *f, const float *__restrict__ p, int lane, int C, float fill) {
@@ -78,7 +101,7 @@ template <int L> __device__ __forceinline__ float row_sum(float a, float2 *slots
 // v -> its normalised form (v - mu) r; returns r.  Two passes over the registers for `layer` (mean, then centred squares): no
 // cancellation.  Channels behind C hold zero and stay out of the centred squares; a row slot without a row is called with a positive
 // eps, so that its zeros stay zeros.
-template <typename T, int L>
+template <typename T, int L, bool RAGGED>
 __device__ __forceinline__ float row_normalise(float *v, int lane, int C, float inv_c, bool layer, float eps, float2 *slots, int &turn) {
   if (layer) {
     float s = 0.f;
@@ -86,7 +109,7 @@ __device__ __forceinline__ float row_normalise(float *v, int lane, int C, float 
     for (int i = 0; i < 8; ++i) s += v[i];
     const float mu = row_sum<L>(s, slots, turn) * inv_c;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = norm_col<T, L>(lane, i) < C ? v[i] - mu : 0.f;
+    for (int i = 0; i < 8; ++i) v[i] = norm_col<T, L>(lane, RAGGED ? i : i & -cpfn_piece<T>::N) < C ? v[i] - mu : 0.f;
   }
   float q = 0.f;
 #pragma unroll
@@ -97,7 +120,11 @@ __device__ __forceinline__ float row_normalise(float *v, int lane, int C, float 
   return r;
 }
 
-__device__ __forceinline__ float norm_sigmoid(float v) { return __builtin_amdgcn_rcpf(1.f + expf(-v)); }
+// 1 / (1 + exp(-v)).  fp32 rows: exp within 2 units in the last place.  16-bit rows: exp2(-v log2 e) with the product rounded, off by
+// |v| 2^-24 relative on top (2^-18 at |v| = 64; the results are rounded to 2^-9), a third of the instructions.
+template <typename T> __device__ __forceinline__ float norm_sigmoid(float v) {
+  return __builtin_amdgcn_rcpf(1.f + (sizeof(T) == 4 ? expf(-v) : __builtin_amdgcn_exp2f(v * -1.44269504f)));
+}
 
 // the gate's row for row r (a 64-bit division only where 32 bits do not hold the rows)
 __device__ __forceinline__ long long norm_gate_row(long long r, long long rows_per_gate, long long P) {

@@ -15,6 +15,8 @@
 
 namespace {
 
+constexpr long long BWD_WAVES = 2048;         // waves of a launch: what is resident together (two for each SIMD)
+
 template <typename T> struct NormBwd {
   const T *x, *y, *gate, *d_out, *d_normed;
   const float *weight, *bias, *scale, *next_weight;
@@ -55,7 +57,7 @@ template <typename T, int L, typename F> __device__ __forceinline__ void slots_s
   }
 }
 
-template <typename T, int L>
+template <typename T, int L, bool RAGGED>
 __global__ __launch_bounds__((NormShape<T, L>::THREADS)) void norm_residual_bwd_kernel(const NormBwd<T> a) {
   constexpr int ROWS = NormShape<T, L>::ROWS, THREADS = NormShape<T, L>::THREADS;
   __shared__ float2 slots[32];
@@ -71,6 +73,21 @@ __global__ __launch_bounds__((NormShape<T, L>::THREADS)) void norm_residual_bwd_
   param_load<T, L>(nw, a.next_weight, lane, C, 1.f);
 #pragma unroll
   for (int i = 0; i < 8; ++i) { s1[i] = s2[i] = s3[i] = s4[i] = sg[i] = 0.f; }
+  const RowRaw<T, L> mask = row_mask<T, L, RAGGED>(lane, C);
+  // the rows of the NEXT step are requested before this one's are worked on
+  RowRaw<T, L> rx, ry, rg, rd, rn;
+  row_zero(rx); row_zero(ry); row_zero(rg); row_zero(rd); row_zero(rn);
+  const auto request = [&](long long g, long long r, long long row1) {
+    if (r < row1) {
+      if (next) row_load<T, L, RAGGED>(rx, a.x, r, a.P, lane, C, mask);
+      if (has_y) row_load<T, L, RAGGED>(ry, a.y, r, a.P, lane, C, mask);
+      if (a.gate) row_load<T, L, RAGGED>(rg, a.gate, a.shared_gate ? g : r, a.shared_gate ? a.groups : a.P, lane, C, mask);
+      if (a.d_out) row_load<T, L, RAGGED>(rd, a.d_out, r, a.P, lane, C, mask);
+      if (next) row_load<T, L, RAGGED>(rn, a.d_normed, r, a.P, lane, C, mask);
+    } else {
+      row_zero(rx); row_zero(ry); row_zero(rg); row_zero(rd); row_zero(rn);
+    }
+  };
   const long long g0 = a.blocks_per_group > 1 ? blockIdx.x / a.blocks_per_group : (long long)blockIdx.x * a.groups_per_block;
   long long g1 = a.blocks_per_group > 1 ? g0 + 1 : g0 + a.groups_per_block;
   if (g1 > a.groups) g1 = a.groups;
@@ -81,28 +98,22 @@ __global__ __launch_bounds__((NormShape<T, L>::THREADS)) void norm_residual_bwd_
       row0 += (long long)(blockIdx.x % a.blocks_per_group) * a.chunk;
       if (row0 + a.chunk < row1) row1 = row0 + a.chunk;
     }
+    request(g, row0 + slot, row1);
     for (long long base = row0; base < row1; base += ROWS) {
       const long long r = base + slot;
       const bool there = r < row1;
       const float eps = there ? a.eps : 1.f;
-      RowRaw<T, L> rx, ry, rg, rd, rn;
-      row_zero(rx); row_zero(ry); row_zero(rg); row_zero(rd); row_zero(rn);
-      if (there) {
-        if (next) row_load(rx, a.x + r * C, lane, C);
-        if (has_y) row_load(ry, a.y + r * C, lane, C);
-        if (a.gate) row_load(rg, a.gate + (a.shared_gate ? g : r) * C, lane, C);
-        if (a.d_out) row_load(rd, a.d_out + r * C, lane, C);
-        if (next) row_load(rn, a.d_normed + r * C, lane, C);
-      }
+      const RowRaw<T, L> cx = rx, cy = ry, cg = rg, cd = rd, cn = rn;
+      request(g, r + ROWS, row1);
       float hat2[8], ga[8], r2 = 0.f;
       if (has_y) {
-        row_unpack(ry, hat2);
-        if (post) r2 = row_normalise<T, L>(hat2, lane, C, inv_c, layer, eps, slots, turn);
+        row_unpack(cy, hat2);
+        if (post) r2 = row_normalise<T, L, RAGGED>(hat2, lane, C, inv_c, layer, eps, slots, turn);
         if (a.gate) {
-          row_unpack(rg, ga);
+          row_unpack(cg, ga);
           if (a.sigmoid) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) ga[i] = norm_sigmoid(ga[i]);
+            for (int i = 0; i < 8; ++i) ga[i] = norm_sigmoid<T>(ga[i]);
           }
         } else {
 #pragma unroll
@@ -110,16 +121,16 @@ __global__ __launch_bounds__((NormShape<T, L>::THREADS)) void norm_residual_bwd_
         }
       }
       float D[8];
-      row_unpack(rd, D);
+      row_unpack(cd, D);
       if (next) {
         float h[8], dn[8];
-        row_unpack(rx, h);
-        row_unpack(rn, dn);
+        row_unpack(cx, h);
+        row_unpack(cn, dn);
         if (has_y) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) h[i] = fmaf(s[i], ga[i] * fmaf(hat2[i], w[i], b[i]), h[i]);
         }
-        const float r1 = row_normalise<T, L>(h, lane, C, inv_c, layer, eps, slots, turn);
+        const float r1 = row_normalise<T, L, RAGGED>(h, lane, C, inv_c, layer, eps, slots, turn);
         float m1 = 0.f, m2 = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -135,7 +146,7 @@ __global__ __launch_bounds__((NormShape<T, L>::THREADS)) void norm_residual_bwd_
 #pragma unroll
         for (int i = 0; i < 8; ++i) D[i] = fmaf(r1, dn[i] - m1 - h[i] * m2, D[i]);
       }
-      if (there && a.d_x) row_store<T, L>(a.d_x + r * C, lane, C, D);
+      if (there && a.d_x) row_store<T, L, RAGGED>(a.d_x + r * C, lane, C, D);
       if (has_y) {
         float e[8], m1 = 0.f, m2 = 0.f;
 #pragma unroll
@@ -155,7 +166,7 @@ __global__ __launch_bounds__((NormShape<T, L>::THREADS)) void norm_residual_bwd_
             if (a.sigmoid) dg[i] *= ga[i] * (1.f - ga[i]);
             sg[i] += dg[i];
           }
-          if (there && !a.shared_gate) row_store<T, L>(a.d_gate + r * C, lane, C, dg);
+          if (there && !a.shared_gate) row_store<T, L, RAGGED>(a.d_gate + r * C, lane, C, dg);
         }
         if (post) {
           row_sum2<L>(m1, m2, slots, turn);
@@ -164,7 +175,7 @@ __global__ __launch_bounds__((NormShape<T, L>::THREADS)) void norm_residual_bwd_
 #pragma unroll
           for (int i = 0; i < 8; ++i) e[i] = r2 * (e[i] - m1 - hat2[i] * m2);
         }
-        if (there && a.d_y) row_store<T, L>(a.d_y + r * C, lane, C, e);
+        if (there && a.d_y) row_store<T, L, RAGGED>(a.d_y + r * C, lane, C, e);
       }
     }
     if (a.shared_gate && a.d_gate && a.blocks_per_group == 1) {        // this workgroup has seen all rows of the gate's row
@@ -234,13 +245,13 @@ template <typename T> __global__ __launch_bounds__(1024) void norm_residual_redu
 // How the rows are split over workgroups.
 struct NormSplit { long long groups, rows_per_gate, chunk; int nblk, blocks_per_group, groups_per_block; };
 NormSplit norm_split(long long P, int C, long long gate_rows) {
-  const int L = norm_lanes(C), threads = L <= 256 ? 256 : L, rows = threads / L;
+  const int L = norm_lanes(C), threads = L <= 64 ? 256 : L, rows = threads / L;
   const bool shared = gate_rows > 0 && gate_rows < P;
   NormSplit s;
   s.groups = shared ? gate_rows : 1;
   s.rows_per_gate = P / s.groups;
   const long long sets = (s.rows_per_gate + rows - 1) / rows;             // row sets of a group
-  const long long want = 768 * 256 / threads;                             // workgroups that are resident together
+  const long long want = BWD_WAVES * 64 / threads;
   long long bpg = (want + s.groups - 1) / s.groups;
   if (bpg > (sets + 3) / 4) bpg = (sets + 3) / 4;                         // (at least four row sets each: the sums have to be paid for)
   if (bpg < 1) bpg = 1;
@@ -259,7 +270,8 @@ NormSplit norm_split(long long P, int C, long long gate_rows) {
 }
 
 template <typename T, int L> void launch(const NormBwd<T> &a, int nblk, hipStream_t st) {
-  norm_residual_bwd_kernel<T, L><<<nblk, NormShape<T, L>::THREADS, 0, st>>>(a);
+  if (a.C % cpfn_piece<T>::N) norm_residual_bwd_kernel<T, L, true><<<nblk, NormShape<T, L>::THREADS, 0, st>>>(a);
+  else norm_residual_bwd_kernel<T, L, false><<<nblk, NormShape<T, L>::THREADS, 0, st>>>(a);
 }
 
 struct Grads { float *d_weight, *d_bias, *d_scale, *d_next_weight, *d_next_bias; };

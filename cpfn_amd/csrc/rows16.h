@@ -93,15 +93,64 @@ template <typename T> __device__ __forceinline__ typename cpfn_piece<T>::vec cpf
   }
   return r;
 }
+// (a vector's element goes through a value: __builtin_bit_cast of the element itself reads element 0 with this compiler)
+__device__ __forceinline__ unsigned cpfn_word(float v) { return __float_as_uint(v); }
+__device__ __forceinline__ unsigned cpfn_word(unsigned v) { return v; }
+__device__ __forceinline__ void cpfn_word_to(unsigned m, cpfn_piece<float>::vec &v, int i) { v[i] = __uint_as_float(m); }
+__device__ __forceinline__ void cpfn_word_to(unsigned m, cpfn_piece<cpfn_bf16>::vec &v, int i) { v[i] = m; }
+// the words of a piece that n of its elements fill (n >= N: all), as masks
+template <typename T> __device__ __forceinline__ typename cpfn_piece<T>::vec cpfn_piece_mask(int n) {
+  constexpr int PER = cpfn_piece<T>::N / 4;              // elements of a word
+  unsigned m[4];
+#pragma unroll
+  for (int w = 0; w < 4; ++w) m[w] = n >= (w + 1) * PER ? 0xffffffffu : PER == 2 && n == 2 * w + 1 ? 0xffffu : 0u;
+  typename cpfn_piece<T>::vec v;
+  cpfn_word_to(m[0], v, 0); cpfn_word_to(m[1], v, 1); cpfn_word_to(m[2], v, 2); cpfn_word_to(m[3], v, 3);
+  return v;
+}
+__device__ __forceinline__ float cpfn_and_word(float a, float m) { return __uint_as_float(__float_as_uint(a) & __float_as_uint(m)); }
+__device__ __forceinline__ unsigned cpfn_and_word(unsigned a, unsigned m) { return a & m; }
+// ... of a ragged row (C is no multiple of N): the whole 16 bytes are read wherever the tensor reaches that far — `room` elements from p
+// on —, what belongs to the next row is masked away; only at the very end of the tensor does it go element by element
+template <typename T>
+__device__ __forceinline__ typename cpfn_piece<T>::vec cpfn_load_ragged(const T *__restrict__ p, int at, int C, long long room,
+                                                                        const typename cpfn_piece<T>::vec &mask) {
+  typedef typename cpfn_piece<T>::vec V;
+  if (at < C && at + cpfn_piece<T>::N > room) return cpfn_load_piece(p, at, C);
+  V r = {};
+  if (at < C) {
+    r = *(const V *)(p + at);
+    r.x = cpfn_and_word(r.x, mask.x); r.y = cpfn_and_word(r.y, mask.y); r.z = cpfn_and_word(r.z, mask.z); r.w = cpfn_and_word(r.w, mask.w);
+  }
+  return r;
+}
+// 16 bytes, or the first C % N elements of them in one to three stores (which ones is the same for a whole launch)
 template <typename T> __device__ __forceinline__ void cpfn_store_piece(T *__restrict__ p, int at, int C, const float *f) {
   typedef typename cpfn_piece<T>::vec V;
   constexpr int N = cpfn_piece<T>::N;
+  const V v = cpfn_pack(f, (T *)nullptr);
   if (at + N <= C) {
-    *(V *)(p + at) = cpfn_pack(f, (T *)nullptr);
+    *(V *)(p + at) = v;
   } else if (at < C) {
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (at + i < C) p[at + i] = cpfn_from_f32<T>(f[i]);
+    typedef unsigned two __attribute__((ext_vector_type(2), aligned(2)));
+    typedef unsigned one __attribute__((aligned(2)));
+    const unsigned w[4] = {cpfn_word(v.x), cpfn_word(v.y), cpfn_word(v.z), cpfn_word(v.w)};
+    char *o = (char *)(p + at);
+    const int bytes = (C % N) * (int)sizeof(T);
+    if (bytes & 8) {
+      *(two *)o = two{w[0], w[1]};
+      if (bytes & 4) {
+        *(one *)(o + 8) = w[2];
+        if (bytes & 2) *(unsigned short *)(o + 12) = (unsigned short)w[3];
+      } else if (bytes & 2) {
+        *(unsigned short *)(o + 8) = (unsigned short)w[2];
+      }
+    } else if (bytes & 4) {
+      *(one *)o = w[0];
+      if (bytes & 2) *(unsigned short *)(o + 4) = (unsigned short)w[1];
+    } else if (bytes & 2) {
+      *(unsigned short *)o = (unsigned short)w[0];
+    }
   }
 }
 

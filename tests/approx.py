@@ -58,10 +58,12 @@ class Approx:
         q = self.v / o.v
         return Approx._new(q, (self.e + q.abs() * o.e) / o.v.abs(), 3.0)
 
-    def sigmoid(self):
-        """1 / (1 + exp(-v)): exp within 2 units in the last place, one sum, a reciprocal within 1: 8 u covers them."""
+    def sigmoid(self, fast=False):
+        """1 / (1 + exp(-v)): exp within 2 units in the last place, one sum, a reciprocal within 1: 8 u covers them.  fast: exp(-v) as
+        exp2 of the rounded product v log2(e): the product is off by u |v| log2(e), log2(e) itself by u relative, so the power by
+        ln 2 (2 u |v| log2(e)) = 2 u |v| relative, and the sigmoid by at most as much."""
         a = torch.sigmoid(self.v)
-        return Approx._new(a, a * (1.0 - a) * self.e, 8.0)
+        return Approx._new(a, a * (1.0 - a) * self.e, 8.0 + (2.0 * self.v.abs() if fast else 0.0))
 
     def view(self, *shape):
         return Approx(self.v.reshape(*shape), self.e.expand_as(self.v).reshape(*shape))

@@ -39,7 +39,7 @@ def reference(t, kind, act, d_out, d_normed):
         if "gate" in f:
             G = t["gate"].shape[0]
             a = Approx(f["gate"].v.repeat_interleave(P // G, 0))
-            a = a.sigmoid() if act == "sigmoid" else a
+            a = a.sigmoid(fast=t["x"].dtype != torch.float32) if act == "sigmoid" else a
         s = f.get("scale", one)
         total = total + s * (a * u)
         got["out"] = total
