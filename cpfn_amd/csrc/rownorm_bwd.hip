@@ -15,8 +15,6 @@
 
 namespace {
 
-constexpr long long BWD_WAVES = 2048;         // waves of a launch: what is resident together (two for each SIMD)
-
 template <typename T> struct NormBwd {
   const T *x, *y, *gate, *d_out, *d_normed;
   const float *weight, *bias, *scale, *next_weight;
@@ -57,67 +55,86 @@ template <typename T, int L, typename F> __device__ __forceinline__ void slots_s
   }
 }
 
-template <typename T, int L, bool RAGGED>
+template <typename T, int L, NormMode MODE>
 __global__ __launch_bounds__((NormShape<T, L>::THREADS)) void norm_residual_bwd_kernel(const NormBwd<T> a) {
-  constexpr int ROWS = NormShape<T, L>::ROWS, THREADS = NormShape<T, L>::THREADS;
-  __shared__ float2 slots[32];
+  constexpr int ROWS = NormShape<T, L>::ROWS, THREADS = NormShape<T, L>::THREADS, NP = NormShape<T, L>::NP;
+  __shared__ float2 slots[16];
   __shared__ float comb[ROWS > 1 ? THREADS * 8 : 1];
   int turn = 0;
   const int lane = threadIdx.x & (L - 1), slot = threadIdx.x / L, C = a.C;
   const float inv_c = 1.f / (float)C;
-  const bool layer = a.layer != 0, post = a.weight != nullptr, has_y = a.y != nullptr, next = a.d_normed != nullptr;
+  const bool layer = a.layer != 0, post = a.weight != nullptr, has_y = a.y != nullptr, next = a.d_normed != nullptr, has_gate = a.gate != nullptr;
   float w[8], b[8], s[8], nw[8], s1[8], s2[8], s3[8], s4[8], sg[8];
-  param_load<T, L>(w, a.weight, lane, C, 1.f);
-  param_load<T, L>(b, a.bias, lane, C, 0.f);
-  param_load<T, L>(s, a.scale, lane, C, 1.f);
-  param_load<T, L>(nw, a.next_weight, lane, C, 1.f);
+  param_load<T, L, MODE != WHOLE>(w, a.weight, lane, C, 1.f);
+  param_load<T, L, MODE != WHOLE>(b, a.bias, lane, C, 0.f);
+  param_load<T, L, MODE != WHOLE>(s, a.scale, lane, C, 1.f);
+  param_load<T, L, MODE != WHOLE>(nw, a.next_weight, lane, C, 1.f);
 #pragma unroll
   for (int i = 0; i < 8; ++i) { s1[i] = s2[i] = s3[i] = s4[i] = sg[i] = 0.f; }
-  const RowRaw<T, L> mask = row_mask<T, L, RAGGED>(lane, C);
-  // the rows of the NEXT step are requested before this one's are worked on
-  RowRaw<T, L> rx, ry, rg, rd, rn;
-  row_zero(rx); row_zero(ry); row_zero(rg); row_zero(rd); row_zero(rn);
-  const auto request = [&](long long g, long long r, long long row1) {
-    if (r < row1) {
-      if (next) row_load<T, L, RAGGED>(rx, a.x, r, a.P, lane, C, mask);
-      if (has_y) row_load<T, L, RAGGED>(ry, a.y, r, a.P, lane, C, mask);
-      if (a.gate) row_load<T, L, RAGGED>(rg, a.gate, a.shared_gate ? g : r, a.shared_gate ? a.groups : a.P, lane, C, mask);
-      if (a.d_out) row_load<T, L, RAGGED>(rd, a.d_out, r, a.P, lane, C, mask);
-      if (next) row_load<T, L, RAGGED>(rn, a.d_normed, r, a.P, lane, C, mask);
-    } else {
-      row_zero(rx); row_zero(ry); row_zero(rg); row_zero(rd); row_zero(rn);
-    }
-  };
   const long long g0 = a.blocks_per_group > 1 ? blockIdx.x / a.blocks_per_group : (long long)blockIdx.x * a.groups_per_block;
   long long g1 = a.blocks_per_group > 1 ? g0 + 1 : g0 + a.groups_per_block;
   if (g1 > a.groups) g1 = a.groups;
   const int nsums = 4 + (a.shared_gate && a.blocks_per_group > 1);
+  const unsigned set_bytes = (unsigned)(ROWS * C) * (unsigned)sizeof(T);
   for (long long g = g0; g < g1; ++g) {
     long long row0 = g * a.rows_per_gate, row1 = row0 + a.rows_per_gate;
     if (a.blocks_per_group > 1) {
       row0 += (long long)(blockIdx.x % a.blocks_per_group) * a.chunk;
       if (row0 + a.chunk < row1) row1 = row0 + a.chunk;
     }
-    request(g, row0 + slot, row1);
-    for (long long base = row0; base < row1; base += ROWS) {
+    RowChunk<T, L, MODE> ch;
+    ch.begin(row0, row1, a.P, C, lane, slot);
+    const T *own_gate = a.shared_gate ? nullptr : a.gate;
+    T *d_own_gate = a.shared_gate ? nullptr : a.d_gate;
+    const auto bx = ch.source(next ? a.x : nullptr), by = ch.source(a.y), bg = ch.source(own_gate), bd = ch.source(a.d_out), bn = ch.source(a.d_normed);
+    const auto tx = ch.target(a.d_x), ty = ch.target(a.d_y), tg = ch.target(d_own_gate);
+    RowRaw<T, L> rx, ry, rg, rd, rn, shared;
+    unsigned o[NP], sh[NP];
+    const auto request = [&](unsigned step, long long r) {
+      if (MODE == EACH) {
+        each_load(rx, next ? a.x : nullptr, r, lane, C, r < row1);
+        each_load(ry, a.y, r, lane, C, r < row1);
+        each_load(rg, own_gate, r, lane, C, r < row1);
+        each_load(rd, a.d_out, r, lane, C, r < row1);
+        each_load(rn, a.d_normed, r, lane, C, r < row1);
+      } else {
+        ch.at(o, sh, step, r < row1);
+        ch.load(rx, bx, o);
+        ch.load(ry, by, o);
+        ch.load(rg, bg, o);
+        ch.load(rd, bd, o);
+        ch.load(rn, bn, o);
+      }
+    };
+    float gs[8];
+    if (a.shared_gate) {
+      single_load<T, L>(shared, a.gate + g * C, lane, C);
+      row_unpack(shared, gs);
+      arrived(gs);
+    }
+    arrived(w); arrived(b); arrived(s); arrived(nw);
+    request(0, row0 + slot);
+    arrived(rx); arrived(ry); arrived(rg); arrived(rd); arrived(rn);
+    unsigned step = 0;
+    for (long long base = row0; base < row1; base += ROWS, step += set_bytes) {
       const long long r = base + slot;
       const bool there = r < row1;
       const float eps = there ? a.eps : 1.f;
-      const RowRaw<T, L> cx = rx, cy = ry, cg = rg, cd = rd, cn = rn;
-      request(g, r + ROWS, row1);
+      RowRaw<T, L> cx = rx, cy = ry, cg = rg, cd = rd, cn = rn;
+      unsigned csh[NP];
+#pragma unroll
+      for (int q = 0; q < NP; ++q) csh[q] = MODE == RAGGED ? sh[q] : 0u;
+      request(step + set_bytes, r + ROWS);
+      ch.settle(cx, csh); ch.settle(cy, csh); ch.settle(cg, csh); ch.settle(cd, csh); ch.settle(cn, csh);
       float hat2[8], ga[8], r2 = 0.f;
       if (has_y) {
         row_unpack(cy, hat2);
-        if (post) r2 = row_normalise<T, L, RAGGED>(hat2, lane, C, inv_c, layer, eps, slots, turn);
-        if (a.gate) {
-          row_unpack(cg, ga);
-          if (a.sigmoid) {
+        if (post) r2 = row_normalise<T, L, MODE>(hat2, lane, C, inv_c, layer, eps, slots, turn);
+        row_unpack(cg, ga);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) ga[i] = norm_sigmoid<T>(ga[i]);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) ga[i] = 1.f;
+        for (int i = 0; i < 8; ++i) {
+          const float t = a.shared_gate ? gs[i] : ga[i];
+          ga[i] = !has_gate ? 1.f : a.sigmoid ? norm_sigmoid<T>(t) : t;
         }
       }
       float D[8];
@@ -130,7 +147,7 @@ __global__ __launch_bounds__((NormShape<T, L>::THREADS)) void norm_residual_bwd_
 #pragma unroll
           for (int i = 0; i < 8; ++i) h[i] = fmaf(s[i], ga[i] * fmaf(hat2[i], w[i], b[i]), h[i]);
         }
-        const float r1 = row_normalise<T, L, RAGGED>(h, lane, C, inv_c, layer, eps, slots, turn);
+        const float r1 = row_normalise<T, L, MODE>(h, lane, C, inv_c, layer, eps, slots, turn);
         float m1 = 0.f, m2 = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -146,9 +163,11 @@ __global__ __launch_bounds__((NormShape<T, L>::THREADS)) void norm_residual_bwd_
 #pragma unroll
         for (int i = 0; i < 8; ++i) D[i] = fmaf(r1, dn[i] - m1 - h[i] * m2, D[i]);
       }
-      if (there && a.d_x) row_store<T, L, RAGGED>(a.d_x + r * C, lane, C, D);
+      if (MODE == EACH) each_store<T, L>(a.d_x, r, lane, C, there, D);
+      else ch.store(tx, step, D);
+      float e[8], dg[8];
       if (has_y) {
-        float e[8], m1 = 0.f, m2 = 0.f;
+        float m1 = 0.f, m2 = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const float da = D[i] * ga[i];
@@ -159,14 +178,12 @@ __global__ __launch_bounds__((NormShape<T, L>::THREADS)) void norm_residual_bwd_
           m2 = fmaf(e[i], hat2[i], m2);
         }
         if (a.d_gate) {
-          float dg[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             dg[i] = D[i] * s[i] * fmaf(hat2[i], w[i], b[i]);
             if (a.sigmoid) dg[i] *= ga[i] * (1.f - ga[i]);
             sg[i] += dg[i];
           }
-          if (there && !a.shared_gate) row_store<T, L, RAGGED>(a.d_gate + r * C, lane, C, dg);
         }
         if (post) {
           row_sum2<L>(m1, m2, slots, turn);
@@ -175,8 +192,15 @@ __global__ __launch_bounds__((NormShape<T, L>::THREADS)) void norm_residual_bwd_
 #pragma unroll
           for (int i = 0; i < 8; ++i) e[i] = r2 * (e[i] - m1 - hat2[i] * m2);
         }
-        if (there && a.d_y) row_store<T, L, RAGGED>(a.d_y + r * C, lane, C, e);
       }
+      if (MODE == EACH) {
+        each_store<T, L>(d_own_gate, r, lane, C, there, dg);
+        each_store<T, L>(a.d_y, r, lane, C, there, e);
+      } else {
+        ch.store(tg, step, dg);
+        ch.store(ty, step, e);
+      }
+      arrived(rx); arrived(ry); arrived(rg); arrived(rd); arrived(rn);
     }
     if (a.shared_gate && a.d_gate && a.blocks_per_group == 1) {        // this workgroup has seen all rows of the gate's row
       slots_sum<T, L>(sg, comb, C, [&](int c, float v) { a.d_gate[g * C + c] = cpfn_from_f32<T>(v); });
@@ -242,36 +266,14 @@ template <typename T> __global__ __launch_bounds__(1024) void norm_residual_redu
   }
 }
 
-// How the rows are split over workgroups.
-struct NormSplit { long long groups, rows_per_gate, chunk; int nblk, blocks_per_group, groups_per_block; };
-NormSplit norm_split(long long P, int C, long long gate_rows) {
-  const int L = norm_lanes(C), threads = L <= 64 ? 256 : L, rows = threads / L;
-  const bool shared = gate_rows > 0 && gate_rows < P;
-  NormSplit s;
-  s.groups = shared ? gate_rows : 1;
-  s.rows_per_gate = P / s.groups;
-  const long long sets = (s.rows_per_gate + rows - 1) / rows;             // row sets of a group
-  const long long want = BWD_WAVES * 64 / threads;
-  long long bpg = (want + s.groups - 1) / s.groups;
-  if (bpg > (sets + 3) / 4) bpg = (sets + 3) / 4;                         // (at least four row sets each: the sums have to be paid for)
-  if (bpg < 1) bpg = 1;
-  s.chunk = (sets + bpg - 1) / bpg * rows;
-  bpg = (s.rows_per_gate + s.chunk - 1) / s.chunk;
-  s.blocks_per_group = (int)bpg;
-  s.groups_per_block = 1;
-  if (bpg == 1) {
-    const long long per = (s.groups + want - 1) / want;
-    s.groups_per_block = (int)per;
-    s.nblk = (int)((s.groups + per - 1) / per);
-  } else {
-    s.nblk = (int)(bpg * s.groups);
-  }
-  return s;
-}
+// two waves for each SIMD are resident together; at least four row sets for each workgroup, or its sums cost as much as its rows
+NormSplit split(long long P, int C, long long gate_rows) { return norm_split(P, C, gate_rows, 2048, 4); }
 
-template <typename T, int L> void launch(const NormBwd<T> &a, int nblk, hipStream_t st) {
-  if (a.C % cpfn_piece<T>::N) norm_residual_bwd_kernel<T, L, true><<<nblk, NormShape<T, L>::THREADS, 0, st>>>(a);
-  else norm_residual_bwd_kernel<T, L, false><<<nblk, NormShape<T, L>::THREADS, 0, st>>>(a);
+template <typename T, int L> void launch(const NormBwd<T> &a, int nblk, NormMode mode, hipStream_t st) {
+  constexpr int THREADS = NormShape<T, L>::THREADS;
+  if (mode == WHOLE) norm_residual_bwd_kernel<T, L, WHOLE><<<nblk, THREADS, 0, st>>>(a);
+  // (ragged fp32 rows of more than 2048 channels: the registers of 512 lanes do not hold what the piecewise form needs)
+  else norm_residual_bwd_kernel<T, L, L == 512 && sizeof(T) == 4 ? EACH : RAGGED><<<nblk, THREADS, 0, st>>>(a);
 }
 
 struct Grads { float *d_weight, *d_bias, *d_scale, *d_next_weight, *d_next_bias; };
@@ -280,7 +282,7 @@ template <typename T>
 int backward(const void *x, const void *y, const void *gate, const float *weight, const float *bias, const float *scale,
              const float *next_weight, const void *d_out, const void *d_normed, long long P, int C, long long gate_rows, int layer,
              int sigmoid, float eps, void *d_x, void *d_y, void *d_gate, const Grads &d, float *workspace, hipStream_t st) {
-  const NormSplit s = norm_split(P, C, gate_rows);
+  const NormSplit s = split(P, C, gate_rows);
   NormBwd<T> a;
   a.x = (const T *)x; a.y = (const T *)y; a.gate = (const T *)gate; a.d_out = (const T *)d_out; a.d_normed = (const T *)d_normed;
   a.weight = weight; a.bias = bias; a.scale = scale; a.next_weight = next_weight;
@@ -292,14 +294,19 @@ int backward(const void *x, const void *y, const void *gate, const float *weight
   a.shared_gate = gate && gate_rows < P;
   a.sums12 = d.d_weight || d.d_bias || d.d_scale;
   a.sums34 = d.d_next_weight || d.d_next_bias;
-  switch (norm_lanes(C)) {
-    case 8: launch<T, 8>(a, s.nblk, st); break;
-    case 16: launch<T, 16>(a, s.nblk, st); break;
-    case 32: launch<T, 32>(a, s.nblk, st); break;
-    case 64: launch<T, 64>(a, s.nblk, st); break;
-    case 128: launch<T, 128>(a, s.nblk, st); break;
-    case 256: launch<T, 256>(a, s.nblk, st); break;
-    default: launch<T, 512>(a, s.nblk, st); break;
+  const NormMode mode = norm_mode<T>(P, C, gate_rows);
+  if (mode == EACH) {
+    norm_residual_bwd_kernel<T, 8, EACH><<<s.nblk, 256, 0, st>>>(a);
+  } else {
+    switch (norm_lanes(C)) {
+      case 8: launch<T, 8>(a, s.nblk, mode, st); break;
+      case 16: launch<T, 16>(a, s.nblk, mode, st); break;
+      case 32: launch<T, 32>(a, s.nblk, mode, st); break;
+      case 64: launch<T, 64>(a, s.nblk, mode, st); break;
+      case 128: launch<T, 128>(a, s.nblk, mode, st); break;
+      case 256: launch<T, 256>(a, s.nblk, mode, st); break;
+      default: launch<T, 512>(a, s.nblk, mode, st); break;
+    }
   }
   const bool gate_part = a.shared_gate && d_gate && s.blocks_per_group > 1;
   if (a.sums12 || a.sums34 || gate_part) {
@@ -319,7 +326,7 @@ int backward(const void *x, const void *y, const void *gate, const float *weight
 extern "C" long long cpfn_norm_residual_workspace(long long P, int C, long long gate_rows) {
   if (P < 0 || C < 1 || C > CPFN_NORM_MAX_C || gate_rows < 0 || (gate_rows > 0 && P % gate_rows != 0)) return -1;
   if (P == 0) return 0;
-  return (long long)norm_split(P, C, gate_rows).nblk * 5 * C * (long long)sizeof(float);
+  return (long long)split(P, C, gate_rows).nblk * 5 * C * (long long)sizeof(float);
 }
 
 extern "C" int cpfn_norm_residual_bwd(const void *x, const void *y, const void *gate, const float *weight, const float *bias,

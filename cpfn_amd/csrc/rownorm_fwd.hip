@@ -5,116 +5,151 @@
 
 namespace {
 
-constexpr long long FWD_WAVES = 4096;         // waves of a launch: what is resident together
-
 template <typename T> struct NormFwd {
   const T *x, *y, *gate;
   const float *weight, *bias, *scale, *next_weight, *next_bias;
-  long long P, rows_per_gate, gate_rows;
+  long long P, rows_per_gate, groups, chunk;
+  int blocks_per_group, groups_per_block, shared_gate;
   int C, layer, sigmoid;
   float eps;
   T *out, *normed;
 };
 
-template <typename T, int L, bool RAGGED>
+template <typename T, int L, NormMode MODE>
 __global__ __launch_bounds__((NormShape<T, L>::THREADS)) void norm_residual_fwd_kernel(const NormFwd<T> a) {
-  constexpr int ROWS = NormShape<T, L>::ROWS;
-  __shared__ float2 slots[32];
+  constexpr int ROWS = NormShape<T, L>::ROWS, NP = NormShape<T, L>::NP;
+  __shared__ float2 slots[16];
   int turn = 0;
   const int lane = threadIdx.x & (L - 1), slot = threadIdx.x / L, C = a.C;
   const float inv_c = 1.f / (float)C;
-  const bool layer = a.layer != 0, post = a.weight != nullptr, has_y = a.y != nullptr;
-  const RowRaw<T, L> mask = row_mask<T, L, RAGGED>(lane, C);
-  // the rows of the NEXT step are requested before this one's are worked on
-  RowRaw<T, L> rx, ry, rg;
-  row_zero(rx); row_zero(ry); row_zero(rg);
-  const auto request = [&](long long r) {
-    if (r < a.P) {
-      row_load<T, L, RAGGED>(rx, a.x, r, a.P, lane, C, mask);
-      if (has_y) row_load<T, L, RAGGED>(ry, a.y, r, a.P, lane, C, mask);
-      if (a.gate) row_load<T, L, RAGGED>(rg, a.gate, norm_gate_row(r, a.rows_per_gate, a.P), a.gate_rows, lane, C, mask);
-    } else {
-      row_zero(rx); row_zero(ry); row_zero(rg);
-    }
-  };
-  const long long step = (long long)gridDim.x * ROWS;
-  long long base = (long long)blockIdx.x * ROWS;
-  request(base + slot);
+  const bool layer = a.layer != 0, post = a.weight != nullptr, has_y = a.y != nullptr, has_gate = a.gate != nullptr;
   float w[8], b[8], s[8], nw[8], nb[8];
-  param_load<T, L>(w, a.weight, lane, C, 1.f);
-  param_load<T, L>(b, a.bias, lane, C, 0.f);
-  param_load<T, L>(s, a.scale, lane, C, 1.f);
-  param_load<T, L>(nw, a.next_weight, lane, C, 1.f);
-  param_load<T, L>(nb, a.next_bias, lane, C, 0.f);
-  // (every row slot of a workgroup takes part in the barriers of row_sum: the loop runs over whole row sets)
-  for (; base < a.P; base += step) {
-    const long long r = base + slot;
-    const bool there = r < a.P;
-    const float eps = there ? a.eps : 1.f;
-    const RowRaw<T, L> cx = rx, cy = ry, cg = rg;
-    request(r + step);
-    float o[8];
-    row_unpack(cx, o);
-    if (has_y) {
-      float u[8];
-      row_unpack(cy, u);
-      if (post) {
-        row_normalise<T, L, RAGGED>(u, lane, C, inv_c, layer, eps, slots, turn);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) u[i] = fmaf(u[i], w[i], b[i]);
+  param_load<T, L, MODE != WHOLE>(w, a.weight, lane, C, 1.f);
+  param_load<T, L, MODE != WHOLE>(b, a.bias, lane, C, 0.f);
+  param_load<T, L, MODE != WHOLE>(s, a.scale, lane, C, 1.f);
+  param_load<T, L, MODE != WHOLE>(nw, a.next_weight, lane, C, 1.f);
+  param_load<T, L, MODE != WHOLE>(nb, a.next_bias, lane, C, 0.f);
+  const long long g0 = a.blocks_per_group > 1 ? blockIdx.x / a.blocks_per_group : (long long)blockIdx.x * a.groups_per_block;
+  long long g1 = a.blocks_per_group > 1 ? g0 + 1 : g0 + a.groups_per_block;
+  if (g1 > a.groups) g1 = a.groups;
+  const unsigned set_bytes = (unsigned)(ROWS * C) * (unsigned)sizeof(T);
+  for (long long g = g0; g < g1; ++g) {
+    long long row0 = g * a.rows_per_gate, row1 = row0 + a.rows_per_gate;
+    if (a.blocks_per_group > 1) {
+      row0 += (long long)(blockIdx.x % a.blocks_per_group) * a.chunk;
+      if (row0 + a.chunk < row1) row1 = row0 + a.chunk;
+    }
+    RowChunk<T, L, MODE> ch;
+    ch.begin(row0, row1, a.P, C, lane, slot);
+    const auto sx = ch.source(a.x), sy = ch.source(a.y), sg = ch.source(a.shared_gate ? nullptr : a.gate);
+    const auto to = ch.target(a.out), tn = ch.target(a.normed);
+    RowRaw<T, L> rx, ry, rg, shared;
+    unsigned o[NP], sh[NP];
+    const auto request = [&](unsigned step, long long r) {
+      if (MODE == EACH) {
+        each_load(rx, a.x, r, lane, C, r < row1);
+        each_load(ry, a.y, r, lane, C, r < row1);
+        each_load(rg, a.shared_gate ? nullptr : a.gate, r, lane, C, r < row1);
+      } else {
+        ch.at(o, sh, step, r < row1);
+        ch.load(rx, sx, o);
+        ch.load(ry, sy, o);
+        ch.load(rg, sg, o);
       }
-      if (a.gate) {
-        float g[8];
-        row_unpack(cg, g);
-        if (a.sigmoid) {
+    };
+    if (a.shared_gate) single_load<T, L>(shared, a.gate + g * C, lane, C);
+    float gs[8];
+    if (a.shared_gate) row_unpack(shared, gs);
+    if (a.shared_gate) arrived(gs);
+    arrived(w); arrived(b); arrived(s); arrived(nw); arrived(nb);
+    request(0, row0 + slot);
+    arrived(rx); arrived(ry); arrived(rg);
+    unsigned step = 0;
+    // (every row slot of a workgroup takes part in the barriers of row_sum: the loop runs over whole row sets)
+    for (long long base = row0; base < row1; base += ROWS, step += set_bytes) {
+      const long long r = base + slot;
+      const bool there = r < row1;
+      const float eps = there ? a.eps : 1.f;
+      RowRaw<T, L> cx = rx, cy = ry, cg = rg;
+      unsigned csh[NP];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) g[i] = norm_sigmoid<T>(g[i]);
+      for (int q = 0; q < NP; ++q) csh[q] = MODE == RAGGED ? sh[q] : 0u;
+      request(step + set_bytes, r + ROWS);
+      ch.settle(cx, csh);
+      float v[8], u[8];
+      row_unpack(cx, v);
+      if (has_y) {
+        ch.settle(cy, csh);
+        row_unpack(cy, u);
+        if (post) {
+          row_normalise<T, L, MODE>(u, lane, C, inv_c, layer, eps, slots, turn);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) u[i] = fmaf(u[i], w[i], b[i]);
+        }
+        if (has_gate) {
+          float gv[8];
+          ch.settle(cg, csh);
+          row_unpack(cg, gv);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float t = a.shared_gate ? gs[i] : gv[i];
+            u[i] *= a.sigmoid ? norm_sigmoid<T>(t) : t;
+          }
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) u[i] *= g[i];
+        for (int i = 0; i < 8; ++i) v[i] = fmaf(s[i], u[i], v[i]);
       }
+      if (MODE == EACH) each_store<T, L>(a.out, r, lane, C, there, v);
+      else ch.store(to, step, v);
+      if (a.normed) {
+        // (of the fp32 sum, not of its rounded copy in `out`)
+        row_normalise<T, L, MODE>(v, lane, C, inv_c, layer, eps, slots, turn);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) o[i] = fmaf(s[i], u[i], o[i]);
-      if (there) row_store<T, L, RAGGED>(a.out + r * C, lane, C, o);
-    }
-    if (a.normed) {
-      // (of the fp32 sum, not of its rounded copy in `out`)
-      row_normalise<T, L, RAGGED>(o, lane, C, inv_c, layer, eps, slots, turn);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) o[i] = fmaf(o[i], nw[i], nb[i]);
-      if (there) row_store<T, L, RAGGED>(a.normed + r * C, lane, C, o);
+        for (int i = 0; i < 8; ++i) v[i] = fmaf(v[i], nw[i], nb[i]);
+      }
+      if (MODE == EACH) each_store<T, L>(a.normed, r, lane, C, there, v);
+      else ch.store(tn, step, v);
+      arrived(rx); arrived(ry); arrived(rg);
     }
   }
 }
 
-template <typename T, int L> int launch(const NormFwd<T> &a, hipStream_t st) {
-  const long long sets = (a.P + NormShape<T, L>::ROWS - 1) / NormShape<T, L>::ROWS;
-  const long long most = FWD_WAVES * 64 / NormShape<T, L>::THREADS;
-  const unsigned blocks = (unsigned)(sets < most ? sets : most);
-  if (a.C % cpfn_piece<T>::N) norm_residual_fwd_kernel<T, L, true><<<blocks, NormShape<T, L>::THREADS, 0, st>>>(a);
-  else norm_residual_fwd_kernel<T, L, false><<<blocks, NormShape<T, L>::THREADS, 0, st>>>(a);
-  return cpfn_launch_status();
+constexpr int FWD_WAVES = 4096;             // resident together (four for each SIMD)
+
+template <typename T, int L> void launch(const NormFwd<T> &a, int nblk, NormMode mode, hipStream_t st) {
+  constexpr int THREADS = NormShape<T, L>::THREADS;
+  if (mode == WHOLE) norm_residual_fwd_kernel<T, L, WHOLE><<<nblk, THREADS, 0, st>>>(a);
+  else norm_residual_fwd_kernel<T, L, RAGGED><<<nblk, THREADS, 0, st>>>(a);
 }
 
 template <typename T>
 int forward(const void *x, const void *y, const void *gate, const float *weight, const float *bias, const float *scale,
             const float *next_weight, const float *next_bias, long long P, int C, long long gate_rows, int layer, int sigmoid, float eps,
             void *out, void *normed, hipStream_t st) {
+  if (!gate) gate_rows = 0;
+  const NormSplit s = norm_split(P, C, gate_rows, FWD_WAVES, 1);
   NormFwd<T> a;
   a.x = (const T *)x; a.y = (const T *)y; a.gate = (const T *)gate;
   a.weight = weight; a.bias = bias; a.scale = scale; a.next_weight = next_weight; a.next_bias = next_bias;
-  a.P = P; a.rows_per_gate = gate ? P / gate_rows : 1; a.gate_rows = gate_rows;
+  a.P = P; a.rows_per_gate = s.rows_per_gate; a.groups = s.groups; a.chunk = s.chunk;
+  a.blocks_per_group = s.blocks_per_group; a.groups_per_block = s.groups_per_block; a.shared_gate = gate && gate_rows < P;
   a.C = C; a.layer = layer; a.sigmoid = sigmoid; a.eps = eps;
   a.out = (T *)out; a.normed = (T *)normed;
-  switch (norm_lanes(C)) {
-    case 8: return launch<T, 8>(a, st);
-    case 16: return launch<T, 16>(a, st);
-    case 32: return launch<T, 32>(a, st);
-    case 64: return launch<T, 64>(a, st);
-    case 128: return launch<T, 128>(a, st);
-    case 256: return launch<T, 256>(a, st);
-    default: return launch<T, 512>(a, st);
+  const NormMode mode = norm_mode<T>(P, C, gate_rows);
+  if (mode == EACH) {
+    norm_residual_fwd_kernel<T, 8, EACH><<<s.nblk, 256, 0, st>>>(a);
+    return cpfn_launch_status();
   }
+  switch (norm_lanes(C)) {
+    case 8: launch<T, 8>(a, s.nblk, mode, st); break;
+    case 16: launch<T, 16>(a, s.nblk, mode, st); break;
+    case 32: launch<T, 32>(a, s.nblk, mode, st); break;
+    case 64: launch<T, 64>(a, s.nblk, mode, st); break;
+    case 128: launch<T, 128>(a, s.nblk, mode, st); break;
+    case 256: launch<T, 256>(a, s.nblk, mode, st); break;
+    default: launch<T, 512>(a, s.nblk, mode, st); break;
+  }
+  return cpfn_launch_status();
 }
 
 }  // namespace

@@ -36,18 +36,23 @@ template <> struct cpfn_piece<cpfn_f16> {
 __device__ __forceinline__ void cpfn_unpack(const cpfn_piece<float>::vec &r, float *f, float *) {
   f[0] = r.x; f[1] = r.y; f[2] = r.z; f[3] = r.w;
 }
+template <typename T> __device__ __forceinline__ float cpfn_half_lo(unsigned u);                // a word's two 16-bit elements
+template <typename T> __device__ __forceinline__ float cpfn_half_hi(unsigned u);
+template <> __device__ __forceinline__ float cpfn_half_lo<cpfn_bf16>(unsigned u) { return __uint_as_float(u << 16); }
+template <> __device__ __forceinline__ float cpfn_half_hi<cpfn_bf16>(unsigned u) { return __uint_as_float(u & 0xffff0000u); }
+template <> __device__ __forceinline__ float cpfn_half_lo<cpfn_f16>(unsigned u) { return (float)__builtin_bit_cast(_Float16, (unsigned short)u); }
+template <> __device__ __forceinline__ float cpfn_half_hi<cpfn_f16>(unsigned u) { return (float)__builtin_bit_cast(_Float16, (unsigned short)(u >> 16)); }
+template <> __device__ __forceinline__ float cpfn_half_lo<float>(unsigned u) { return 0.f; }    // (never called)
+template <> __device__ __forceinline__ float cpfn_half_hi<float>(unsigned u) { return 0.f; }
 __device__ __forceinline__ void cpfn_unpack(const cpfn_piece<cpfn_bf16>::vec &r, float *f, cpfn_bf16 *) {
   const unsigned u[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(u[i] << 16); f[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u); }
+  for (int i = 0; i < 4; ++i) { f[2 * i] = cpfn_half_lo<cpfn_bf16>(u[i]); f[2 * i + 1] = cpfn_half_hi<cpfn_bf16>(u[i]); }
 }
 __device__ __forceinline__ void cpfn_unpack(const cpfn_piece<cpfn_f16>::vec &r, float *f, cpfn_f16 *) {
   const unsigned u[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[2 * i] = (float)__builtin_bit_cast(_Float16, (unsigned short)(u[i] & 0xffffu));
-    f[2 * i + 1] = (float)__builtin_bit_cast(_Float16, (unsigned short)(u[i] >> 16));
-  }
+  for (int i = 0; i < 4; ++i) { f[2 * i] = cpfn_half_lo<cpfn_f16>(u[i]); f[2 * i + 1] = cpfn_half_hi<cpfn_f16>(u[i]); }
 }
 __device__ __forceinline__ cpfn_piece<float>::vec cpfn_pack(const float *f, float *) {
   cpfn_piece<float>::vec r;
@@ -96,34 +101,6 @@ template <typename T> __device__ __forceinline__ typename cpfn_piece<T>::vec cpf
 // (a vector's element goes through a value: __builtin_bit_cast of the element itself reads element 0 with this compiler)
 __device__ __forceinline__ unsigned cpfn_word(float v) { return __float_as_uint(v); }
 __device__ __forceinline__ unsigned cpfn_word(unsigned v) { return v; }
-__device__ __forceinline__ void cpfn_word_to(unsigned m, cpfn_piece<float>::vec &v, int i) { v[i] = __uint_as_float(m); }
-__device__ __forceinline__ void cpfn_word_to(unsigned m, cpfn_piece<cpfn_bf16>::vec &v, int i) { v[i] = m; }
-// the words of a piece that n of its elements fill (n >= N: all), as masks
-template <typename T> __device__ __forceinline__ typename cpfn_piece<T>::vec cpfn_piece_mask(int n) {
-  constexpr int PER = cpfn_piece<T>::N / 4;              // elements of a word
-  unsigned m[4];
-#pragma unroll
-  for (int w = 0; w < 4; ++w) m[w] = n >= (w + 1) * PER ? 0xffffffffu : PER == 2 && n == 2 * w + 1 ? 0xffffu : 0u;
-  typename cpfn_piece<T>::vec v;
-  cpfn_word_to(m[0], v, 0); cpfn_word_to(m[1], v, 1); cpfn_word_to(m[2], v, 2); cpfn_word_to(m[3], v, 3);
-  return v;
-}
-__device__ __forceinline__ float cpfn_and_word(float a, float m) { return __uint_as_float(__float_as_uint(a) & __float_as_uint(m)); }
-__device__ __forceinline__ unsigned cpfn_and_word(unsigned a, unsigned m) { return a & m; }
-// ... of a ragged row (C is no multiple of N): the whole 16 bytes are read wherever the tensor reaches that far — `room` elements from p
-// on —, what belongs to the next row is masked away; only at the very end of the tensor does it go element by element
-template <typename T>
-__device__ __forceinline__ typename cpfn_piece<T>::vec cpfn_load_ragged(const T *__restrict__ p, int at, int C, long long room,
-                                                                        const typename cpfn_piece<T>::vec &mask) {
-  typedef typename cpfn_piece<T>::vec V;
-  if (at < C && at + cpfn_piece<T>::N > room) return cpfn_load_piece(p, at, C);
-  V r = {};
-  if (at < C) {
-    r = *(const V *)(p + at);
-    r.x = cpfn_and_word(r.x, mask.x); r.y = cpfn_and_word(r.y, mask.y); r.z = cpfn_and_word(r.z, mask.z); r.w = cpfn_and_word(r.w, mask.w);
-  }
-  return r;
-}
 // 16 bytes, or the first C % N elements of them in one to three stores (which ones is the same for a whole launch)
 template <typename T> __device__ __forceinline__ void cpfn_store_piece(T *__restrict__ p, int at, int C, const float *f) {
   typedef typename cpfn_piece<T>::vec V;
