@@ -1,4 +1,4 @@
-// The norm over all gradients of a model, and their clipping, in two launches for up to LIST_MAX tensors of mixed types and lengths.
+// The norm over all gradients of a model, and their clipping, in two launches for each LIST_MAX tensors of mixed types and lengths.
 //
 //   norm = (sum |g|^p)^(1/p), p = 1, 2 or infinity (the largest |g|);   coef = min(1, max_norm / (norm + 1e-6));   out = coef g
 //
@@ -15,15 +15,17 @@
 
 namespace {
 
-constexpr int LIST_MAX = 128, GN_THREADS = 256;
+constexpr int LIST_MAX = 104, GN_THREADS = 256;        // (4 KB of kernel arguments)
 constexpr int SHARE = 16384;               // elements of a workgroup before the workgroups are limited ...
 constexpr int MOST_BLOCKS = 2048;          // ... to about so many in a call
+constexpr long long KEPT = 48ll << 20;     // elements at the end of the list that pass 1 leaves in the last-level cache (96 or 192 of its 256 MB)
 constexpr int DIRECT_PARTS = 1024;         // partial sums that the scaling workgroups add themselves; above, one launch in between does
 
 struct List {
   const void *src[LIST_MAX];
   void *dst[LIST_MAX];
   long long n[LIST_MAX];
+  long long from_end[LIST_MAX];            // elements of the whole call from the tensor's first one to the end of the list
   int block0[LIST_MAX + 1];                // first workgroup of each tensor
   unsigned char from[LIST_MAX], to[LIST_MAX];
   int count;
@@ -62,17 +64,18 @@ template <int P> __device__ __forceinline__ double gn_block(double v, double *ld
   return v;
 }
 
-// four 16-byte pieces of a tensor in flight for every lane
-template <int P, typename T> __device__ __forceinline__ double gn_share(const T *__restrict__ p, long long n, long long first, long long step) {
+// this lane's 16-byte pieces [first, end) of a tensor in steps of `step`, four in flight; ONCE: not kept in the caches
+template <int P, bool ONCE, typename T>
+__device__ __forceinline__ long long gn_pieces(const T *__restrict__ p, long long i, long long end, long long step, double (&acc)[4]) {
   constexpr int N = cpfn_piece<T>::N;
   typedef typename cpfn_piece<T>::vec V;
-  double acc[4] = {0.0, 0.0, 0.0, 0.0};
-  const long long whole = n / N;
-  long long i = first;
-  for (; i + 3 * step < whole; i += 4 * step) {
+  for (; i + 3 * step < end; i += 4 * step) {
     V v[4];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) v[q] = *(const V *)(p + (i + q * step) * N);
+    for (int q = 0; q < 4; ++q) {
+      const V *at = (const V *)(p + (i + q * step) * N);
+      v[q] = ONCE ? __builtin_nontemporal_load(at) : *at;
+    }
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       float f[N];
@@ -81,25 +84,37 @@ template <int P, typename T> __device__ __forceinline__ double gn_share(const T 
       for (int j = 0; j < N; ++j) acc[q] = gn_add<P>(acc[q], f[j]);
     }
   }
-  for (; i < whole; i += step) {
+  if (ONCE) return i;
+  for (; i < end; i += step) {
     float f[N];
     cpfn_unpack(*(const V *)(p + i * N), f, (T *)nullptr);
 #pragma unroll
     for (int j = 0; j < N; ++j) acc[0] = gn_add<P>(acc[0], f[j]);
   }
-  if (whole * N + first < n && first < N) acc[1] = gn_add<P>(acc[1], cpfn_to_f32(p[whole * N + first]));      // the last n % N
+  return i;
+}
+// keep: elements from here on are read a second time soon (the scaling pass), those before it are not kept
+template <int P, typename T> __device__ __forceinline__ double gn_share(const T *__restrict__ p, long long n, long long keep, long long first, long long step) {
+  constexpr int N = cpfn_piece<T>::N;
+  double acc[4] = {0.0, 0.0, 0.0, 0.0};
+  const long long whole = n / N;
+  const long long i = gn_pieces<P, true>(p, first, keep / N, step, acc);
+  gn_pieces<P, false>(p, i, whole, step, acc);
+  if (whole * N + first < n) acc[1] = gn_add<P>(acc[1], cpfn_to_f32(p[whole * N + first]));      // the last n % N
   return gn_join<P>(gn_join<P>(acc[0], acc[1]), gn_join<P>(acc[2], acc[3]));
 }
 
-template <int P> __global__ __launch_bounds__(GN_THREADS) void grad_norm_kernel(const List a, double *__restrict__ part) {
+template <int P> __global__ __launch_bounds__(GN_THREADS, 8) void grad_norm_kernel(const List a, long long kept, double *__restrict__ part) {
   __shared__ double lds[GN_THREADS / 64];
   const int d = list_find(a, blockIdx.x);
   const long long first = (long long)(blockIdx.x - a.block0[d]) * GN_THREADS + threadIdx.x;
   const long long step = (long long)(a.block0[d + 1] - a.block0[d]) * GN_THREADS;
+  // the last `kept` elements of this launch's list are the ones that the scaling pass begins with
+  const long long n = a.n[d], behind = a.from_end[d] - kept, keep = behind <= 0 ? 0 : behind < n ? behind : n;
   double v = 0.0;
-  if (a.from[d] == CPFN_F32) v = gn_share<P>((const float *)a.src[d], a.n[d], first, step);
-  else if (a.from[d] == CPFN_BF16) v = gn_share<P>((const cpfn_bf16 *)a.src[d], a.n[d], first, step);
-  else v = gn_share<P>((const cpfn_f16 *)a.src[d], a.n[d], first, step);
+  if (a.from[d] == CPFN_F32) v = gn_share<P>((const float *)a.src[d], n, keep, first, step);
+  else if (a.from[d] == CPFN_BF16) v = gn_share<P>((const cpfn_bf16 *)a.src[d], n, keep, first, step);
+  else v = gn_share<P>((const cpfn_f16 *)a.src[d], n, keep, first, step);
   v = gn_block<P>(v, lds);
   if (threadIdx.x == 0) part[blockIdx.x] = v;
 }
@@ -121,22 +136,43 @@ template <int P> __global__ __launch_bounds__(GN_THREADS) void grad_norm_finish_
   }
 }
 
+// Elements of a lane and step: 16 bytes on the wider side, so that the lanes of an access lie next to each other on both.  Four steps
+// in flight, from the tensor's end backwards (in place: T = U, every element is read before it is written).
 template <typename T, typename U>
 __device__ __forceinline__ void scale_share(const T *__restrict__ p, U *__restrict__ o, long long n, float coef, long long first, long long step) {
-  // eight elements a lane and step: 16 or 32 bytes in, 16 or 32 out (in place: T = U, every element is read before it is written)
-  const long long whole = n / 8;
-  for (long long i = first; i < whole; i += step) {
+  constexpr int N = cpfn_piece<T>::N < cpfn_piece<U>::N ? cpfn_piece<T>::N : cpfn_piece<U>::N, AHEAD = 4;
+  constexpr bool narrow = N * sizeof(T) == 8;                        // 8 bytes in, 16 out
+  typedef unsigned half __attribute__((ext_vector_type(2), aligned(2)));
+  typedef typename cpfn_piece<T>::vec V;
+  typedef typename cpfn_piece<U>::vec W;
+  const long long whole = n / N;
+  const auto one = [&](const V &v, long long i) {
     float f[8];
+    cpfn_unpack(v, f, (T *)nullptr);
 #pragma unroll
-    for (int q = 0; q < 8 / cpfn_piece<T>::N; ++q)
-      cpfn_unpack(*(const typename cpfn_piece<T>::vec *)(p + i * 8 + q * cpfn_piece<T>::N), f + q * cpfn_piece<T>::N, (T *)nullptr);
+    for (int j = 0; j < N; ++j) f[j] *= coef;
+    __builtin_nontemporal_store(cpfn_pack(f, (U *)nullptr), (W *)(o + i * N));
+  };
+  const auto get = [&](long long i) {
+    V v = {};
+    if (narrow) {
+      const half h = *(const half *)(p + i * N);
+      v.x = h.x; v.y = h.y;
+    } else {
+      v = *(const V *)(p + i * N);
+    }
+    return v;
+  };
+  long long i = whole - 1 - first;
+  for (; i - (AHEAD - 1) * step >= 0; i -= AHEAD * step) {
+    V v[AHEAD];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] *= coef;
+    for (int k = 0; k < AHEAD; ++k) v[k] = get(i - k * step);
 #pragma unroll
-    for (int q = 0; q < 8 / cpfn_piece<U>::N; ++q)
-      *(typename cpfn_piece<U>::vec *)(o + i * 8 + q * cpfn_piece<U>::N) = cpfn_pack(f + q * cpfn_piece<U>::N, (U *)nullptr);
+    for (int k = 0; k < AHEAD; ++k) one(v[k], i - k * step);
   }
-  if (first < n - whole * 8) o[whole * 8 + first] = cpfn_from_f32<U>(cpfn_to_f32(p[whole * 8 + first]) * coef);
+  for (; i >= 0; i -= step) one(get(i), i);
+  if (first < n - whole * N) o[whole * N + first] = cpfn_from_f32<U>(cpfn_to_f32(p[whole * N + first]) * coef);
 }
 
 // parts == 0: `part` is the norm itself.  elsewhere: the results go to other tensors (always written); in place nothing is to be done
@@ -204,7 +240,9 @@ bool overlapping(const void *const *src, void *const *dst, const long long *n, c
 }
 
 // tensors base.. of the list into `a`; returns the index behind the last one taken.  Empty tensors take no place.
-int fill(List &a, int base, const void *const *src, void *const *dst, const long long *n, const int *from, const int *to, int count, long long share) {
+// left: elements from tensor `base` on; taken down by what was put into `a`.
+int fill(List &a, int base, const void *const *src, void *const *dst, const long long *n, const int *from, const int *to, int count, long long share,
+         long long &left) {
   a.count = 0;
   a.block0[0] = 0;
   int i = base;
@@ -214,6 +252,8 @@ int fill(List &a, int base, const void *const *src, void *const *dst, const long
     a.src[c] = src[i];
     a.dst[c] = dst ? dst[i] : nullptr;
     a.n[c] = n[i];
+    a.from_end[c] = left;
+    left -= n[i];
     a.from[c] = (unsigned char)from[i];
     a.to[c] = (unsigned char)(to ? to[i] : from[i]);
     a.block0[c + 1] = a.block0[c] + blocks_of(n[i], share);
@@ -221,13 +261,22 @@ int fill(List &a, int base, const void *const *src, void *const *dst, const long
   return i;
 }
 
-template <int P> int norm_pass(const void *const *src, const long long *n, const int *type, int count, long long share, double *part, hipStream_t st) {
+long long sum_of(const long long *n, int count) {
+  long long sum = 0;
+  for (int i = 0; i < count; ++i) sum += n[i];
+  return sum;
+}
+
+// kept: so many elements from the list's end are read again soon
+template <int P>
+int norm_pass(const void *const *src, const long long *n, const int *type, int count, long long share, long long kept, double *part, hipStream_t st) {
   int parts = 0;
+  long long left = sum_of(n, count);
   for (int base = 0; base < count;) {
     List a;
-    base = fill(a, base, src, nullptr, n, type, nullptr, count, share);
+    base = fill(a, base, src, nullptr, n, type, nullptr, count, share, left);
     if (a.count == 0) break;
-    grad_norm_kernel<P><<<a.block0[a.count], GN_THREADS, 0, st>>>(a, part + parts);
+    grad_norm_kernel<P><<<a.block0[a.count], GN_THREADS, 0, st>>>(a, kept, part + parts);
     parts += a.block0[a.count];
   }
   return parts;
@@ -238,7 +287,7 @@ int run(const void *const *src, void *const *dst, const long long *n, const int 
         bool clip, bool elsewhere, float *norm, double *ws, hipStream_t st) {
   const long long share = share_of(n, count);
   double *part = ws + 1;
-  int parts = norm_pass<P>(src, n, from, count, share, part, st);
+  int parts = norm_pass<P>(src, n, from, count, share, clip ? KEPT : 0, part, st);
   if (!clip || parts > DIRECT_PARTS || parts == 0) {
     grad_norm_finish_kernel<P><<<1, GN_THREADS, 0, st>>>(part, parts, ws, norm);
     norm = nullptr;                                     // (written)
@@ -246,9 +295,10 @@ int run(const void *const *src, void *const *dst, const long long *n, const int 
     if (!clip || parts == 0) return cpfn_launch_status();
     parts = 0;
   }
+  long long left = sum_of(n, count);
   for (int base = 0; base < count;) {
     List a;
-    base = fill(a, base, src, dst, n, from, to, count, share);
+    base = fill(a, base, src, dst, n, from, to, count, share, left);
     if (a.count == 0) break;
     grad_scale_kernel<P><<<a.block0[a.count], GN_THREADS, 0, st>>>(a, part, parts, max_norm, elsewhere ? 1 : 0, norm);
     norm = nullptr;
@@ -306,6 +356,6 @@ extern "C" int cpfn_grad_sumsq(const float *g, long long n, double *parts, void 
   if (n < 0 || n > (1ll << 48) || (n > 0 && (!g || !parts)) || ((uintptr_t)parts & 7)) return CPFN_EINVAL;
   const void *src = g;
   const int type = CPFN_F32;
-  norm_pass<2>(&src, &n, &type, 1, share_of(&n, 1), parts, (hipStream_t)stream);
+  norm_pass<2>(&src, &n, &type, 1, share_of(&n, 1), n, parts, (hipStream_t)stream);
   return cpfn_launch_status();
 }

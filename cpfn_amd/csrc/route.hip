@@ -27,15 +27,17 @@ template <typename I> __device__ __forceinline__ int expert_of(const I *__restri
   return v >= 0 && v < (I)E ? (int)v : -1;
 }
 
-// mask of the lanes of this wave whose expert is this lane's (of lanes that have one)
+// mask of the lanes of this wave whose expert is this lane's (of lanes that have one): a lane keeps the lanes whose bit is its own
 __device__ __forceinline__ unsigned long long same_expert(int e, int bits) {
-  unsigned long long m = __ballot(e >= 0);
+  const unsigned long long valid = __ballot(e >= 0);
+  unsigned lo = (unsigned)valid, hi = (unsigned)(valid >> 32);
   for (int b = 0; b < bits; ++b) {
-    const bool one = (e >> b) & 1;
-    const unsigned long long v = __ballot(one);
-    m &= one ? v : ~v;
+    const unsigned mine = (unsigned)((e << (31 - b)) >> 31);                      // all ones: my bit is set
+    const unsigned long long v = __ballot(mine != 0u);
+    lo &= ~((unsigned)v ^ mine);
+    hi &= ~((unsigned)(v >> 32) ^ mine);
   }
-  return m;
+  return (unsigned long long)hi << 32 | lo;
 }
 
 // the ranks of a wave's choices among the wave's own; `mine`: the wave's counters, zero before, the wave's counts afterwards
@@ -86,19 +88,36 @@ __device__ __forceinline__ int wave_scan(int v, int lane) {                     
   return v;
 }
 
-// counts[e][0..tiles) -> exclusive sums over the tiles, totals[e]: one wave for each expert
-__global__ __launch_bounds__(256) void route_scan_kernel(int *__restrict__ counts, int *__restrict__ totals, int E, int tiles) {
-  const int e = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (e >= E) return;
+// counts[e][0..tiles) -> exclusive sums over the tiles, totals[e]: a workgroup for each expert, four tiles a lane and step
+__global__ __launch_bounds__(256) void route_scan_kernel(int *__restrict__ counts, int *__restrict__ totals, int tiles) {
+  __shared__ int wsum[2][4];
+  const int e = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int *row = counts + (long long)e * tiles;
-  int carry = 0;
-  for (int b = 0; b < tiles; b += 64) {
-    const int v = b + lane < tiles ? row[b + lane] : 0;
-    const int s = wave_scan(v, lane);
-    if (b + lane < tiles) row[b + lane] = carry + s - v;
-    carry += __shfl(s, 63, 64);
+  int carry = 0, turn = 0;
+  for (int b = 0; b < tiles; b += 1024, turn ^= 1) {
+    const int at = b + tid * 4;
+    int v[4], s = 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] = at + q < tiles ? row[at + q] : 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) s += v[q];
+    const int up_to = wave_scan(s, lane);
+    if (lane == 63) wsum[turn][wave] = up_to;
+    __syncthreads();
+    int before = carry + up_to - s;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const int x = wsum[turn][w];
+      if (w < wave) before += x;
+      carry += x;
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (at + q < tiles) row[at + q] = before;
+      before += v[q];
+    }
   }
-  if (lane == 0) totals[e] = carry;
+  if (tid == 0) totals[e] = carry;
 }
 
 // mode 0: one tile (its own counts are all there is); 1: sums the tiles' counts itself; 2: counts are exclusive sums, totals given
@@ -172,7 +191,7 @@ __global__ __launch_bounds__(RANK_WAVES * 64) void route_rank_kernel(const I *__
 }
 
 // ---------------------------------------------------------------- the moves
-constexpr int MOVE_THREADS = 256;
+constexpr int MOVE_THREADS = 256, MOVE_BLOCKS = 2048;
 
 // rows behind the last expert's, [offsets[E], n): zero, shared out over all row slots of the launch
 template <typename T>
@@ -185,137 +204,192 @@ __device__ __forceinline__ void zero_tail(T *__restrict__ out, const int *__rest
     for (int c = lane * cpfn_piece<T>::N; c < C; c += lanes * cpfn_piece<T>::N) cpfn_store_piece(out + p * C, c, C, z);
 }
 
-// LANES lanes per row, 16 bytes each and step
-template <typename T>
+// How a launch walks its rows: 1 << lanes_log2 lanes for a row, 16 bytes each and step; ROWS rows of a lane group in flight.
+struct Walk {
+  int lanes, lane;
+  long long slot, slots;
+  __device__ __forceinline__ explicit Walk(int lanes_log2) {
+    lanes = 1 << lanes_log2;
+    lane = threadIdx.x & (lanes - 1);
+    slot = (long long)blockIdx.x * (MOVE_THREADS >> lanes_log2) + (threadIdx.x >> lanes_log2);
+    slots = (long long)gridDim.x * (MOVE_THREADS >> lanes_log2);
+  }
+};
+
+// KT: choices of a row that are taken at once (their places in flight together)
+template <typename T, int KT>
 __global__ __launch_bounds__(MOVE_THREADS) void route_gather_kernel(const T *__restrict__ rows, const int *__restrict__ place,
                                                                     const int *__restrict__ end, long long R, int k, int C, int lanes_log2,
                                                                     T *__restrict__ out) {
-  constexpr int N = cpfn_piece<T>::N;
+  constexpr int N = cpfn_piece<T>::N, ROWS = KT <= 2 ? 4 : 2;
   typedef typename cpfn_piece<T>::vec V;                // (bits are moved, not values: NaNs keep theirs)
-  const int lanes = 1 << lanes_log2, lane = threadIdx.x & (lanes - 1);
-  const long long slot = (long long)blockIdx.x * (MOVE_THREADS >> lanes_log2) + (threadIdx.x >> lanes_log2);
-  const long long slots = (long long)gridDim.x * (MOVE_THREADS >> lanes_log2);
-  for (long long r = slot; r < R; r += slots) {
-    for (int c = lane * N; c < C; c += lanes * N) {
-      if (c + N <= C) {
-        const V v = *(const V *)(rows + r * C + c);
-        for (int j = 0; j < k; ++j) {
-          const int p = place[r * k + j];
-          if (p >= 0) *(V *)(out + (long long)p * C + c) = v;
+  const Walk w(lanes_log2);
+  for (long long r0 = w.slot; r0 < R; r0 += ROWS * w.slots) {
+    for (int j0 = 0; j0 < k; j0 += KT) {
+      int p[ROWS][KT];
+#pragma unroll
+      for (int u = 0; u < ROWS; ++u)
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+          const long long r = r0 + u * w.slots;
+          p[u][t] = r < R && j0 + t < k ? place[r * k + j0 + t] : -1;
         }
-      } else {                                          // the row ends inside this piece
-        for (int q = c; q < C; ++q) {
-          const T v = rows[r * C + q];
-          for (int j = 0; j < k; ++j) {
-            const int p = place[r * k + j];
-            if (p >= 0) out[(long long)p * C + q] = v;
+      for (int c = w.lane * N; c < C; c += w.lanes * N) {
+        if (c + N <= C) {
+          V v[ROWS];
+#pragma unroll
+          for (int u = 0; u < ROWS; ++u) {
+            const long long r = r0 + u * w.slots;
+            v[u] = *(const V *)(rows + (r < R ? r : R - 1) * C + c);
           }
+#pragma unroll
+          for (int u = 0; u < ROWS; ++u)
+#pragma unroll
+            for (int t = 0; t < KT; ++t)
+              if (p[u][t] >= 0) __builtin_nontemporal_store(v[u], (V *)(out + (long long)p[u][t] * C + c));
+        } else {                                        // the row ends inside this piece
+          for (int q = c; q < C; ++q)
+#pragma unroll
+            for (int u = 0; u < ROWS; ++u) {
+              const long long r = r0 + u * w.slots;
+              const T v = rows[(r < R ? r : R - 1) * C + q];
+#pragma unroll
+              for (int t = 0; t < KT; ++t)
+                if (p[u][t] >= 0) out[(long long)p[u][t] * C + q] = v;
+            }
         }
       }
     }
   }
-  zero_tail(out, end, R * k, C, lane, lanes, slot, slots);
+  zero_tail(out, end, R * k, C, w.lane, w.lanes, w.slot, w.slots);
 }
 
-template <typename T>
+template <typename T, int KT>
 __global__ __launch_bounds__(MOVE_THREADS) void route_combine_kernel(const T *__restrict__ sorted, const float *__restrict__ weights,
                                                                      const int *__restrict__ place, long long R, int k, int C,
                                                                      int lanes_log2, T *__restrict__ out) {
-  constexpr int N = cpfn_piece<T>::N, AHEAD = 4;        // rows of one sum in flight
-  const int lanes = 1 << lanes_log2, lane = threadIdx.x & (lanes - 1);
-  const long long slot = (long long)blockIdx.x * (MOVE_THREADS >> lanes_log2) + (threadIdx.x >> lanes_log2);
-  const long long slots = (long long)gridDim.x * (MOVE_THREADS >> lanes_log2);
-  for (long long r = slot; r < R; r += slots) {
-    for (int c = lane * N; c < C; c += lanes * N) {
-      float acc[N];
+  constexpr int N = cpfn_piece<T>::N, ROWS = KT <= 2 ? 4 : 2;
+  typedef typename cpfn_piece<T>::vec V;
+  const Walk walk(lanes_log2);
+  for (long long r0 = walk.slot; r0 < R; r0 += ROWS * walk.slots) {
+    int p[ROWS][KT];
+    float w[ROWS][KT];
+    const auto choices = [&](int j0) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) acc[i] = 0.f;
-      for (int j0 = 0; j0 < k; j0 += AHEAD) {
-        typename cpfn_piece<T>::vec v[AHEAD];
-        float w[AHEAD];
-        bool there[AHEAD];
+      for (int u = 0; u < ROWS; ++u)
 #pragma unroll
-        for (int t = 0; t < AHEAD; ++t) {
-          const int p = j0 + t < k ? place[r * k + j0 + t] : -1;
-          there[t] = p >= 0;
-          v[t] = {};
-          w[t] = 1.f;
-          if (there[t]) {
-            v[t] = cpfn_load_piece(sorted + (long long)p * C, c, C);
-            if (weights) w[t] = weights[r * k + j0 + t];
-          }
+        for (int t = 0; t < KT; ++t) {
+          const long long r = r0 + u * walk.slots;
+          const bool is = r < R && j0 + t < k;
+          const long long at = is ? r * k + j0 + t : 0;
+          p[u][t] = is ? place[at] : -1;
+          w[u][t] = weights ? weights[at] : 1.f;
         }
+    };
+    choices(0);
+    for (int c = walk.lane * N; c < C; c += walk.lanes * N) {
+      float acc[ROWS][N];
 #pragma unroll
-        for (int t = 0; t < AHEAD; ++t) {
-          if (there[t]) {                                // (a choice that is not there adds nothing, whatever its weight)
+      for (int u = 0; u < ROWS; ++u)
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[u][i] = 0.f;
+      for (int j0 = 0; j0 < k; j0 += KT) {
+        if (k > KT) choices(j0);
+        V v[ROWS][KT];
+#pragma unroll
+        for (int u = 0; u < ROWS; ++u)
+#pragma unroll
+          for (int t = 0; t < KT; ++t) v[u][t] = cpfn_load_piece(sorted + (long long)(p[u][t] < 0 ? 0 : p[u][t]) * C, c, C);
+#pragma unroll
+        for (int u = 0; u < ROWS; ++u)
+#pragma unroll
+          for (int t = 0; t < KT; ++t) {
             float f[N];
-            cpfn_unpack(v[t], f, (T *)nullptr);
+            cpfn_unpack(v[u][t], f, (T *)nullptr);
+            const bool is = p[u][t] >= 0;               // (a choice that is not there adds nothing, whatever stands in its places)
 #pragma unroll
-            for (int i = 0; i < N; ++i) acc[i] = fmaf(w[t], f[i], acc[i]);
+            for (int i = 0; i < N; ++i) acc[u][i] = is ? fmaf(w[u][t], f[i], acc[u][i]) : acc[u][i];
           }
-        }
       }
-      cpfn_store_piece(out + r * C, c, C, acc);
+#pragma unroll
+      for (int u = 0; u < ROWS; ++u) {
+        const long long r = r0 + u * walk.slots;
+        if (r < R) cpfn_store_piece(out + r * C, c, C, acc[u]);
+      }
     }
   }
 }
 
 // LANES <= 64: the products of a row meet inside a wave
-template <typename T, int LANES>
+template <typename T, int LANES, int KT>
 __global__ __launch_bounds__(MOVE_THREADS) void route_combine_bwd_kernel(const T *__restrict__ g, const T *__restrict__ sorted,
                                                                          const float *__restrict__ weights, const int *__restrict__ place,
                                                                          const int *__restrict__ end, long long R, int k, int C,
                                                                          T *__restrict__ d_sorted, float *__restrict__ d_weights) {
-  constexpr int N = cpfn_piece<T>::N, AHEAD = 4, ROWS = MOVE_THREADS / LANES;
+  constexpr int N = cpfn_piece<T>::N, GROUPS = MOVE_THREADS / LANES, ROWS = KT <= 2 ? 2 : 1;
+  typedef typename cpfn_piece<T>::vec V;
   const int lane = threadIdx.x & (LANES - 1);
-  const long long slot = (long long)blockIdx.x * ROWS + threadIdx.x / LANES, slots = (long long)gridDim.x * ROWS;
+  const long long slot = (long long)blockIdx.x * GROUPS + threadIdx.x / LANES, slots = (long long)gridDim.x * GROUPS;
   // (whole row sets: the lanes of a wave stay together for the row sums)
-  for (long long r0 = (long long)blockIdx.x * ROWS; r0 < R; r0 += slots) {
-    const long long r = r0 + threadIdx.x / LANES;
-    const bool row = r < R;
-    for (int j0 = 0; j0 < k; j0 += AHEAD) {
-      int p[AHEAD];
-      float w[AHEAD], dot[AHEAD];
+  for (long long s0 = (long long)blockIdx.x * GROUPS; s0 < R; s0 += ROWS * slots) {
+    const long long r0 = s0 + threadIdx.x / LANES;
+    for (int j0 = 0; j0 < k; j0 += KT) {
+      int p[ROWS][KT];
+      float w[ROWS][KT], dot[ROWS][KT];
 #pragma unroll
-      for (int t = 0; t < AHEAD; ++t) {
-        p[t] = row && j0 + t < k ? place[r * k + j0 + t] : -1;
-        w[t] = p[t] >= 0 && weights ? weights[r * k + j0 + t] : 1.f;
-        dot[t] = 0.f;
-      }
-      if (row) {
-        for (int c = lane * N; c < C; c += LANES * N) {
+      for (int u = 0; u < ROWS; ++u)
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+          const long long r = r0 + u * slots;
+          const bool is = r < R && j0 + t < k;
+          const long long at = is ? r * k + j0 + t : 0;
+          p[u][t] = is ? place[at] : -1;
+          w[u][t] = weights ? weights[at] : 1.f;
+          dot[u][t] = 0.f;
+        }
+      for (int c = lane * N; c < C; c += LANES * N) {
+        V gv[ROWS], v[ROWS][KT];
+#pragma unroll
+        for (int u = 0; u < ROWS; ++u) {
+          const long long r = r0 + u * slots;
+          gv[u] = cpfn_load_piece(g + (r < R ? r : R - 1) * C, c, C);
+        }
+        if (d_weights) {
+#pragma unroll
+          for (int u = 0; u < ROWS; ++u)
+#pragma unroll
+            for (int t = 0; t < KT; ++t) v[u][t] = cpfn_load_piece(sorted + (long long)(p[u][t] < 0 ? 0 : p[u][t]) * C, c, C);
+        }
+#pragma unroll
+        for (int u = 0; u < ROWS; ++u) {
           float gf[N];
-          cpfn_unpack(cpfn_load_piece(g + r * C, c, C), gf, (T *)nullptr);
-          typename cpfn_piece<T>::vec v[AHEAD];
+          cpfn_unpack(gv[u], gf, (T *)nullptr);
 #pragma unroll
-          for (int t = 0; t < AHEAD; ++t) {
-            v[t] = {};
-            if (d_weights && p[t] >= 0) v[t] = cpfn_load_piece(sorted + (long long)p[t] * C, c, C);
-          }
-#pragma unroll
-          for (int t = 0; t < AHEAD; ++t) {
-            if (p[t] < 0) continue;
-            if (d_weights) {
+          for (int t = 0; t < KT; ++t) {
+            if (d_weights) {                            // (of a choice that is not there the sum is not used)
               float f[N];
-              cpfn_unpack(v[t], f, (T *)nullptr);
+              cpfn_unpack(v[u][t], f, (T *)nullptr);
 #pragma unroll
-              for (int i = 0; i < N; ++i) dot[t] = fmaf(gf[i], f[i], dot[t]);
+              for (int i = 0; i < N; ++i) dot[u][t] = fmaf(gf[i], f[i], dot[u][t]);
             }
-            if (d_sorted) {
+            if (d_sorted && p[u][t] >= 0) {
               float f[N];
 #pragma unroll
-              for (int i = 0; i < N; ++i) f[i] = w[t] * gf[i];
-              cpfn_store_piece(d_sorted + (long long)p[t] * C, c, C, f);
+              for (int i = 0; i < N; ++i) f[i] = w[u][t] * gf[i];
+              cpfn_store_piece(d_sorted + (long long)p[u][t] * C, c, C, f);
             }
           }
         }
       }
       if (d_weights) {
 #pragma unroll
-        for (int t = 0; t < AHEAD; ++t) {
-          const float s = cpfn_lanes_sum<LANES>(dot[t]);
-          if (row && lane == 0 && j0 + t < k) d_weights[r * k + j0 + t] = p[t] >= 0 ? s : 0.f;
-        }
+        for (int u = 0; u < ROWS; ++u)
+#pragma unroll
+          for (int t = 0; t < KT; ++t) {
+            const long long r = r0 + u * slots;
+            const float sum = cpfn_lanes_sum<LANES>(dot[u][t]);
+            if (r < R && lane == 0 && j0 + t < k) d_weights[r * k + j0 + t] = p[u][t] >= 0 ? sum : 0.f;
+          }
       }
     }
   }
@@ -327,9 +401,10 @@ int lanes_log2_for(int C, int per_lane, int most) {
   while (l < most && (per_lane << l) < C) ++l;
   return l;
 }
+// as many workgroups as are resident together, or one row for each lane group
 unsigned move_blocks(long long R, int lanes_log2) {
   const long long rows = MOVE_THREADS >> lanes_log2, b = (R + rows - 1) / rows;
-  return (unsigned)(b < 8192 ? b : 8192);
+  return (unsigned)(b < MOVE_BLOCKS ? b : MOVE_BLOCKS);
 }
 
 template <typename I>
@@ -341,26 +416,35 @@ int plan(const I *choice, long long n, int E, int *offsets, int *place, int *ws,
   const int mode = tiles == 1 ? 0 : tiles <= DIRECT_TILES && E <= DIRECT_E ? 1 : 2;
   int *counts = ws, *totals = ws + (size_t)tiles * E;
   if (mode) route_count_kernel<I><<<tiles, RANK_WAVES * 64, (size_t)E * 4, st>>>(choice, n, E, tiles, counts);
-  if (mode == 2) route_scan_kernel<<<cpfn_cdiv(E, 4), 256, 0, st>>>(counts, totals, E, tiles);
+  if (mode == 2) route_scan_kernel<<<E, 256, 0, st>>>(counts, totals, tiles);
   route_rank_kernel<I><<<tiles, RANK_WAVES * 64, lds_rank, st>>>(choice, n, E, bits, tiles, mode, counts, totals, offsets, place);
   return cpfn_launch_status();
 }
 
 template <typename T> int gather(const void *rows, const int *place, const int *offsets, long long R, int k, int E, int C, void *out, hipStream_t st) {
   const int l = lanes_log2_for(C, cpfn_piece<T>::N, 8);
-  route_gather_kernel<T><<<move_blocks(R, l), MOVE_THREADS, 0, st>>>((const T *)rows, place, offsets + E, R, k, C, l, (T *)out);
+  const unsigned b = move_blocks(R, l);
+  if (k == 1) route_gather_kernel<T, 1><<<b, MOVE_THREADS, 0, st>>>((const T *)rows, place, offsets + E, R, k, C, l, (T *)out);
+  else if (k == 2) route_gather_kernel<T, 2><<<b, MOVE_THREADS, 0, st>>>((const T *)rows, place, offsets + E, R, k, C, l, (T *)out);
+  else route_gather_kernel<T, 4><<<b, MOVE_THREADS, 0, st>>>((const T *)rows, place, offsets + E, R, k, C, l, (T *)out);
   return cpfn_launch_status();
 }
 template <typename T> int combine(const void *sorted, const float *weights, const int *place, long long R, int k, int C, void *out, hipStream_t st) {
   const int l = lanes_log2_for(C, cpfn_piece<T>::N, 8);
-  route_combine_kernel<T><<<move_blocks(R, l), MOVE_THREADS, 0, st>>>((const T *)sorted, weights, place, R, k, C, l, (T *)out);
+  const unsigned b = move_blocks(R, l);
+  if (k == 1) route_combine_kernel<T, 1><<<b, MOVE_THREADS, 0, st>>>((const T *)sorted, weights, place, R, k, C, l, (T *)out);
+  else if (k == 2) route_combine_kernel<T, 2><<<b, MOVE_THREADS, 0, st>>>((const T *)sorted, weights, place, R, k, C, l, (T *)out);
+  else route_combine_kernel<T, 4><<<b, MOVE_THREADS, 0, st>>>((const T *)sorted, weights, place, R, k, C, l, (T *)out);
   return cpfn_launch_status();
 }
 template <typename T, int L>
 void combine_bwd_launch(const void *g, const void *sorted, const float *weights, const int *place, const int *end, long long R, int k, int C,
                         void *d_sorted, float *d_weights, int l, hipStream_t st) {
-  route_combine_bwd_kernel<T, L><<<move_blocks(R, l), MOVE_THREADS, 0, st>>>((const T *)g, (const T *)sorted, weights, place, end, R, k, C,
-                                                                            (T *)d_sorted, d_weights);
+  const unsigned b = move_blocks(R, l);
+  if (k <= 2)
+    route_combine_bwd_kernel<T, L, 2><<<b, MOVE_THREADS, 0, st>>>((const T *)g, (const T *)sorted, weights, place, end, R, k, C, (T *)d_sorted, d_weights);
+  else
+    route_combine_bwd_kernel<T, L, 4><<<b, MOVE_THREADS, 0, st>>>((const T *)g, (const T *)sorted, weights, place, end, R, k, C, (T *)d_sorted, d_weights);
 }
 template <typename T>
 int combine_bwd(const void *g, const void *sorted, const float *weights, const int *place, const int *offsets, long long R, int k, int E, int C,

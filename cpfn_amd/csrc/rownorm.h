@@ -130,9 +130,10 @@ template <typename T, int L, NormMode MODE> struct RowChunk {
       }
     }
   }
-  __device__ __forceinline__ void load(RowRaw<T, L> &raw, __amdgpu_buffer_rsrc_t rs, const unsigned *o) const {
+  // STREAM: the values are not kept in the caches (the last reader of whole rows; ragged rows share their cache lines)
+  template <bool STREAM = false> __device__ __forceinline__ void load(RowRaw<T, L> &raw, __amdgpu_buffer_rsrc_t rs, const unsigned *o) const {
 #pragma unroll
-    for (int q = 0; q < NP; ++q) raw.p[q] = __builtin_amdgcn_raw_buffer_load_b128(rs, o[q], 0, 0);
+    for (int q = 0; q < NP; ++q) raw.p[q] = __builtin_amdgcn_raw_buffer_load_b128(rs, o[q], 0, STREAM && MODE == WHOLE ? 2 : 0);
   }
   // what was loaded -> the row's values, zero behind its end
   __device__ __forceinline__ void settle(RowRaw<T, L> &raw, const unsigned *shift) const {
@@ -157,7 +158,7 @@ template <typename T, int L, NormMode MODE> struct RowChunk {
 #pragma unroll
     for (int q = 0; q < NP; ++q) {
       const cpfn_u32x4 v = piece_pack<T>(f + q * VN);
-      __builtin_amdgcn_raw_buffer_store_b128(v, rs, off[q] + step, 0, 0);
+      __builtin_amdgcn_raw_buffer_store_b128(v, rs, off[q] + step, 0, 2);       // (2: non-temporal)
       if (MODE == RAGGED) {                              // 8, 4 and 2 bytes of the partial piece, as C % VN says (the same for all rows)
         const unsigned n = (unsigned)(C % VN) * (unsigned)sizeof(T), t = tail[q] + step;
         const bool b8 = n & 8, b4 = n & 4, b2 = n & 2;

@@ -99,11 +99,11 @@ __global__ __launch_bounds__((NormShape<T, L>::THREADS)) void norm_residual_bwd_
         each_load(rn, a.d_normed, r, lane, C, r < row1);
       } else {
         ch.at(o, sh, step, r < row1);
-        ch.load(rx, bx, o);
-        ch.load(ry, by, o);
-        ch.load(rg, bg, o);
-        ch.load(rd, bd, o);
-        ch.load(rn, bn, o);
+        ch.template load<true>(rx, bx, o);
+        ch.template load<true>(ry, by, o);
+        ch.template load<true>(rg, bg, o);
+        ch.template load<true>(rd, bd, o);
+        ch.template load<true>(rn, bn, o);
       }
     };
     float gs[8];
@@ -239,7 +239,7 @@ template <typename T> __global__ __launch_bounds__(1024) void norm_residual_redu
   const int k = gate ? 4 : blockIdx.y * 2;
   double t1 = 0.0, t2 = 0.0;
   if (c < a.C) {
-#pragma unroll 4
+#pragma unroll 8
     for (int i = first + q; i < last; i += 64) {
       const float *p = a.part + ((size_t)i * a.nsums + k) * a.C + c;
       t1 += (double)p[0];

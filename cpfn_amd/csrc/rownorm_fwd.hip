@@ -114,7 +114,6 @@ __global__ __launch_bounds__((NormShape<T, L>::THREADS)) void norm_residual_fwd_
   }
 }
 
-constexpr int FWD_WAVES = 4096;             // resident together (four for each SIMD)
 
 template <typename T, int L> void launch(const NormFwd<T> &a, int nblk, NormMode mode, hipStream_t st) {
   constexpr int THREADS = NormShape<T, L>::THREADS;
@@ -127,7 +126,8 @@ int forward(const void *x, const void *y, const void *gate, const float *weight,
             const float *next_weight, const float *next_bias, long long P, int C, long long gate_rows, int layer, int sigmoid, float eps,
             void *out, void *normed, hipStream_t st) {
   if (!gate) gate_rows = 0;
-  const NormSplit s = norm_split(P, C, gate_rows, FWD_WAVES, 1);
+  const NormSplit s = norm_split(P, C, gate_rows, sizeof(T) == 4 ? 3072 : 4096, 1);       // waves that are resident together: three (fp32:
+                                                                                              // 130 to 154 registers) or four for each SIMD
   NormFwd<T> a;
   a.x = (const T *)x; a.y = (const T *)y; a.gate = (const T *)gate;
   a.weight = weight; a.bias = bias; a.scale = scale; a.next_weight = next_weight; a.next_bias = next_bias;
