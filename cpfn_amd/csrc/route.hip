@@ -13,11 +13,16 @@
 namespace {
 
 // ---------------------------------------------------------------- the order
-// A workgroup ranks TILE consecutive choices; a wave takes a contiguous part of them, 64 at a time.  Rank inside 64: the lanes with
+// A workgroup ranks a tile of consecutive choices; a wave takes a contiguous part of them, 64 at a time.  Rank inside 64: the lanes with
 // the same expert are found by one ballot for each bit of the index; the first such lane adds their number to the wave's own LDS
 // counter of that expert: no atomics, so the order is the input's order by construction.
-constexpr int RANK_WAVES = 8, RANK_ITEMS = 8, RANK_TILE = RANK_WAVES * RANK_ITEMS * 64;
-constexpr int ROUTE_MAX_E = 2048;                 // a 16-bit counter for each wave (a tile has 4096 choices) and a base: 40 KB of LDS
+// ITEMS: 64-choice steps of a wave.  4 up to RANK_SMALL choices (more workgroups: 60000 choices, 28 experts 10.6 -> 8.3 us), 8 above (fewer
+// counts to scan: 4000000 choices, 2000 experts 57 -> 44 us; 4194304, 128: 30.9 -> 30.5).
+constexpr int RANK_WAVES = 8;
+constexpr long long RANK_SMALL = 1 << 19;
+constexpr int rank_tile(int items) { return RANK_WAVES * items * 64; }
+int rank_items(long long n) { return n <= RANK_SMALL ? 4 : 8; }
+constexpr int ROUTE_MAX_E = 2048;                 // a 16-bit counter for each wave (a tile has 4096 choices at most) and a base: 40 KB of LDS
 // up to so many tiles and experts every workgroup sums the tiles' counts by itself, instead of a launch that does it once
 constexpr int DIRECT_TILES = 64, DIRECT_E = 256;
 
@@ -27,29 +32,25 @@ template <typename I> __device__ __forceinline__ int expert_of(const I *__restri
   return v >= 0 && v < (I)E ? (int)v : -1;
 }
 
-// mask of the lanes of this wave whose expert is this lane's (of lanes that have one): a lane keeps the lanes whose bit is its own
-__device__ __forceinline__ unsigned long long same_expert(int e, int bits) {
-  const unsigned long long valid = __ballot(e >= 0);
-  unsigned lo = (unsigned)valid, hi = (unsigned)(valid >> 32);
-  for (int b = 0; b < bits; ++b) {
-    const unsigned mine = (unsigned)((e << (31 - b)) >> 31);                      // all ones: my bit is set
-    const unsigned long long v = __ballot(mine != 0u);
-    lo &= ~((unsigned)v ^ mine);
-    hi &= ~((unsigned)(v >> 32) ^ mine);
-  }
-  return (unsigned long long)hi << 32 | lo;
-}
-
 // the ranks of a wave's choices among the wave's own; `mine`: the wave's counters, zero before, the wave's counts afterwards
-__device__ __forceinline__ void wave_ranks(const int *e, int *rank, unsigned short *mine, int bits, int lane) {
+template <int RANK_ITEMS> __device__ __forceinline__ void wave_ranks(const int *e, int *rank, unsigned short *mine, int bits) {
 #pragma unroll
   for (int t = 0; t < RANK_ITEMS; ++t) {
-    const unsigned long long m = same_expert(e[t], bits);
+    // the lanes whose expert is this lane's: for each bit, those whose bit is its own (of lanes that have an expert)
+    const unsigned long long valid = __ballot(e[t] >= 0);
+    unsigned lo = (unsigned)valid, hi = (unsigned)(valid >> 32);
+    for (int b = 0; b < bits; ++b) {
+      const unsigned own = (unsigned)__builtin_amdgcn_sbfe(e[t], b, 1);           // all ones: my bit is set
+      const unsigned long long v = __ballot(own != 0u);
+      lo &= ~((unsigned)v ^ own);
+      hi &= ~((unsigned)(v >> 32) ^ own);
+    }
+    const int ahead = (int)__builtin_amdgcn_mbcnt_hi(hi, __builtin_amdgcn_mbcnt_lo(lo, 0u));      // of them, those before this lane
     rank[t] = 0;
     if (e[t] >= 0) {
       const int before = mine[e[t]];
-      rank[t] = before + __popcll(m & ((1ull << lane) - 1ull));
-      if (__builtin_ctzll(m) == lane) mine[e[t]] = (unsigned short)(before + __popcll(m));
+      rank[t] = before + ahead;
+      if (ahead == 0) mine[e[t]] = (unsigned short)(before + __popc(lo) + __popc(hi));
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");      // the next 64 read what these wrote
     __builtin_amdgcn_wave_barrier();
@@ -61,13 +62,13 @@ __device__ __forceinline__ void zero_counters(unsigned short *cnt, int E) {     
   __syncthreads();
 }
 
-// counts[e][tile] (several tiles only): a histogram by LDS additions, whose order does not show in an integer
-template <typename I>
-__global__ __launch_bounds__(RANK_WAVES * 64) void route_count_kernel(const I *__restrict__ choice, long long n, int E, int tiles,
+// counts[tile][e] (several tiles only): a histogram by LDS additions, whose order does not show in an integer
+template <typename I, int RANK_ITEMS>
+__global__ __launch_bounds__(RANK_WAVES * 64) void route_count_kernel(const I *__restrict__ choice, long long n, int E,
                                                                       int *__restrict__ counts) {
   extern __shared__ unsigned lds[];               // [E]
   for (int x = threadIdx.x; x < E; x += RANK_WAVES * 64) lds[x] = 0u;
-  const long long i0 = (long long)blockIdx.x * RANK_TILE + threadIdx.x;
+  const long long i0 = (long long)blockIdx.x * rank_tile(RANK_ITEMS) + threadIdx.x;
   int e[RANK_ITEMS];
 #pragma unroll
   for (int t = 0; t < RANK_ITEMS; ++t) e[t] = expert_of(choice, i0 + t * (RANK_WAVES * 64), n, E);
@@ -76,7 +77,7 @@ __global__ __launch_bounds__(RANK_WAVES * 64) void route_count_kernel(const I *_
   for (int t = 0; t < RANK_ITEMS; ++t)
     if (e[t] >= 0) atomicAdd(&lds[e[t]], 1u);
   __syncthreads();
-  for (int x = threadIdx.x; x < E; x += RANK_WAVES * 64) counts[(long long)x * tiles + blockIdx.x] = (int)lds[x];
+  for (int x = threadIdx.x; x < E; x += RANK_WAVES * 64) counts[(long long)blockIdx.x * E + x] = (int)lds[x];
 }
 
 __device__ __forceinline__ int wave_scan(int v, int lane) {                       // inclusive
@@ -88,40 +89,41 @@ __device__ __forceinline__ int wave_scan(int v, int lane) {                     
   return v;
 }
 
-// counts[e][0..tiles) -> exclusive sums over the tiles, totals[e]: a workgroup for each expert, four tiles a lane and step
-__global__ __launch_bounds__(256) void route_scan_kernel(int *__restrict__ counts, int *__restrict__ totals, int tiles) {
-  __shared__ int wsum[2][4];
-  const int e = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  int *row = counts + (long long)e * tiles;
-  int carry = 0, turn = 0;
-  for (int b = 0; b < tiles; b += 1024, turn ^= 1) {
-    const int at = b + tid * 4;
-    int v[4], s = 0;
+// counts[0..tiles)[e] -> exclusive sums over the tiles, totals[e]: 16 experts x 64 stretches of tiles for each workgroup
+__global__ __launch_bounds__(1024) void route_scan_kernel(int *__restrict__ counts, int *__restrict__ totals, int E, int tiles) {
+  __shared__ int part[64][17];
+  const int x = threadIdx.x & 15, q = threadIdx.x >> 4, e = blockIdx.x * 16 + x;
+  const int per = (tiles + 63) / 64, t0 = q * per, t1 = t0 + per < tiles ? t0 + per : tiles;
+  int s = 0;
+  if (e < E) {
+#pragma unroll 16
+    for (int t = t0; t < t1; ++t) s += counts[(long long)t * E + e];
+  }
+  part[q][x] = s;
+  __syncthreads();
+  {                                                // a wave for each expert: the stretches' sums -> exclusive
+    const int lane = threadIdx.x & 63, wx = threadIdx.x >> 6;
+    const int v = part[lane][wx], up_to = wave_scan(v, lane);
+    part[lane][wx] = up_to - v;
+    if (lane == 63 && blockIdx.x * 16 + wx < E) totals[blockIdx.x * 16 + wx] = up_to;
+  }
+  __syncthreads();
+  if (e >= E) return;
+  s = part[q][x];
+  for (int t = t0; t < t1; t += 16) {
+    int v[16];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) v[q] = at + q < tiles ? row[at + q] : 0;
+    for (int i = 0; i < 16; ++i) v[i] = t + i < t1 ? counts[(long long)(t + i) * E + e] : 0;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) s += v[q];
-    const int up_to = wave_scan(s, lane);
-    if (lane == 63) wsum[turn][wave] = up_to;
-    __syncthreads();
-    int before = carry + up_to - s;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const int x = wsum[turn][w];
-      if (w < wave) before += x;
-      carry += x;
-    }
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      if (at + q < tiles) row[at + q] = before;
-      before += v[q];
+    for (int i = 0; i < 16; ++i) {
+      if (t + i < t1) counts[(long long)(t + i) * E + e] = s;
+      s += v[i];
     }
   }
-  if (tid == 0) totals[e] = carry;
 }
 
 // mode 0: one tile (its own counts are all there is); 1: sums the tiles' counts itself; 2: counts are exclusive sums, totals given
-template <typename I>
+template <typename I, int RANK_ITEMS>
 __global__ __launch_bounds__(RANK_WAVES * 64) void route_rank_kernel(const I *__restrict__ choice, long long n, int E, int bits, int tiles,
                                                                      int mode, const int *__restrict__ counts,
                                                                      const int *__restrict__ totals, int *__restrict__ offsets,
@@ -132,21 +134,21 @@ __global__ __launch_bounds__(RANK_WAVES * 64) void route_rank_kernel(const I *__
   unsigned short *cnt = (unsigned short *)lds;
   int *base = (int *)(lds + RANK_WAVES * E / 2);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const long long i0 = (long long)blockIdx.x * RANK_TILE + wave * (RANK_ITEMS * 64) + lane;
+  const long long i0 = (long long)blockIdx.x * rank_tile(RANK_ITEMS) + wave * (RANK_ITEMS * 64) + lane;
   unsigned short *mine = cnt + wave * E;
   int e[RANK_ITEMS], rank[RANK_ITEMS];
 #pragma unroll
   for (int t = 0; t < RANK_ITEMS; ++t) e[t] = expert_of(choice, i0 + t * 64, n, E);
   if (mode == 1) {                                // tiles <= 64: a lane for each tile, a wave for each expert
     for (int x = wave; x < E; x += RANK_WAVES) {
-      const int v = lane < tiles ? counts[x * tiles + lane] : 0;
+      const int v = lane < tiles ? counts[lane * E + x] : 0;
       const int s = wave_scan(v, lane);
       if (lane == (int)blockIdx.x) d_before[x] = s - v;
       if (lane == 63) d_total[x] = s;
     }
   }
   zero_counters(cnt, E);
-  wave_ranks(e, rank, mine, bits, lane);
+  wave_ranks<RANK_ITEMS>(e, rank, mine, bits);
   __syncthreads();
   // per expert: exclusive sums over the waves (in place), the tiles before this one, and the total; the totals' exclusive sum over
   // the experts is the expert's first position (a carry from one THREADS-wide step to the next)
@@ -163,7 +165,7 @@ __global__ __launch_bounds__(RANK_WAVES * 64) void route_rank_kernel(const I *__
         s += v;
       }
       total = mode == 0 ? s : mode == 1 ? d_total[x] : totals[x];
-      before = mode == 0 ? 0 : mode == 1 ? d_before[x] : counts[(long long)x * tiles + blockIdx.x];
+      before = mode == 0 ? 0 : mode == 1 ? d_before[x] : counts[(long long)blockIdx.x * E + x];
     }
     const int s = wave_scan(total, lane);
     if (lane == 63) wsum[wave] = s;
@@ -191,21 +193,14 @@ __global__ __launch_bounds__(RANK_WAVES * 64) void route_rank_kernel(const I *__
 }
 
 // ---------------------------------------------------------------- the moves
-constexpr int MOVE_THREADS = 256, MOVE_BLOCKS = 2048;
+// One row for each group of lanes of a launch (up to MOVE_BLOCKS workgroups; several rows in flight for a group, with fewer
+// workgroups, measured 0 to 40 % slower at 131072 x 128 .. 50000 x 1024 rows: the chip holds enough groups).  A row is walked in
+// 16-byte pieces; the last piece of a row whose length is no multiple of one ENDS with the row and overlaps the piece before it: its
+// lane moves (or computes) a few elements that another lane moves too, to the same value.  Rows shorter than a piece go element by element.
+constexpr int MOVE_THREADS = 256;
+constexpr long long MOVE_BLOCKS = 1 << 20;
 
-// rows behind the last expert's, [offsets[E], n): zero, shared out over all row slots of the launch
-template <typename T>
-__device__ __forceinline__ void zero_tail(T *__restrict__ out, const int *__restrict__ end, long long n, int C, int lane, int lanes,
-                                          long long slot, long long slots) {
-  float z[cpfn_piece<T>::N];
-#pragma unroll
-  for (int i = 0; i < cpfn_piece<T>::N; ++i) z[i] = 0.f;
-  for (long long p = *end + slot; p < n; p += slots)
-    for (int c = lane * cpfn_piece<T>::N; c < C; c += lanes * cpfn_piece<T>::N) cpfn_store_piece(out + p * C, c, C, z);
-}
-
-// How a launch walks its rows: 1 << lanes_log2 lanes for a row, 16 bytes each and step; ROWS rows of a lane group in flight.
-struct Walk {
+struct Walk {                     // 1 << lanes_log2 lanes for a row
   int lanes, lane;
   long long slot, slots;
   __device__ __forceinline__ explicit Walk(int lanes_log2) {
@@ -215,48 +210,49 @@ struct Walk {
     slots = (long long)gridDim.x * (MOVE_THREADS >> lanes_log2);
   }
 };
+template <typename T> __device__ __forceinline__ int piece_at(int c, int C) { return c + cpfn_piece<T>::N <= C ? c : C - cpfn_piece<T>::N; }
+
+// rows behind the last expert's, [offsets[E], n): zero, shared out over all row slots of the launch
+template <typename T>
+__device__ __forceinline__ void zero_tail(T *__restrict__ out, const int *__restrict__ end, long long n, int C, int lane, int lanes,
+                                          long long slot, long long slots) {
+  constexpr int N = cpfn_piece<T>::N;
+  const typename cpfn_piece<T>::vec z = {};
+  for (long long p = *end + slot; p < n; p += slots)
+    for (int c = lane * N; c < C; c += lanes * N) {
+      if (C >= N) *(typename cpfn_piece<T>::vec *)(out + p * C + piece_at<T>(c, C)) = z;
+      else
+        for (int q = 0; q < C; ++q) out[p * C + q] = cpfn_from_f32<T>(0.f);
+    }
+}
 
 // KT: choices of a row that are taken at once (their places in flight together)
 template <typename T, int KT>
 __global__ __launch_bounds__(MOVE_THREADS) void route_gather_kernel(const T *__restrict__ rows, const int *__restrict__ place,
                                                                     const int *__restrict__ end, long long R, int k, int C, int lanes_log2,
                                                                     T *__restrict__ out) {
-  constexpr int N = cpfn_piece<T>::N, ROWS = KT <= 2 ? 4 : 2;
+  constexpr int N = cpfn_piece<T>::N;
   typedef typename cpfn_piece<T>::vec V;                // (bits are moved, not values: NaNs keep theirs)
   const Walk w(lanes_log2);
-  for (long long r0 = w.slot; r0 < R; r0 += ROWS * w.slots) {
+  for (long long r = w.slot; r < R; r += w.slots) {
     for (int j0 = 0; j0 < k; j0 += KT) {
-      int p[ROWS][KT];
+      int p[KT];
 #pragma unroll
-      for (int u = 0; u < ROWS; ++u)
-#pragma unroll
-        for (int t = 0; t < KT; ++t) {
-          const long long r = r0 + u * w.slots;
-          p[u][t] = r < R && j0 + t < k ? place[r * k + j0 + t] : -1;
-        }
+      for (int t = 0; t < KT; ++t) p[t] = j0 + t < k ? place[r * k + j0 + t] : -1;
       for (int c = w.lane * N; c < C; c += w.lanes * N) {
-        if (c + N <= C) {
-          V v[ROWS];
+        if (C >= N) {
+          const int at = piece_at<T>(c, C);
+          const V v = *(const V *)(rows + r * C + at);
 #pragma unroll
-          for (int u = 0; u < ROWS; ++u) {
-            const long long r = r0 + u * w.slots;
-            v[u] = *(const V *)(rows + (r < R ? r : R - 1) * C + c);
-          }
-#pragma unroll
-          for (int u = 0; u < ROWS; ++u)
+          for (int t = 0; t < KT; ++t)
+            if (p[t] >= 0) __builtin_nontemporal_store(v, (V *)(out + (long long)p[t] * C + at));
+        } else {
+          for (int q = 0; q < C; ++q) {
+            const T v = rows[r * C + q];
 #pragma unroll
             for (int t = 0; t < KT; ++t)
-              if (p[u][t] >= 0) __builtin_nontemporal_store(v[u], (V *)(out + (long long)p[u][t] * C + c));
-        } else {                                        // the row ends inside this piece
-          for (int q = c; q < C; ++q)
-#pragma unroll
-            for (int u = 0; u < ROWS; ++u) {
-              const long long r = r0 + u * w.slots;
-              const T v = rows[(r < R ? r : R - 1) * C + q];
-#pragma unroll
-              for (int t = 0; t < KT; ++t)
-                if (p[u][t] >= 0) out[(long long)p[u][t] * C + q] = v;
-            }
+              if (p[t] >= 0) out[(long long)p[t] * C + q] = v;
+          }
         }
       }
     }
@@ -264,58 +260,55 @@ __global__ __launch_bounds__(MOVE_THREADS) void route_gather_kernel(const T *__r
   zero_tail(out, end, R * k, C, w.lane, w.lanes, w.slot, w.slots);
 }
 
+// a piece as floats, zeros behind a row shorter than a piece
+template <typename T> __device__ __forceinline__ void piece_get(const T *__restrict__ row, int at, int C, typename cpfn_piece<T>::vec &v) {
+  if (C >= cpfn_piece<T>::N) v = *(const typename cpfn_piece<T>::vec *)(row + at);
+  else v = cpfn_load_piece(row, 0, C);
+}
+template <typename T> __device__ __forceinline__ void piece_put(T *__restrict__ row, int at, int C, const float *f) {
+  if (C >= cpfn_piece<T>::N) __builtin_nontemporal_store(cpfn_pack(f, (T *)nullptr), (typename cpfn_piece<T>::vec *)(row + at));
+  else cpfn_store_piece(row, 0, C, f);
+}
+
 template <typename T, int KT>
 __global__ __launch_bounds__(MOVE_THREADS) void route_combine_kernel(const T *__restrict__ sorted, const float *__restrict__ weights,
                                                                      const int *__restrict__ place, long long R, int k, int C,
                                                                      int lanes_log2, T *__restrict__ out) {
-  constexpr int N = cpfn_piece<T>::N, ROWS = KT <= 2 ? 4 : 2;
-  typedef typename cpfn_piece<T>::vec V;
+  constexpr int N = cpfn_piece<T>::N;
   const Walk walk(lanes_log2);
-  for (long long r0 = walk.slot; r0 < R; r0 += ROWS * walk.slots) {
-    int p[ROWS][KT];
-    float w[ROWS][KT];
+  for (long long r = walk.slot; r < R; r += walk.slots) {
+    int p[KT];
+    float w[KT];
     const auto choices = [&](int j0) {
 #pragma unroll
-      for (int u = 0; u < ROWS; ++u)
-#pragma unroll
-        for (int t = 0; t < KT; ++t) {
-          const long long r = r0 + u * walk.slots;
-          const bool is = r < R && j0 + t < k;
-          const long long at = is ? r * k + j0 + t : 0;
-          p[u][t] = is ? place[at] : -1;
-          w[u][t] = weights ? weights[at] : 1.f;
-        }
+      for (int t = 0; t < KT; ++t) {
+        const bool is = j0 + t < k;
+        const long long at = r * k + (is ? j0 + t : 0);
+        p[t] = is ? place[at] : -1;
+        w[t] = weights ? weights[at] : 1.f;
+      }
     };
     choices(0);
     for (int c = walk.lane * N; c < C; c += walk.lanes * N) {
-      float acc[ROWS][N];
+      const int here = C >= N ? piece_at<T>(c, C) : 0;
+      float acc[N];
 #pragma unroll
-      for (int u = 0; u < ROWS; ++u)
-#pragma unroll
-        for (int i = 0; i < N; ++i) acc[u][i] = 0.f;
+      for (int i = 0; i < N; ++i) acc[i] = 0.f;
       for (int j0 = 0; j0 < k; j0 += KT) {
         if (k > KT) choices(j0);
-        V v[ROWS][KT];
+        typename cpfn_piece<T>::vec v[KT];
 #pragma unroll
-        for (int u = 0; u < ROWS; ++u)
+        for (int t = 0; t < KT; ++t) piece_get(sorted + (long long)(p[t] < 0 ? 0 : p[t]) * C, here, C, v[t]);
 #pragma unroll
-          for (int t = 0; t < KT; ++t) v[u][t] = cpfn_load_piece(sorted + (long long)(p[u][t] < 0 ? 0 : p[u][t]) * C, c, C);
+        for (int t = 0; t < KT; ++t) {
+          float f[N];
+          cpfn_unpack(v[t], f, (T *)nullptr);
+          const bool is = p[t] >= 0;                    // (a choice that is not there adds nothing, whatever stands in its places)
 #pragma unroll
-        for (int u = 0; u < ROWS; ++u)
-#pragma unroll
-          for (int t = 0; t < KT; ++t) {
-            float f[N];
-            cpfn_unpack(v[u][t], f, (T *)nullptr);
-            const bool is = p[u][t] >= 0;               // (a choice that is not there adds nothing, whatever stands in its places)
-#pragma unroll
-            for (int i = 0; i < N; ++i) acc[u][i] = is ? fmaf(w[u][t], f[i], acc[u][i]) : acc[u][i];
-          }
+          for (int i = 0; i < N; ++i) acc[i] = is ? fmaf(w[t], f[i], acc[i]) : acc[i];
+        }
       }
-#pragma unroll
-      for (int u = 0; u < ROWS; ++u) {
-        const long long r = r0 + u * walk.slots;
-        if (r < R) cpfn_store_piece(out + r * C, c, C, acc[u]);
-      }
+      piece_put(out + r * C, here, C, acc);
     }
   }
 }
@@ -326,70 +319,62 @@ __global__ __launch_bounds__(MOVE_THREADS) void route_combine_bwd_kernel(const T
                                                                          const float *__restrict__ weights, const int *__restrict__ place,
                                                                          const int *__restrict__ end, long long R, int k, int C,
                                                                          T *__restrict__ d_sorted, float *__restrict__ d_weights) {
-  constexpr int N = cpfn_piece<T>::N, GROUPS = MOVE_THREADS / LANES, ROWS = KT <= 2 ? 2 : 1;
+  constexpr int N = cpfn_piece<T>::N, GROUPS = MOVE_THREADS / LANES;
   typedef typename cpfn_piece<T>::vec V;
   const int lane = threadIdx.x & (LANES - 1);
   const long long slot = (long long)blockIdx.x * GROUPS + threadIdx.x / LANES, slots = (long long)gridDim.x * GROUPS;
   // (whole row sets: the lanes of a wave stay together for the row sums)
-  for (long long s0 = (long long)blockIdx.x * GROUPS; s0 < R; s0 += ROWS * slots) {
-    const long long r0 = s0 + threadIdx.x / LANES;
+  for (long long s0 = (long long)blockIdx.x * GROUPS; s0 < R; s0 += slots) {
+    const long long r = s0 + threadIdx.x / LANES;
+    const bool row = r < R;
     for (int j0 = 0; j0 < k; j0 += KT) {
-      int p[ROWS][KT];
-      float w[ROWS][KT], dot[ROWS][KT];
+      int p[KT];
+      float w[KT], dot[KT];
 #pragma unroll
-      for (int u = 0; u < ROWS; ++u)
-#pragma unroll
-        for (int t = 0; t < KT; ++t) {
-          const long long r = r0 + u * slots;
-          const bool is = r < R && j0 + t < k;
-          const long long at = is ? r * k + j0 + t : 0;
-          p[u][t] = is ? place[at] : -1;
-          w[u][t] = weights ? weights[at] : 1.f;
-          dot[u][t] = 0.f;
-        }
+      for (int t = 0; t < KT; ++t) {
+        const bool is = row && j0 + t < k;
+        const long long at = is ? r * k + j0 + t : 0;
+        p[t] = is ? place[at] : -1;
+        w[t] = weights ? weights[at] : 1.f;
+        dot[t] = 0.f;
+      }
       for (int c = lane * N; c < C; c += LANES * N) {
-        V gv[ROWS], v[ROWS][KT];
-#pragma unroll
-        for (int u = 0; u < ROWS; ++u) {
-          const long long r = r0 + u * slots;
-          gv[u] = cpfn_load_piece(g + (r < R ? r : R - 1) * C, c, C);
-        }
+        const int here = C >= N ? piece_at<T>(c, C) : 0, twice = c - here;        // elements that the lane before has too
+        V gv, v[KT];
+        piece_get(g + (row ? r : 0) * C, here, C, gv);
         if (d_weights) {
 #pragma unroll
-          for (int u = 0; u < ROWS; ++u)
-#pragma unroll
-            for (int t = 0; t < KT; ++t) v[u][t] = cpfn_load_piece(sorted + (long long)(p[u][t] < 0 ? 0 : p[u][t]) * C, c, C);
+          for (int t = 0; t < KT; ++t) piece_get(sorted + (long long)(p[t] < 0 ? 0 : p[t]) * C, here, C, v[t]);
         }
+        float gf[N];
+        cpfn_unpack(gv, gf, (T *)nullptr);
 #pragma unroll
-        for (int u = 0; u < ROWS; ++u) {
-          float gf[N];
-          cpfn_unpack(gv[u], gf, (T *)nullptr);
+        for (int t = 0; t < KT; ++t) {
+          if (d_weights) {                              // (of a choice that is not there the sum is not used)
+            float f[N];
+            cpfn_unpack(v[t], f, (T *)nullptr);
+            if (C % N && C >= N) {
 #pragma unroll
-          for (int t = 0; t < KT; ++t) {
-            if (d_weights) {                            // (of a choice that is not there the sum is not used)
-              float f[N];
-              cpfn_unpack(v[u][t], f, (T *)nullptr);
+              for (int i = 0; i < N; ++i) dot[t] = i >= twice ? fmaf(gf[i], f[i], dot[t]) : dot[t];
+            } else {
 #pragma unroll
-              for (int i = 0; i < N; ++i) dot[u][t] = fmaf(gf[i], f[i], dot[u][t]);
+              for (int i = 0; i < N; ++i) dot[t] = fmaf(gf[i], f[i], dot[t]);
             }
-            if (d_sorted && p[u][t] >= 0) {
-              float f[N];
+          }
+          if (d_sorted && p[t] >= 0) {
+            float f[N];
 #pragma unroll
-              for (int i = 0; i < N; ++i) f[i] = w[u][t] * gf[i];
-              cpfn_store_piece(d_sorted + (long long)p[u][t] * C, c, C, f);
-            }
+            for (int i = 0; i < N; ++i) f[i] = w[t] * gf[i];
+            piece_put(d_sorted + (long long)p[t] * C, here, C, f);
           }
         }
       }
       if (d_weights) {
 #pragma unroll
-        for (int u = 0; u < ROWS; ++u)
-#pragma unroll
-          for (int t = 0; t < KT; ++t) {
-            const long long r = r0 + u * slots;
-            const float sum = cpfn_lanes_sum<LANES>(dot[u][t]);
-            if (r < R && lane == 0 && j0 + t < k) d_weights[r * k + j0 + t] = p[u][t] >= 0 ? sum : 0.f;
-          }
+        for (int t = 0; t < KT; ++t) {
+          const float sum = cpfn_lanes_sum<LANES>(dot[t]);
+          if (row && lane == 0 && j0 + t < k) d_weights[r * k + j0 + t] = p[t] >= 0 ? sum : 0.f;
+        }
       }
     }
   }
@@ -401,24 +386,31 @@ int lanes_log2_for(int C, int per_lane, int most) {
   while (l < most && (per_lane << l) < C) ++l;
   return l;
 }
-// as many workgroups as are resident together, or one row for each lane group
 unsigned move_blocks(long long R, int lanes_log2) {
   const long long rows = MOVE_THREADS >> lanes_log2, b = (R + rows - 1) / rows;
   return (unsigned)(b < MOVE_BLOCKS ? b : MOVE_BLOCKS);
 }
 
-template <typename I>
+int tiles_of(long long n) {
+  const int tile = rank_tile(rank_items(n));
+  return n > tile ? (int)((n + tile - 1) / tile) : 1;
+}
+
+template <typename I, int ITEMS>
 int plan(const I *choice, long long n, int E, int *offsets, int *place, int *ws, hipStream_t st) {
-  const int tiles = n > RANK_TILE ? (int)((n + RANK_TILE - 1) / RANK_TILE) : 1;
+  const int tiles = tiles_of(n);
   int bits = 0;
   while ((1 << bits) < E) ++bits;
   const size_t lds_rank = (size_t)RANK_WAVES * E * 2 + (size_t)E * 4;
   const int mode = tiles == 1 ? 0 : tiles <= DIRECT_TILES && E <= DIRECT_E ? 1 : 2;
   int *counts = ws, *totals = ws + (size_t)tiles * E;
-  if (mode) route_count_kernel<I><<<tiles, RANK_WAVES * 64, (size_t)E * 4, st>>>(choice, n, E, tiles, counts);
-  if (mode == 2) route_scan_kernel<<<E, 256, 0, st>>>(counts, totals, tiles);
-  route_rank_kernel<I><<<tiles, RANK_WAVES * 64, lds_rank, st>>>(choice, n, E, bits, tiles, mode, counts, totals, offsets, place);
+  if (mode) route_count_kernel<I, ITEMS><<<tiles, RANK_WAVES * 64, (size_t)E * 4, st>>>(choice, n, E, counts);
+  if (mode == 2) route_scan_kernel<<<cpfn_cdiv(E, 16), 1024, 0, st>>>(counts, totals, E, tiles);
+  route_rank_kernel<I, ITEMS><<<tiles, RANK_WAVES * 64, lds_rank, st>>>(choice, n, E, bits, tiles, mode, counts, totals, offsets, place);
   return cpfn_launch_status();
+}
+template <typename I> int plan(const I *choice, long long n, int E, int *offsets, int *place, int *ws, hipStream_t st) {
+  return rank_items(n) == 4 ? plan<I, 4>(choice, n, E, offsets, place, ws, st) : plan<I, 8>(choice, n, E, offsets, place, ws, st);
 }
 
 template <typename T> int gather(const void *rows, const int *place, const int *offsets, long long R, int k, int E, int C, void *out, hipStream_t st) {
@@ -469,12 +461,12 @@ bool bad_sizes(long long R, int k, int E, int C) {
 
 extern "C" long long cpfn_route_workspace(long long n, int E) {
   if (n < 0 || n > 0x7fffffffll || E < 1 || E > ROUTE_MAX_E) return -1;
-  const long long tiles = (n + RANK_TILE - 1) / RANK_TILE;
+  const long long tiles = tiles_of(n);
   return tiles <= 1 ? 0 : (tiles + 1) * E * (long long)sizeof(int);
 }
 
 extern "C" int cpfn_route_plan(const void *choice, int wide, long long n, int E, int *offsets, int *place, void *workspace, void *stream) {
-  if (bad_sizes(n, 1, E, 1) || !offsets || (n > 0 && (!choice || !place)) || (n > RANK_TILE && !workspace)) return CPFN_EINVAL;
+  if (bad_sizes(n, 1, E, 1) || !offsets || (n > 0 && (!choice || !place)) || (tiles_of(n) > 1 && !workspace)) return CPFN_EINVAL;
   hipStream_t st = (hipStream_t)stream;
   return wide ? plan((const long long *)choice, n, E, offsets, place, (int *)workspace, st)
               : plan((const int *)choice, n, E, offsets, place, (int *)workspace, st);
