@@ -286,37 +286,7 @@ gather_rows = GatherRows.apply
 
 
 # ----------------------------------------------------------- a routed residual block's row operators
-class NormResidual(torch.autograd.Function):
-    """The end of a residual block and the norm of the next one in one launch each way (ops.norm_residual_fwd / _bwd).  Only the inputs
-    are kept for the backward pass: out, the normalised rows and both norms' statistics are formed again from them, in fp32 as the
-    forward pass had them."""
-
-    @staticmethod
-    def forward(ctx, x, y, weight, bias, gate, scale, next_weight, next_bias, gate_act, kind, eps):
-        x = x.contiguous()
-        y = None if y is None else y.contiguous()
-        gate = None if gate is None else gate.contiguous()
-        out, normed = ops.norm_residual_fwd(x, y, weight, bias, gate, gate_act, scale, next_weight, next_bias, kind, eps)
-        ctx.save_for_backward(x, y, weight, bias, gate, scale, next_weight)
-        ctx.how = (gate_act, kind, eps)
-        ctx.set_materialize_grads(False)
-        return out, normed
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, d_out, d_normed):
-        x, y, weight, bias, gate, scale, next_weight = ctx.saved_tensors
-        gate_act, kind, eps = ctx.how
-        if d_out is None and d_normed is None:
-            return (None,) * 11
-        names = ("x", "y", "weight", "bias", "gate", "scale", "next_weight", "next_bias")
-        needs = [n for n, need in zip(names, ctx.needs_input_grad) if need]
-        got = ops.norm_residual_bwd(x, y, weight, bias, gate, gate_act, scale, next_weight,
-                                    None if d_out is None else d_out.contiguous(),
-                                    None if d_normed is None else d_normed.contiguous(), kind, eps, needs)
-        return tuple(got.get(n) for n in names) + (None, None, None)
-
-
+# (the autograd nodes: csrc/native.cpp; rows that are not contiguous are copied, as by the nodes above)
 def norm_residual(x, y, weight=None, bias=None, gate=None, gate_act="none", scale=None, next_weight=None, next_bias=None, kind="rms",
                   eps=1e-5):
     """The rows x [P, C] that run past a residual block and the block's result y [P, C] (fp32, bf16 or fp16) -> (out, normed):
@@ -326,63 +296,29 @@ def norm_residual(x, y, weight=None, bias=None, gate=None, gate_act="none", scal
 
     norm(v; w, b) = (v - mu) / sqrt(mean((v - mu)^2) + eps) * w + b over the channels, mu = 0 (kind="rms") or the mean ("layer"); without
     a weight y is taken as it is.  gate: [P, C], or [G, C] shared by P / G consecutive rows each (a gate for each cloud), through
-    gate_act ("none" or "sigmoid").  scale, weight, bias, next_weight, next_bias: fp32 [C].  fp32 arithmetic; `normed` is the norm of the
-    unrounded sum.  Differentiable in all tensors, once."""
-    return NormResidual.apply(x, y, weight, bias, gate, scale, next_weight, next_bias, gate_act, kind, eps)
+    gate_act ("none" or "sigmoid").  scale, weight, bias, next_weight, next_bias: fp32 [C], C <= 4096.  fp32 arithmetic; `normed` is the
+    norm of the unrounded sum.  One launch forward; backward one and a small one.  Only the inputs are kept for it: out, the normalised
+    rows and the statistics are formed again.  Differentiable in all tensors, once."""
+    layer, sigmoid = ops._norm_how(kind, gate_act)
+    return ops._native_call("norm_residual", x, y, weight, bias, gate, sigmoid, scale, next_weight, next_bias, layer, eps)
 
 
 def row_norm(x, weight, bias=None, kind="rms", eps=1e-5):
     """norm(x; weight, bias) over the channels of rows x [P, C]: the norm in front of a block (norm_residual gives the following blocks
     theirs)."""
-    return NormResidual.apply(x, None, None, None, None, None, weight, bias, "none", kind, eps)[1]
-
-
-class RouteGather(torch.autograd.Function):
-    """rows [R, C] -> rows in the order of their experts [R k, C]; adjoint: each row's sum over its places (no atomics)."""
-
-    @staticmethod
-    def forward(ctx, rows, plan):
-        out = ops.route_gather_fwd(rows.contiguous(), plan)
-        ctx.save_for_backward(plan.offsets, plan.place)
-        ctx.n_experts = plan.n_experts
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g):
-        return ops.route_combine_fwd(g.contiguous(), None, ops.RoutePlan(*ctx.saved_tensors, ctx.n_experts)), None
-
-
-class RouteCombine(torch.autograd.Function):
-    """rows in the order of their experts [R k, C], weights [R, k] f32 or None -> [R, C]; one launch for both gradients."""
-
-    @staticmethod
-    def forward(ctx, sorted_rows, weights, plan):
-        sorted_rows = sorted_rows.contiguous()
-        weights = None if weights is None else weights.contiguous()
-        out = ops.route_combine_fwd(sorted_rows, weights, plan)
-        ctx.save_for_backward(sorted_rows if ctx.needs_input_grad[1] else None, weights, plan.offsets, plan.place)
-        ctx.n_experts = plan.n_experts
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g):
-        sorted_rows, weights, offsets, place = ctx.saved_tensors
-        need_rows, need_weights = ctx.needs_input_grad[:2]
-        d_rows, d_weights = ops.route_combine_bwd(g.contiguous(), sorted_rows, weights, ops.RoutePlan(offsets, place, ctx.n_experts),
-                                                  need_rows, need_weights)
-        return d_rows, d_weights, None
+    layer, _ = ops._norm_how(kind, "none")
+    return ops._native_call("norm_residual", x, None, None, None, None, False, None, weight, bias, layer, eps)[1]
 
 
 def route_gather(rows, plan):
     """rows [R, C] -> [R k, C], sorted by expert (ops.route_plan): what the experts' layers take.  The rows behind plan.offsets[-1],
-    which belong to choices that are not routed, are zero, and their gradients are not looked at."""
-    return RouteGather.apply(rows, plan)
+    which belong to choices that are not routed, are zero, and their gradients are not looked at.  Adjoint: each row's sum over its
+    places (no atomics)."""
+    return ops._native_call("route_gather", rows, *ops._plan(plan))
 
 
 def route_combine(sorted_rows, weights, plan):
     """The experts' results [R k, C] -> [R, C]: each row's weighted sum over its choices; weights [R, k] f32 (the router's), or None for
-    a plain sum.  Differentiable in sorted_rows and weights; the gradient of rows behind plan.offsets[-1] is zero, and what they hold is
-    not looked at."""
-    return RouteCombine.apply(sorted_rows, weights, plan)
+    a plain sum.  Differentiable in sorted_rows and weights (one launch for both gradients); the gradient of rows behind
+    plan.offsets[-1] is zero, and what they hold is not looked at."""
+    return ops._native_call("route_combine", sorted_rows, weights, *ops._plan(plan))

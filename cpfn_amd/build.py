@@ -18,7 +18,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(CSRC, "build")
 SO = os.path.join(HERE, "libcpfn_hip.so")
-TABLES = os.path.join(HERE, "_tables.so")
+NATIVE = os.path.join(HERE, "_native.so")
 ARCH = "gfx950"
 
 # no packed fp32 instructions at all (v_pk_{add,mul,fma}_f32 have given wrong results on this hardware now and then)
@@ -141,31 +141,30 @@ def _check_isa(src):
             os.remove(os.path.join(OBJ, f))
 
 
-def _build_tables(force):
-    """_tables.so (csrc/tables.cpp): a CPython extension over torch's own headers; host code only."""
+def _build_native(force):
+    """_native.so (csrc/native.cpp): the torch extension over the C ABI; host code only, linked to libcpfn_hip.so beside it."""
     import sysconfig
-    src = os.path.join(CSRC, "tables.cpp")
-    if not force and not _stale(TABLES, [src]):
+    src = os.path.join(CSRC, "native.cpp")
+    if not force and not _stale(NATIVE, [src, os.path.join(HERE, "..", "include", "cpfn_hip.h")]):
         return
     import torch
     from torch.utils.cpp_extension import include_paths
-    cmd = ["g++", "-O2", "-fPIC", "-shared", "-std=c++17", "-fvisibility=hidden", "-Wall",
-           "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI, "-I" + sysconfig.get_paths()["include"]]
-    for d in include_paths():
+    cmd = ["g++", "-O2", "-fPIC", "-shared", "-std=c++17", "-fvisibility=hidden", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+           "-DTORCH_EXTENSION_NAME=_native", "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI]
+    for d in include_paths() + [os.path.join(os.path.dirname(os.path.dirname(_hipcc())), "include"), sysconfig.get_paths()["include"]]:
         cmd += ["-isystem", d]
-    cmd += [src, "-o", TABLES, "-L" + os.path.join(os.path.dirname(torch.__file__), "lib"), "-lc10", "-ltorch_cpu", "-ltorch_python"]
+    cmd += [src, "-o", NATIVE, "-L" + os.path.join(os.path.dirname(torch.__file__), "lib"), "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip",
+            "-ltorch", "-ltorch_python", "-L" + HERE, "-l:libcpfn_hip.so", "-Wl,-rpath,$ORIGIN"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError("g++ failed for tables.cpp:\n%s" % r.stderr[-4000:])
+        raise RuntimeError("g++ failed for native.cpp:\n%s" % r.stderr[-4000:])
 
 
 def build(force=False, verbose=False):
     os.makedirs(OBJ, exist_ok=True)
     srcs = {s: f for s, f in SOURCES.items() if os.path.exists(os.path.join(CSRC, s))}
     with ThreadPoolExecutor(max_workers=min(6, len(srcs))) as ex:
-        tables = ex.submit(_build_tables, force)
         res = list(ex.map(lambda kv: _compile(kv[0], kv[1], force), srcs.items()))
-        tables.result()
     objs = [o for o, _ in res]
     if force or any(c for _, c in res) or _stale(SO, objs):
         cmd = [_hipcc(), "--offload-arch=" + ARCH, "-shared", "-fPIC", "-o", SO] + objs
@@ -174,6 +173,7 @@ def build(force=False, verbose=False):
             raise RuntimeError("link failed:\n%s" % r.stderr[-4000:])
         if verbose:
             print("linked", SO)
+    _build_native(force)
     return SO
 
 

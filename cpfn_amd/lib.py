@@ -192,6 +192,7 @@ def time_symbols(names):
     for n in names:
         _timed[n] = []
         _bytes[n] = 0
+    _count_native()
 
 
 def add_bytes(name, nbytes):
@@ -205,9 +206,10 @@ def add_bytes(name, nbytes):
         ent[1] += int(nbytes)
 
 
-def counting():
-    """Is anybody counting algorithmic bytes?  (For callers whose sum takes longer than asking.)"""
-    return _census is not None or bool(_bytes)
+def _count_native():
+    """The launches of _native.so report to add_bytes while anybody counts.  (time_symbols' events bracket ctypes calls only.)"""
+    if _native is not None:
+        _native.set_counter(add_bytes if _census is not None or _bytes else None)
 
 
 def timed_bytes(name):
@@ -220,8 +222,10 @@ def byte_census(on):
     global _census
     if on:
         _census = {}
+        _count_native()
         return None
     out, _census = _census, None
+    _count_native()
     return {k: tuple(v) for k, v in (out or {}).items()}
 
 
@@ -292,8 +296,24 @@ def lib():
     return _lib
 
 
+_native = None
+
+
+def native():
+    """The torch extension over the C ABI (csrc/native.cpp), loaded once behind lib().  Raises if it is missing."""
+    global _native
+    if _native is None:
+        lib()
+        try:
+            from . import _native as n
+        except ImportError as e:
+            raise CpfnHipError("cpfn_amd/_native.so cannot be loaded (%s): run `python -m cpfn_amd.build`. There is no fallback." % e) from e
+        _native = n
+        _count_native()
+    return _native
+
+
 def check(status, what):
     if status != 0:
         raise CpfnHipError("%s failed with status %d%s" % (
-            what, status, {-22: " (invalid argument)", -16: " (a tensor that is written shares memory with another one of the lists: "
-                           "a gradient listed twice?)"}.get(status, " (hipError_t)")))
+            what, status, " (invalid argument)" if status == -22 else " (hipError_t)"))

@@ -400,73 +400,24 @@ def csr_build(idx, M):
 
 
 # ----------------------------------------------------------- norms around a residual block, rows sorted by expert and back
-ROW_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # CPFN_F32 / CPFN_BF16 / CPFN_F16
-NORM_MAX_CHANNELS = 4096
-ROUTE_MAX_EXPERTS = 2048
-_KINDS = {"rms": 0, "layer": 1}
-_GATE_ACTS = {"none": 0, "sigmoid": 1}
+# (checks, allocation and launch: csrc/native.cpp)
+_KINDS = {"rms": False, "layer": True}
+_GATE_ACTS = {"none": False, "sigmoid": True}
 
 
-def _launch(name, device, *args):
-    """One call of a C-ABI entry point on the current stream of the tensors' device."""
-    fn, i = getattr(_l.lib(), name), device.index
-    if i == torch._C._cuda_getDevice():
-        status = fn(*args, torch._C._cuda_getCurrentRawStream(i))
-    else:
-        with torch.cuda.device(i):
-            status = fn(*args, torch._C._cuda_getCurrentRawStream(i))
-    if status:
-        _l.check(status, name)
+def _native_call(name, *args):
+    try:
+        return getattr(_l.native(), name)(*args)
+    except TypeError as e:                           # (something that is no tensor, list or number)
+        raise RuntimeError("%s: %s" % (name, str(e).split("Invoked with")[0].strip())) from None
 
 
-def _chk_rows(t, name, like=None):
-    """rows [P, C] of fp32 / bf16 / fp16 (like: of the same type, on the same device)."""
-    if not isinstance(t, torch.Tensor):
-        raise RuntimeError("%s must be a tensor" % name)
-    if not t.is_cuda:
-        raise RuntimeError("%s must be a CUDA(HIP) tensor: CPU not supported" % name)
-    if t.dim() != 2 or not t.is_contiguous():
-        raise RuntimeError("%s must be contiguous rows [P, C]" % name)
-    if t.dtype not in ROW_DTYPES:
-        raise RuntimeError("%s must be a float32, bfloat16 or float16 tensor" % name)
-    if like is not None and (t.dtype != like.dtype or t.device != like.device):
-        raise RuntimeError("%s must have the type and the device of the rows it goes with (%s on %s)" % (name, like.dtype, like.device))
-    return t
-
-
-def _chk_vector(t, name, x):
-    if t is None:
-        return None
-    _chk(t, name, torch.float32)
-    if t.dim() != 1 or t.shape[0] != x.shape[1] or t.device != x.device:
-        raise RuntimeError("%s must hold one value for each of the %d channels, on the rows' device" % (name, x.shape[1]))
-    return t
-
-
-def _chk_norm(x, y, weight, bias, gate, scale, next_weight, next_bias, kind, gate_act, eps):
-    _chk_rows(x, "x")
-    P, C = x.shape
-    if not 1 <= C <= NORM_MAX_CHANNELS:
-        raise RuntimeError("norms take 1 to %d channels (got %d)" % (NORM_MAX_CHANNELS, C))
+def _norm_how(kind, gate_act):
     if kind not in _KINDS:
         raise RuntimeError("kind must be 'rms' or 'layer' (got %r)" % (kind,))
     if gate_act not in _GATE_ACTS:
         raise RuntimeError("gate_act must be 'none' or 'sigmoid' (got %r)" % (gate_act,))
-    if not (0.0 <= eps < float("inf")):
-        raise RuntimeError("eps must be finite and not negative")
-    if y is not None and _chk_rows(y, "y", x).shape != x.shape:
-        raise RuntimeError("y must have the shape of x")
-    if gate is not None:
-        G = _chk_rows(gate, "gate", x).shape[0]
-        if gate.shape[1] != C or (P > 0 and (G < 1 or P % G != 0)) or (P == 0 and G != 0):
-            raise RuntimeError("gate must be [P, C], or [G, C] for G groups of P / G consecutive rows (got %s for %s)"
-                               % (tuple(gate.shape), tuple(x.shape)))
-    for t, n in ((weight, "weight"), (bias, "bias"), (scale, "scale"), (next_weight, "next_weight"), (next_bias, "next_bias")):
-        _chk_vector(t, n, x)
-    if bias is not None and weight is None:
-        raise RuntimeError("a bias needs its weight (no weight: no norm)")
-    if next_bias is not None and next_weight is None:
-        raise RuntimeError("next_bias needs next_weight (no next_weight: no norm)")
+    return _KINDS[kind], _GATE_ACTS[gate_act]
 
 
 def norm_residual_fwd(x, y, weight=None, bias=None, gate=None, gate_act="none", scale=None, next_weight=None, next_bias=None,
@@ -474,62 +425,20 @@ def norm_residual_fwd(x, y, weight=None, bias=None, gate=None, gate_act="none", 
     """x, y [P, C] rows -> (out, normed): out = x + scale * gate * norm(y; weight, bias) and normed = norm(out; next_weight, next_bias)
     in one launch (cpfn_norm_residual_fwd; autograd_ops.norm_residual has the whole description).  y None: out is None and normed the
     norm of x."""
-    _chk_norm(x, y, weight, bias, gate, scale, next_weight, next_bias, kind, gate_act, eps)
-    if y is None and (weight is not None or gate is not None or scale is not None or next_weight is None):
-        raise RuntimeError("without y there is only the norm of x: next_weight, next_bias")
-    P, C = x.shape
-    out = torch.empty_like(x) if y is not None else None
-    normed = torch.empty_like(x) if next_weight is not None else None
-    if P == 0:
-        return out, normed
-    _launch("cpfn_norm_residual_fwd", x.device, _ptr(x), _ptr(y), _ptr(gate), _ptr(weight), _ptr(bias), _ptr(scale), _ptr(next_weight),
-            _ptr(next_bias), P, C, 0 if gate is None else gate.shape[0], ROW_DTYPES[x.dtype], _KINDS[kind], _GATE_ACTS[gate_act], eps,
-            _ptr(out), _ptr(normed))
-    if _l.counting():
-        _l.add_bytes("cpfn_norm_residual_fwd", x.element_size() * (P * C * (1 + 2 * (y is not None) + (normed is not None))
-                                                                   + (0 if gate is None else gate.numel())))
-    return out, normed
+    layer, sigmoid = _norm_how(kind, gate_act)
+    return _native_call("norm_residual_fwd", x, y, weight, bias, gate, sigmoid, scale, next_weight, next_bias, layer, eps)
 
 
-def norm_residual_bwd(x, y, weight, bias, gate, gate_act, scale, next_weight, d_out, d_normed, kind="rms", eps=1e-5,
-                      needs=("x", "y", "gate", "weight", "bias", "scale", "next_weight", "next_bias")):
+_NORM_INPUTS = ("x", "y", "weight", "bias", "gate", "scale", "next_weight", "next_bias")
+
+
+def norm_residual_bwd(x, y, weight, bias, gate, gate_act, scale, next_weight, d_out, d_normed, kind="rms", eps=1e-5, needs=_NORM_INPUTS):
     """Gradients of norm_residual_fwd's results -> {name: gradient} for the names in `needs` (of arguments that were given; the
-    parameters' in fp32).  d_out / d_normed None: no gradient arrived there."""
-    _chk_norm(x, y, weight, bias, gate, scale, next_weight, None, kind, gate_act, eps)
-    for t, n in ((d_out, "d_out"), (d_normed, "d_normed")):
-        if t is not None and _chk_rows(t, n, x).shape != x.shape:
-            raise RuntimeError("%s must have the shape of x" % n)
-    if d_out is None and d_normed is None:
-        raise RuntimeError("no gradient: d_out and d_normed are both None")
-    if d_normed is not None and next_weight is None:
-        raise RuntimeError("d_normed needs next_weight")
-    P, C = x.shape
-    dev = x.device
-    got = {}
-    if "x" in needs:
-        got["x"] = torch.empty_like(x)
-    if y is not None:
-        if "y" in needs:
-            got["y"] = torch.empty_like(x)
-        if gate is not None and "gate" in needs:
-            got["gate"] = torch.empty_like(gate)
-    vectors = [n for n, on in (("weight", weight is not None), ("bias", bias is not None), ("scale", scale is not None),
-                               ("next_weight", d_normed is not None), ("next_bias", d_normed is not None)) if on and n in needs]
-    if vectors:
-        got.update(zip(vectors, (torch.zeros if P == 0 else torch.empty)(len(vectors), C, dtype=torch.float32, device=dev).unbind(0)))
-    if P == 0 or not got:
-        return got
-    G = 0 if gate is None else gate.shape[0]
-    ws = torch.empty(_l.lib().cpfn_norm_residual_workspace(P, C, G) // 4, dtype=torch.float32, device=dev)
-    p = {n: t.data_ptr() for n, t in got.items()}.get
-    _launch("cpfn_norm_residual_bwd", dev, _ptr(x), _ptr(y), _ptr(gate), _ptr(weight), _ptr(bias), _ptr(scale), _ptr(next_weight),
-            _ptr(d_out), _ptr(d_normed), P, C, G, ROW_DTYPES[x.dtype], _KINDS[kind], _GATE_ACTS[gate_act], eps, p("x"), p("y"), p("gate"),
-            p("weight"), p("bias"), p("scale"), p("next_weight"), p("next_bias"), ws.data_ptr())
-    if _l.counting():
-        full = sum(t is not None for t in (y, d_out)) + 2 * (d_normed is not None) + ("x" in got) + ("y" in got)
-        _l.add_bytes("cpfn_norm_residual_bwd", x.element_size() * (P * C * full + (0 if gate is None else gate.numel())
-                                                                   + (got["gate"].numel() if "gate" in got else 0)))
-    return got
+    parameters' in fp32; next_bias needs d_normed only).  d_out / d_normed None: no gradient arrived there."""
+    layer, sigmoid = _norm_how(kind, gate_act)
+    got = _native_call("norm_residual_bwd", x, y, weight, bias, gate, sigmoid, scale, next_weight, d_out, d_normed, layer, eps,
+                       [n in needs for n in _NORM_INPUTS])
+    return {n: g for n, g in zip(_NORM_INPUTS, got) if g is not None}
 
 
 class RoutePlan:
@@ -544,98 +453,30 @@ class RoutePlan:
 def route_plan(choice, n_experts):
     """choice [R, k] i32 or i64: the experts of each row -> RoutePlan: all R k choices in the order of their experts, equal ones in the
     order of the rows (stable).  An index outside [0, n_experts) is a choice that is not routed (an expert that is full, a padded row):
-    it gets no place and moves nothing.  The same expert twice in a row is two choices.  Nothing is read back by the host."""
-    if not isinstance(choice, torch.Tensor):
-        raise RuntimeError("choice must be a tensor")
-    if not choice.is_cuda:
-        raise RuntimeError("choice must be a CUDA(HIP) tensor: CPU not supported")
-    if choice.dim() != 2 or not choice.is_contiguous():
-        raise RuntimeError("choice must be contiguous [R, k]")
-    if choice.dtype not in (torch.int32, torch.int64):
-        raise RuntimeError("choice must be an int32 or int64 tensor")
-    E, n = int(n_experts), choice.numel()
-    if not 1 <= E <= ROUTE_MAX_EXPERTS:
-        raise RuntimeError("routing takes 1 to %d experts (got %d)" % (ROUTE_MAX_EXPERTS, E))
-    if choice.shape[1] < 1 or n >= 2 ** 31:
-        raise RuntimeError("choice must hold at least one choice for each row and fewer than 2^31 in all (got %s)" % (tuple(choice.shape),))
-    dev = choice.device
-    offsets = torch.empty(E + 1, dtype=torch.int32, device=dev)
-    place = torch.empty(choice.shape, dtype=torch.int32, device=dev)
-    nws = _l.lib().cpfn_route_workspace(n, E)
-    ws = torch.empty(nws // 4, dtype=torch.int32, device=dev) if nws else None
-    _launch("cpfn_route_plan", dev, _ptr(choice), 1 if choice.dtype == torch.int64 else 0, n, E, _ptr(offsets), _ptr(place), _ptr(ws))
-    _l.add_bytes("cpfn_route_plan", (choice.element_size() + 4) * n + 4 * (E + 1))
-    return RoutePlan(offsets, place, E)
+    it gets no place and moves nothing.  The same expert twice in a row is two choices.  Up to 2048 experts; nothing is read back by
+    the host."""
+    offsets, place = _native_call("route_plan", choice, n_experts)
+    return RoutePlan(offsets, place, n_experts)
 
 
-def _chk_plan(plan, x, name, sorted_rows):
+def _plan(plan):
     if not isinstance(plan, RoutePlan):
         raise RuntimeError("plan must be a RoutePlan (ops.route_plan)")
-    R, k = plan.place.shape
-    if x.shape[0] != (R * k if sorted_rows else R) or plan.place.device != x.device:
-        raise RuntimeError("%s must have %d rows, on the plan's device (got %s)" % (name, R * k if sorted_rows else R, tuple(x.shape)))
-    if x.shape[1] < 1:
-        raise RuntimeError("%s must have at least one channel" % name)
-    return R, k
-
-
-def _chk_route_weights(weights, plan):
-    if weights is not None:
-        _chk(weights, "weights", torch.float32)
-        if weights.shape != plan.place.shape or weights.device != plan.place.device:
-            raise RuntimeError("weights must be [R, k] = %s, on the plan's device" % (tuple(plan.place.shape),))
-    return weights
+    return plan.offsets, plan.place, plan.n_experts
 
 
 def route_gather_fwd(rows, plan):
     """rows [R, C] -> [R k, C]: row r at each of its places; the rows behind plan.offsets[-1] (choices not routed) are zero."""
-    _chk_rows(rows, "rows")
-    R, k = _chk_plan(plan, rows, "rows", False)
-    C = rows.shape[1]
-    out = torch.empty(R * k, C, dtype=rows.dtype, device=rows.device)
-    if R == 0:
-        return out
-    _launch("cpfn_route_gather", rows.device, _ptr(rows), _ptr(plan.place), _ptr(plan.offsets), R, k, plan.n_experts, C,
-            ROW_DTYPES[rows.dtype], _ptr(out))
-    _l.add_bytes("cpfn_route_gather", rows.element_size() * (R + R * k) * C + 4 * R * k)
-    return out
+    return _native_call("route_gather_fwd", rows, *_plan(plan))
 
 
 def route_combine_fwd(sorted_rows, weights, plan):
     """sorted_rows [R k, C], weights [R, k] f32 or None (all 1) -> [R, C]: the weighted sum of the rows at each row's places, in fp32
     and the order of the choices (weights None: the adjoint of route_gather_fwd)."""
-    _chk_rows(sorted_rows, "sorted_rows")
-    R, k = _chk_plan(plan, sorted_rows, "sorted_rows", True)
-    _chk_route_weights(weights, plan)
-    C = sorted_rows.shape[1]
-    out = torch.empty(R, C, dtype=sorted_rows.dtype, device=sorted_rows.device)
-    if R == 0:
-        return out
-    _launch("cpfn_route_combine", sorted_rows.device, _ptr(sorted_rows), _ptr(weights), _ptr(plan.place), R, k, C,
-            ROW_DTYPES[sorted_rows.dtype], _ptr(out))
-    _l.add_bytes("cpfn_route_combine", sorted_rows.element_size() * (R + R * k) * C + (4 if weights is None else 8) * R * k)
-    return out
+    return _native_call("route_combine_fwd", sorted_rows, weights, *_plan(plan))
 
 
 def route_combine_bwd(grad_out, sorted_rows, weights, plan, need_rows=True, need_weights=True):
     """The adjoint of route_combine_fwd -> (d_sorted [R k, C] or None, d_weights [R, k] f32 or None); sorted_rows may be None where
     d_weights is not wanted."""
-    _chk_rows(grad_out, "grad_out")
-    R, k = _chk_plan(plan, grad_out, "grad_out", False)
-    _chk_route_weights(weights, plan)
-    if not (need_rows or need_weights):
-        return None, None
-    C, dev = grad_out.shape[1], grad_out.device
-    if need_weights:
-        _chk_rows(sorted_rows, "sorted_rows", grad_out)
-        _chk_plan(plan, sorted_rows, "sorted_rows", True)
-        if sorted_rows.shape[1] != C:
-            raise RuntimeError("sorted_rows and grad_out must have the same channels")
-    d_sorted = torch.empty(R * k, C, dtype=grad_out.dtype, device=dev) if need_rows else None
-    d_weights = torch.empty(R, k, dtype=torch.float32, device=dev) if need_weights else None
-    if R == 0:
-        return d_sorted, d_weights
-    _launch("cpfn_route_combine_bwd", dev, _ptr(grad_out), _ptr(sorted_rows) if need_weights else None, _ptr(weights), _ptr(plan.place),
-            _ptr(plan.offsets), R, k, plan.n_experts, C, ROW_DTYPES[grad_out.dtype], _ptr(d_sorted), _ptr(d_weights))
-    _l.add_bytes("cpfn_route_combine_bwd", grad_out.element_size() * (R + R * k * (need_rows + need_weights)) * C + 12 * R * k)
-    return d_sorted, d_weights
+    return _native_call("route_combine_bwd", grad_out, sorted_rows, weights, *_plan(plan), need_rows, need_weights)

@@ -12,12 +12,7 @@ clipping, in two launches for up to 128 tensors; `FlatAdam.step(max_grad_norm=..
 import torch
 
 from . import lib as _l
-from .ops import _launch, _ptr, _stream
-
-try:
-    from . import _tables               # (csrc/tables.cpp)
-except ImportError as e:
-    raise ImportError("cpfn_amd/_tables.so is not built: run `python -m cpfn_amd.build` (%s)" % e) from e
+from .ops import _native_call, _ptr, _stream
 
 _NORMS = {1.0: 1, 2.0: 2, float("inf"): 0}
 
@@ -27,47 +22,25 @@ def _list_of(grads):
 
 
 def _norm_code(norm_type):
-    p = _NORMS.get(float(norm_type))
+    p = _NORMS.get(norm_type)
     if p is None:
         raise RuntimeError("norm_type must be 1, 2 or inf (got %r)" % (norm_type,))
     return p
 
 
-@torch.no_grad()
 def grad_norm(grads, norm_type=2.0):
     """The norm over all values of a list of tensors (fp32, bf16 and fp16 together; any lengths) -> 0-dim fp32 tensor on their device,
-    without a host synchronisation.  norm_type 1, 2 or inf; fp64 sums in a fixed order (bit-reproducible); NaN if any value is NaN."""
-    grads, p = _list_of(grads), _norm_code(norm_type)
-    if not grads:
-        return torch.zeros(())
-    dev, nbytes, ptr, n, types, _, _ = _tables.gradients(grads, None)
-    dev = torch.device("cuda", dev)
-    norm = torch.empty((), dtype=torch.float32, device=dev)
-    ws = torch.empty(_l.lib().cpfn_grad_norm_workspace(n, len(grads)) // 8, dtype=torch.float64, device=dev)
-    _launch("cpfn_grad_norm", dev, ptr, n, types, len(grads), p, norm.data_ptr(), ws.data_ptr())
-    _l.add_bytes("cpfn_grad_norm", nbytes)
-    return norm
+    without a host synchronisation.  norm_type 1, 2 or inf; fp64 sums in a fixed order (bit-reproducible); NaN if any value is NaN.
+    An empty list: a zero on the CPU."""
+    return _native_call("grad_norm", _list_of(grads), _norm_code(norm_type), None, None)
 
 
-@torch.no_grad()
 def clip_grads_(grads, max_norm, norm_type=2.0, out=None):
     """grads *= min(1, max_norm / (norm + 1e-6)) with the norm of grad_norm -> that norm (before clipping, on the device).  Nothing is
     synchronised, and in place nothing is written where the factor is 1.  out: tensors of the same shapes, of the gradients' types or
     fp32 (master gradients), that take the result instead; a gradient listed twice, or memory shared with a tensor that is written, is
     refused.  An infinite norm gives the factor 0 and a NaN one NaN, as the formula has it."""
-    grads, p, max_norm = _list_of(grads), _norm_code(norm_type), float(max_norm)
-    if not max_norm >= 0.0:
-        raise RuntimeError("max_norm must not be negative (got %r)" % max_norm)
-    outs = None if out is None else _list_of(out)
-    if not grads and not outs:
-        return torch.zeros(())
-    dev, nbytes, ptr, n, types, optr, otypes = _tables.gradients(grads, outs)
-    dev = torch.device("cuda", dev)
-    norm = torch.empty((), dtype=torch.float32, device=dev)
-    ws = torch.empty(_l.lib().cpfn_grad_norm_workspace(n, len(grads)) // 8, dtype=torch.float64, device=dev)
-    _launch("cpfn_grad_clip", dev, ptr, optr, n, types, otypes, len(grads), p, max_norm, norm.data_ptr(), ws.data_ptr())
-    _l.add_bytes("cpfn_grad_clip", nbytes if outs else 2 * nbytes)
-    return norm
+    return _native_call("grad_norm", _list_of(grads), _norm_code(norm_type), float(max_norm), None if out is None else _list_of(out))
 
 
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
