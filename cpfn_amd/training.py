@@ -277,7 +277,14 @@ class SPFNTrainer:
 
     def __init__(self, module, batch_size=16, init_learning_rate=1e-3, decay_step=200000, decay_rate=0.7,
                  bn_decay_step=200000, multipliers=None, classes=None, fused_adam=None, use_graphs=False,
-                 require_graphs=False):
+                 require_graphs=False, max_grad_norm=None):
+        """max_grad_norm: every step is taken on the gradients times min(1, max_grad_norm / (their 2-norm + 1e-6)) (the mean over the
+        ranks under data parallelism: the same factor on every rank); None (the reference's loop): as they are.  `grad_norm` has the last step's
+        norm."""
+        if max_grad_norm is not None and not float(max_grad_norm) >= 0.0:
+            raise RuntimeError("max_grad_norm must not be negative (got %r)" % (max_grad_norm,))
+        self.max_grad_norm = None if max_grad_norm is None else float(max_grad_norm)
+        self._grad_norm = None
         self.module = module
         self.batch_size = batch_size
         self.init_learning_rate, self.decay_step, self.decay_rate = init_learning_rate, decay_step, decay_rate
@@ -322,6 +329,25 @@ class SPFNTrainer:
         Reading it synchronises with the device when the capturable / graph path keeps the count there."""
         dev = 0 if self._skipped_dev is None else int(round(float(self._skipped_dev)))
         return self._host_skipped + dev
+
+    @property
+    def grad_norm(self):
+        """The 2-norm of the last step's gradients before clipping, a 0-dim tensor (on the device, without a synchronisation); None
+        without max_grad_norm or before the first step."""
+        if self.max_grad_norm is None:
+            return None
+        from .optim import FlatAdam
+        return self.optimizer.grad_norm if isinstance(self.optimizer, FlatAdam) else self._grad_norm
+
+    def _clip_bucket(self):
+        """Clip the flat bucket in place for an optimizer that is not FlatAdam (which clips what it reads)."""
+        if self.max_grad_norm is None:
+            return
+        if self.bucket.flat.is_cuda:
+            from .optim import clip_grads_
+            self._grad_norm = clip_grads_(self.bucket.flat, self.max_grad_norm)
+        else:
+            self._grad_norm = torch.nn.utils.clip_grad_norm_(self.bucket.params, self.max_grad_norm)
 
     def _skip_counter(self, device):
         if self._skipped_dev is None:
@@ -446,13 +472,23 @@ class SPFNTrainer:
         from .optim import FlatAdam
         if isinstance(self.optimizer, FlatAdam):
             self.optimizer.found_inf = fault
-            self.optimizer.step(check_gradients=nf_flags is None, skipped=skipped, nf_flags=nf_flags, combine=combine)
+            self.optimizer.step(check_gradients=nf_flags is None, skipped=skipped, nf_flags=nf_flags, combine=combine,
+                                max_grad_norm=self.max_grad_norm)
         else:
             assert combine is None
             found = self.bucket.nonfinite_flag()
             self.optimizer.found_inf = found if fault is None else torch.maximum(found, fault)
+            self._clip_bucket()
             self.optimizer.step()
             skipped += self.optimizer.found_inf
+
+    def _clipped_optimizer_step(self):
+        from .optim import FlatAdam
+        if isinstance(self.optimizer, FlatAdam):
+            self.optimizer.step(max_grad_norm=self.max_grad_norm)
+        else:
+            self._clip_bucket()
+            self.optimizer.step()
 
     @staticmethod
     def _feature_kwargs(batch):
@@ -775,7 +811,9 @@ class SPFNTrainer:
                 # (the launches that produce parameter gradients write them into the flat bucket, finite check included:
                 #  FlatGradBucket.sink — no packing copy on one GPU, a one-word copy of the fault slot under data parallelism)
                 from .optim import FlatAdam as _FA
-                with self.bucket.sink(check=world == 1, combine_ok=world == 1 and isinstance(self.optimizer, _FA)) as gsink:
+                # (clipping needs every gradient finished before the norm is taken: the pass's last reduction stays a launch then)
+                with self.bucket.sink(check=world == 1, combine_ok=world == 1 and isinstance(self.optimizer, _FA)
+                                      and self.max_grad_norm is None) as gsink:
                     out[0].backward(st["unit"])          # (no ones_like fill inside the graph)
                 nf = self.bucket.collect(check=world == 1, fault=st["flag_fault"] if world > 1 else None, sink=gsink)
                 if world == 1:
@@ -1144,7 +1182,7 @@ class SPFNTrainer:
         if self.use_graphs:                            # capturable optimizer: skip decided (and counted) on the device
             self._checked_optimizer_step(self._skip_counter(self.bucket.flat.device), fault=reduced_fault)
         elif bool(self.bucket.finite()) and (reduced_fault is None or float(reduced_fault) == 0.0):   # host sync (reference: 148)
-            self.optimizer.step()
+            self._clipped_optimizer_step()
         else:
             self._host_skipped += 1
         self.global_step += 1

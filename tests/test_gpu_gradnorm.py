@@ -198,6 +198,29 @@ def test_streams_repeats_and_captured_graphs():
             assert all(torch.equal(a, b) for a, b in zip(held + out, want))
 
 
+def check_adam_step(opt, before, grad, t, max_norm, lr):
+    """`opt` after step t (1, 2, ..) against Adam's formulas in 64 bits on its state `before` (parameters, moments) and the clipped
+    gradient, the hyper-parameters being the fp32 numbers that they are.  Returns the clipping factor."""
+    one = torch.ones(1, dtype=torch.float64, device=grad.device)
+    b1, b2 = (float(torch.tensor(b, dtype=torch.float32)) for b in (0.9, 0.999))
+    o1, o2 = (float(torch.tensor(1.0, dtype=torch.float32) - torch.tensor(b, dtype=torch.float32)) for b in (0.9, 0.999))
+    lr, eps = (float(torch.tensor(v, dtype=torch.float32)) for v in (lr, 1e-8))
+    p, m, v = (Approx(x.double()) for x in before)
+    norm = exact_norm([grad], 2.0)
+    assert abs(float(opt.grad_norm) - norm) <= (1 + 1e-6) * U * norm
+    coef = min(1.0, max_norm / (norm + 1e-6))
+    g = Approx(grad.double()) * Approx(coef * one, U * coef * one)
+    m = m + (g - m) * o1
+    v = v * b2 + g * g * o2
+    step_size = Approx(one * lr) / Approx(one * (1 - b1 ** t), U * one)
+    denom = v.sqrt() / Approx(one * (1 - b2 ** t), U * one * (1 - b2 ** t)).sqrt() + eps
+    p = p - step_size * (m / denom)
+    assert_within(opt.exp_avg, m, "exp_avg")
+    assert_within(opt.exp_avg_sq, v, "exp_avg_sq")
+    assert_within(opt.flat_p, p, "parameters")
+    return coef
+
+
 def _adam_pair(seed=3):
     from cpfn_amd import training
     from cpfn_amd.optim import FlatAdam
@@ -213,12 +236,6 @@ def test_adam_on_clipped_gradients():
     (with the hyper-parameters as the fp32 numbers they are), errors followed step by step (tests/approx.py).  The bucket keeps the
     gradients, the norm is left on the device."""
     ma, mb, bucket, oa, _ = _adam_pair()
-    b1, b2 = (float(torch.tensor(b, dtype=torch.float32)) for b in (0.9, 0.999))
-    o1, o2 = (float(torch.tensor(1.0, dtype=torch.float32) - torch.tensor(b, dtype=torch.float32)) for b in (0.9, 0.999))
-    lr, eps = (float(torch.tensor(v, dtype=torch.float32)) for v in (1e-2, 1e-8))
-    p = Approx(oa.flat_p.double())
-    m, v = Approx(torch.zeros_like(p.v)), Approx(torch.zeros_like(p.v))
-    one = torch.ones(1, dtype=torch.float64, device=DEV)
     g = torch.Generator().manual_seed(0)
     for step in range(8):
         x = torch.randn(32, 70, generator=g).to(DEV)
@@ -227,22 +244,11 @@ def test_adam_on_clipped_gradients():
         ((ma(x) * (10.0 if step % 2 else 0.01)) ** 2).mean().backward()
         bucket.collect()
         flat = bucket.flat.clone()
+        state = [t.clone() for t in (oa.flat_p, oa.exp_avg, oa.exp_avg_sq)]
         oa.step(max_grad_norm=0.2)
         assert torch.equal(bucket.flat, flat)
-        norm = exact_norm([flat], 2.0)
-        assert abs(float(oa.grad_norm) - norm) <= (1 + 1e-6) * U * norm
-        coef = min(1.0, 0.2 / (norm + 1e-6))
+        coef = check_adam_step(oa, state, flat, step + 1, 0.2, 1e-2)
         assert (coef < 1.0) == bool(step % 2)
-        gr = Approx(flat.double()) * Approx(coef * one, U * coef * one)
-        m = m + (gr - m) * o1
-        v = v * b2 + gr * gr * o2
-        step_size = Approx(one * lr) / Approx(one * (1 - b1 ** (step + 1)), U * one)
-        denom = v.sqrt() / Approx(one * (1 - b2 ** (step + 1)), U * one * (1 - b2 ** (step + 1))).sqrt() + eps
-        p = p - step_size * (m / denom)
-        assert_within(oa.exp_avg, m, "exp_avg")
-        assert_within(oa.exp_avg_sq, v, "exp_avg_sq")
-        assert_within(oa.flat_p, p, "parameters")
-        p, m, v = Approx(oa.flat_p.double()), Approx(oa.exp_avg.double()), Approx(oa.exp_avg_sq.double())      # (step by step)
 
 
 def test_adam_within_the_bound_is_the_plain_step_bit_for_bit():
@@ -275,3 +281,54 @@ def test_adam_skips_gradients_that_are_not_finite():
         opt.step(max_grad_norm=-1.0)
     with pytest.raises(RuntimeError):
         opt.step(max_grad_norm=1.0, combine=(bucket.flat, bucket.flat, 1, bucket.flat))
+
+
+@pytest.mark.parametrize("graphs", [False, True])
+def test_trainer_clips_its_steps(graphs):
+    """SPFNTrainer(max_grad_norm): every step of the network's training, eager and replayed, is Adam on the clipped bucket; a batch whose
+    gradients are not finite is skipped."""
+    import contextlib
+    import io
+    from cpfn_amd import synthetic, training
+    from cpfn_amd.PointNet2 import pn2_network
+    from cpfn_amd.SPFN import fitter_factory
+    with contextlib.redirect_stdout(io.StringIO()):
+        fitter_factory.register_primitives(training.GLOBAL_SPFN_CLASSES)
+    torch.manual_seed(0)
+    model = pn2_network.PointNet2(dim_input=3, dim_pos=3, output_sizes=[3, 4, 28]).to(DEV)
+    model.set_compute_dtype(torch.bfloat16)
+    tr = training.SPFNTrainer(model, batch_size=4, init_learning_rate=1e-3, use_graphs=graphs, require_graphs=graphs, max_grad_norm=0.05)
+    batch = {k: v.to(DEV) for k, v in synthetic.training_batch(4, N=2048, n_prims=6, n_inst_points=128, seed=5).items()}
+    opt = tr.optimizer
+    for step in range(6):
+        state = [t.clone() for t in (opt.flat_p, opt.exp_avg, opt.exp_avg_sq)]
+        tr.step(batch, next_batch=batch)
+        torch.cuda.synchronize()
+        assert check_adam_step(opt, state, tr.bucket.flat.clone(), step + 1, 0.05, 1e-3) < 1.0
+        assert tr.grad_norm is opt.grad_norm
+    assert (tr._graph is not None) == graphs and tr.skipped_steps == 0
+    bad = {k: v.clone() for k, v in batch.items()}
+    bad["P"][1, 100, 2] = float("nan")
+    state = [t.clone() for t in (opt.flat_p, opt.exp_avg, opt.exp_avg_sq)]
+    tr.step(bad)
+    torch.cuda.synchronize()
+    assert tr.skipped_steps == 1
+    assert all(torch.equal(a, b) for a, b in zip(state, (opt.flat_p, opt.exp_avg, opt.exp_avg_sq)))
+    tr.step(batch)
+    torch.cuda.synchronize()
+    assert tr.skipped_steps == 1 and bool(torch.isfinite(opt.flat_p).all()) and not torch.equal(opt.flat_p, state[0])
+
+
+def test_trainer_with_another_optimizer_clips_the_bucket():
+    from cpfn_amd import training
+    torch.manual_seed(1)
+    m = torch.nn.Linear(40, 9).to(DEV)
+    tr = training.SPFNTrainer(m, fused_adam=False, max_grad_norm=0.1)
+    (m(torch.randn(8, 40, device=DEV)) ** 2).sum().backward()
+    tr.bucket.collect()
+    before = tr.bucket.flat.clone()
+    tr._clipped_optimizer_step()
+    norm = exact_norm([before], 2.0)
+    assert norm > 0.1 and abs(float(tr.grad_norm) - norm) <= (1 + 1e-6) * U * norm
+    assert within(tr.bucket.flat, before.double() * (0.1 / (norm + 1e-6)), 0.1)
+    assert training.SPFNTrainer(m, fused_adam=False).grad_norm is None
