@@ -7,6 +7,7 @@
 // without the interpreter.
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
@@ -86,7 +87,7 @@ struct Norm {
     check_rows(x, "x");
     const int64_t P = x.size(0), C = x.size(1);
     REQUIRE(C >= 1 && C <= NORM_MAX_CHANNELS, "norms take 1 to ", NORM_MAX_CHANNELS, " channels (got ", C, ")");
-    REQUIRE(eps >= 0.0 && std::isfinite(eps), "eps must be finite and not negative");
+    REQUIRE(eps >= 0.0 && std::isfinite((float)eps), "eps must be finite and not negative");
     if (y.defined()) {
       check_rows(y, "y", &x);
       REQUIRE(y.sizes() == x.sizes(), "y must have the shape of x (got ", y.sizes(), " for ", x.sizes(), ")");
@@ -198,6 +199,23 @@ void not_again(variable_list &grads, const char *what) {
     if (g.defined()) g = out[k++];
 }
 
+// A backward pass that is captured must not reach a leaf whose gradient is accumulated on the default stream, which cannot take part in a
+// capture.  It is where an eager graph of the same leaf, built on that stream, is still alive: the leaf has one accumulating node, which
+// keeps the stream that it was made on.
+void check_capture(const Tensor &on) {
+  const auto stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(on.get_device());
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (stream.stream() == nullptr || hipStreamIsCapturing(stream.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+  const auto node = torch::autograd::get_current_node();
+  if (!node) return;
+  for (const auto &edge : node->next_edges()) {
+    if (!dynamic_cast<torch::autograd::AccumulateGrad *>(edge.function.get())) continue;
+    const auto made_on = edge.function->stream();
+    REQUIRE(!made_on || c10::hip::HIPStreamMasqueradingAsCUDA(*made_on).stream() != nullptr,
+            "a backward pass is captured while an eager graph of the same leaf lives on the default stream: drop that graph's results first");
+  }
+}
+
 Tensor contiguous(const Tensor &t) { return t.defined() ? t.contiguous() : t; }
 
 // The end of a residual block and the norm of the next one as one node.  Only the inputs are kept: out, the normalised rows and both
@@ -219,6 +237,7 @@ struct NormResidual : public torch::autograd::Function<NormResidual> {
   }
   static variable_list backward(AutogradContext *ctx, const variable_list &d) {
     const auto saved = ctx->get_saved_variables();
+    check_capture(saved[0]);
     const int64_t how = ctx->saved_data["how"].toInt();
     const Norm n{saved[0], saved[1], saved[2], saved[3], saved[4], saved[5], saved[6], Tensor(), (how & 1) != 0, (how & 2) != 0, ctx->saved_data["eps"].toDouble()};
     const bool given[8] = {true, n.y.defined(), n.weight.defined(), n.bias.defined(), n.gate.defined(), n.scale.defined(), n.next_weight.defined(), (how & 4) != 0};
@@ -245,7 +264,7 @@ std::tuple<Maybe, Maybe> norm_residual(const Tensor &x, const Maybe &y, const Ma
 }
 
 // ---------------------------------------------------------------- rows sorted by expert and back
-constexpr int64_t ROUTE_MAX_EXPERTS = 2048;
+constexpr int64_t ROUTE_MAX_EXPERTS = 2048, ROUTE_MAX_CHANNELS = 1ll << 30;
 
 std::tuple<Tensor, Tensor> route_plan(const Tensor &choice, int64_t E) {
   REQUIRE(choice.is_cuda(), "choice must be a CUDA(HIP) tensor: CPU not supported");
@@ -276,7 +295,7 @@ struct Plan {
     check_rows(t, name);
     const int64_t rows = sorted ? R() * k() : R();
     REQUIRE(t.size(0) == rows && t.device() == place.device(), name, " must have ", rows, " rows, on the plan's device (got ", t.sizes(), ")");
-    REQUIRE(t.size(1) >= 1 && t.size(1) < (1ll << 31), name, " must have at least one channel");
+    REQUIRE(t.size(1) >= 1 && t.size(1) <= ROUTE_MAX_CHANNELS, name, " must have 1 to 2^30 channels (got ", t.size(1), ")");
   }
   void check_weights(const Tensor &w) const {
     if (!w.defined()) return;
@@ -341,6 +360,7 @@ struct RouteGather : public torch::autograd::Function<RouteGather> {
   }
   static variable_list backward(AutogradContext *ctx, const variable_list &d) {
     const auto saved = ctx->get_saved_variables();
+    check_capture(saved[1]);
     variable_list grads(4);
     grads[0] = combine_rows(d[0].contiguous(), Tensor(), Plan{saved[0], saved[1], ctx->saved_data["E"].toInt()});
     not_again(grads, "route_gather");
@@ -356,6 +376,7 @@ struct RouteCombine : public torch::autograd::Function<RouteCombine> {
   }
   static variable_list backward(AutogradContext *ctx, const variable_list &d) {
     const auto saved = ctx->get_saved_variables();
+    check_capture(saved[3]);
     const bool weighted = saved[1].defined();
     const auto g = combine_rows_bwd(d[0].contiguous(), saved[0], saved[1], Plan{saved[2], saved[3], ctx->saved_data["E"].toInt()}, ctx->needs_input_grad(0),
                                     weighted && ctx->needs_input_grad(1));
@@ -420,6 +441,10 @@ Tensor grad_norm(const py::list &grads, int p, std::optional<double> max_norm, c
     check_status(cpfn_grad_clip(src.at.data(), out ? dst.at.data() : nullptr, src.n.data(), src.type.data(), out ? dst.type.data() : nullptr, (int)count_, p,
                                 *max_norm, fptr(norm), ptr(ws), stream),
                  "cpfn_grad_clip");
+    for (size_t i = 0; i < count_; ++i) {                 // (written behind autograd's back)
+      const Tensor &t = THPVariable_Unpack(PyList_GET_ITEM(out ? out->ptr() : grads.ptr(), i));
+      if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    }
     count("cpfn_grad_clip", src.bytes + (out ? dst.bytes : src.bytes));
   } else {
     check_status(cpfn_grad_norm(src.at.data(), src.n.data(), src.type.data(), (int)count_, p, fptr(norm), ptr(ws), stream), "cpfn_grad_norm");

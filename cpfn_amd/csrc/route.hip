@@ -199,6 +199,7 @@ __global__ __launch_bounds__(RANK_WAVES * 64) void route_rank_kernel(const I *__
 // lane moves (or computes) a few elements that another lane moves too, to the same value.  Rows shorter than a piece go element by element.
 constexpr int MOVE_THREADS = 256;
 constexpr long long MOVE_BLOCKS = 1 << 20;
+constexpr int MOVE_MAX_C = 1 << 30;               // (a row is walked with 32-bit steps of up to 2048 elements)
 
 struct Walk {                     // 1 << lanes_log2 lanes for a row
   int lanes, lane;
@@ -218,12 +219,18 @@ __device__ __forceinline__ void zero_tail(T *__restrict__ out, const int *__rest
                                           long long slot, long long slots) {
   constexpr int N = cpfn_piece<T>::N;
   const typename cpfn_piece<T>::vec z = {};
-  for (long long p = *end + slot; p < n; p += slots)
+  for (long long p = (*end < 0 ? 0 : *end) + slot; p < n; p += slots)
     for (int c = lane * N; c < C; c += lanes * N) {
       if (C >= N) *(typename cpfn_piece<T>::vec *)(out + p * C + piece_at<T>(c, C)) = z;
       else
         for (int q = 0; q < C; ++q) out[p * C + q] = cpfn_from_f32<T>(0.f);
     }
+}
+
+// A place that is not one of the n sorted rows (-1; anything else only in tensors that no plan left) is a choice that is not there.
+__device__ __forceinline__ int place_of(const int *__restrict__ place, long long at, long long n) {
+  const int p = place[at];
+  return (unsigned)p < (unsigned)n ? p : -1;
 }
 
 // KT: choices of a row that are taken at once (their places in flight together)
@@ -238,7 +245,7 @@ __global__ __launch_bounds__(MOVE_THREADS) void route_gather_kernel(const T *__r
     for (int j0 = 0; j0 < k; j0 += KT) {
       int p[KT];
 #pragma unroll
-      for (int t = 0; t < KT; ++t) p[t] = j0 + t < k ? place[r * k + j0 + t] : -1;
+      for (int t = 0; t < KT; ++t) p[t] = j0 + t < k ? place_of(place, r * k + j0 + t, R * k) : -1;
       for (int c = w.lane * N; c < C; c += w.lanes * N) {
         if (C >= N) {
           const int at = piece_at<T>(c, C);
@@ -284,7 +291,7 @@ __global__ __launch_bounds__(MOVE_THREADS) void route_combine_kernel(const T *__
       for (int t = 0; t < KT; ++t) {
         const bool is = j0 + t < k;
         const long long at = r * k + (is ? j0 + t : 0);
-        p[t] = is ? place[at] : -1;
+        p[t] = is ? place_of(place, at, R * k) : -1;
         w[t] = weights ? weights[at] : 1.f;
       }
     };
@@ -334,7 +341,7 @@ __global__ __launch_bounds__(MOVE_THREADS) void route_combine_bwd_kernel(const T
       for (int t = 0; t < KT; ++t) {
         const bool is = row && j0 + t < k;
         const long long at = is ? r * k + j0 + t : 0;
-        p[t] = is ? place[at] : -1;
+        p[t] = is ? place_of(place, at, R * k) : -1;
         w[t] = weights ? weights[at] : 1.f;
         dot[t] = 0.f;
       }
@@ -454,7 +461,7 @@ int combine_bwd(const void *g, const void *sorted, const float *weights, const i
 }
 
 bool bad_sizes(long long R, int k, int E, int C) {
-  return R < 0 || k < 1 || E < 1 || E > ROUTE_MAX_E || C < 1 || R > 0x7fffffffll / k;
+  return R < 0 || k < 1 || E < 1 || E > ROUTE_MAX_E || C < 1 || C > MOVE_MAX_C || R > 0x7fffffffll / k;
 }
 
 }  // namespace

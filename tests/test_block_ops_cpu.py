@@ -88,6 +88,14 @@ def test_c_abi_refuses_bad_routes():
     assert h.cpfn_route_combine_bwd(A, None, A, A, A, 8, 2, 4, 16, 1, A, A, None) == EINVAL
 
 
+def test_c_abi_refuses_rows_that_are_walked_out_of_32_bits():
+    h = lib.lib()
+    for R in (0, 1):
+        assert h.cpfn_route_gather(A, A, A, R, 1, 4, (1 << 30) + 1, 1, A, None) == EINVAL
+        assert h.cpfn_route_combine(A, A, A, R, 1, (1 << 30) + 1, 1, A, None) == EINVAL
+        assert h.cpfn_route_combine_bwd(A, A, A, A, A, R, 1, 4, (1 << 30) + 1, 1, A, A, None) == EINVAL
+
+
 def test_c_abi_refuses_bad_gradient_lists():
     h = lib.lib()
 

@@ -332,3 +332,23 @@ def test_trainer_with_another_optimizer_clips_the_bucket():
     assert norm > 0.1 and abs(float(tr.grad_norm) - norm) <= (1 + 1e-6) * U * norm
     assert within(tr.bucket.flat, before.double() * (0.1 / (norm + 1e-6)), 0.1)
     assert training.SPFNTrainer(m, fused_adam=False).grad_norm is None
+
+
+def test_what_is_clipped_counts_as_changed():
+    """Autograd notices that a tensor which it kept was scaled, in place and through `out`."""
+    from cpfn_amd import optim
+    for elsewhere in (False, True):
+        leaf = torch.randn(100, device=DEV, requires_grad=True)
+        a = leaf * 2.0
+        b = (a * a).sum()                                           # (keeps a)
+        d = a.detach()
+        if elsewhere:
+            optim.clip_grads_([torch.ones(100, device=DEV)], 0.5, out=[d])
+        else:
+            optim.clip_grads_([d], 0.5)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            b.backward()
+    with torch.inference_mode():
+        x = torch.randn(100, device=DEV)
+        norm = optim.clip_grads_([x], 0.5)
+    assert abs(float(x.double().norm()) - 0.5) < 1e-5 and abs(float(norm)) > 0.5

@@ -233,3 +233,48 @@ def test_offsets_that_pass_32_bits():
     assert torch.equal(out[-1].float(), (2 * rows[-1].float()).to(torch.bfloat16).float()) and not bool(out[:-1].any())
     d_sorted, d_w = ops.route_combine_bwd(rows, srt, None, plan)
     assert torch.equal(d_sorted, srt) and not bool(d_w[:-1].any()) and bool((d_w[-1] > 0).all())
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("C", [3, 40, 131])
+def test_places_that_no_plan_left_are_choices_that_are_not_there(C, dtype):
+    """A RoutePlan is two tensors that a caller can write to: places outside the sorted rows, and an end in front of them, are neither
+    read from nor written to (results between guard rows, at the C ABI)."""
+    from cpfn_amd import lib
+    h, st = lib.lib(), torch.cuda.current_stream().cuda_stream
+    R, k, E, guard = 50, 2, 4, 64
+    dt, code = T[dtype], {"fp32": 0, "bf16": 1}[dtype]
+    c, rows, mid, w, _, g = problem(R, k, E, C, dt, 0.0)
+    n = R * k
+    good = torch.randperm(n, generator=torch.Generator().manual_seed(1)).int().to(DEV).view(R, k)
+    bad = torch.tensor([n, n + 1, -1, -2, -2 ** 31, 2 ** 31 - 1, 2 ** 30, n + 63], dtype=torch.int32, device=DEV)
+    place = good.clone()
+    place[::3, 0] = bad.repeat(R)[:place[::3].shape[0]]
+    place[5, 1] = n
+    there = (place >= 0) & (place < n)
+    for end in (n, n + 1000, -1, -2 ** 31):
+        offsets = torch.tensor([0] * E + [end], dtype=torch.int32, device=DEV)
+
+        def held(count):
+            return torch.full((count + 2 * guard, C), 7.0, dtype=dt, device=DEV)
+
+        def inside(t):
+            assert bool((t[:guard] == 7).all()) and bool((t[-guard:] == 7).all())
+            return t[guard:-guard]
+        srt, out, d_mid = held(n), held(R), held(n)
+        d_w = torch.empty(R, k, device=DEV)
+        size = C * srt.element_size() * guard
+        assert h.cpfn_route_gather(rows.data_ptr(), place.data_ptr(), offsets.data_ptr(), R, k, E, C, code, srt.data_ptr() + size, st) == 0
+        assert h.cpfn_route_combine(mid.data_ptr(), w.data_ptr(), place.data_ptr(), R, k, C, code, out.data_ptr() + size, st) == 0
+        assert h.cpfn_route_combine_bwd(g.data_ptr(), mid.data_ptr(), w.data_ptr(), place.data_ptr(), offsets.data_ptr(), R, k, E, C, code,
+                                        d_mid.data_ptr() + size, d_w.data_ptr(), st) == 0
+        torch.cuda.synchronize()
+        srt, out, d_mid = inside(srt), inside(out), inside(d_mid)
+        if end >= n:                                              # (an earlier end's zeros and the rows are written in no order)
+            want = torch.full((n, C), 7.0, dtype=dt, device=DEV)
+            want[place[there].long()] = rows.detach().repeat_interleave(k, 0).view(R, k, C)[there]
+            assert torch.equal(srt, want)
+        picked = torch.where(there[:, :, None], mid.detach().double()[place.long().clamp(0, n - 1)], torch.zeros((), dtype=torch.float64, device=DEV))
+        assert_within(out, (Approx(picked) * Approx(w.detach().double()[:, :, None])).sum(1).view(R, C), "out")
+        assert_within(d_w, (Approx(picked) * Approx(g.double()[:, None, :])).sum(2).view(R, k), "d_weights")
+        assert not bool(d_w[~there].any())

@@ -203,3 +203,46 @@ def test_bytes_are_counted_for_the_native_calls():
     assert got["cpfn_norm_residual_bwd"] == (1, 3 * 64 * 32 * 4)
     autograd_ops.row_norm(x, torch.ones(32, device=DEV))
     assert lib.byte_census(False) == {}
+
+
+def test_a_captured_backward_pass_beside_an_eager_graph_of_the_same_leaves_is_refused():
+    """The leaf's accumulating node belongs to the default stream then, which cannot take part in a capture.  Without that graph the same
+    pass is captured, and its replays leave the eager pass's gradients."""
+    from cpfn_amd import autograd_ops, ops
+    torch.manual_seed(3)
+    P, C, k, E = 64, 32, 2, 4
+    x = torch.randn(P, C, device=DEV, requires_grad=True)
+    w = torch.rand(C, device=DEV, requires_grad=True)
+    plan = ops.route_plan(torch.randint(0, E, (P, k), device=DEV), E)
+    y = torch.randn(P * k, C, device=DEV, requires_grad=True)
+    rw = torch.rand(P, k, device=DEV, requires_grad=True)
+    g, gs = torch.randn(P, C, device=DEV), torch.randn(P * k, C, device=DEV)
+    cases = ((lambda: autograd_ops.row_norm(x, w), g, [x, w]), (lambda: autograd_ops.route_gather(x, plan), gs, [x]),
+             (lambda: autograd_ops.route_combine(y, rw, plan), g, [y, rw]))
+    for call, d, leaves in cases:
+        call().backward(d)
+        want = [t.grad.clone() for t in leaves]
+        for t in leaves:
+            t.grad = None
+        lives = call()
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="eager graph"):
+            with torch.cuda.graph(graph, stream=s):
+                call().backward(d)
+        torch.cuda.synchronize()
+        del lives
+        assert all(t.grad is None for t in leaves)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            call().backward(d)
+        for _ in range(3):
+            for t in leaves:
+                t.grad.zero_()
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(t.grad, v) for t, v in zip(leaves, want))
+        for t in leaves:
+            t.grad = None
