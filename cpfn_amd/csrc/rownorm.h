@@ -19,6 +19,11 @@
 // EACH: element by element (the whole tensor is smaller than a piece)
 enum NormMode { WHOLE, RAGGED, EACH };
 
+// What a launch has to do.  ANY: whatever pointers it is given, asked for step by step.  The whole block (y, its norm and the next norm)
+// has kernels of its own, without those branches, and without the registers of a gate where rows share one or there is none (BLOCK).
+// FRONT: no y (backward only; the forward kernel is as fast with its branches).
+enum NormForm { ANY, BLOCK, BLOCK_OWN, FRONT };
+
 // (rows of several waves have a workgroup of their own: its barriers then wait for nobody else)
 template <typename T, int L> struct NormShape {
   enum { THREADS = L <= 64 ? 256 : L, ROWS = THREADS / L, VN = cpfn_piece<T>::N, NP = 8 / VN };
@@ -232,6 +237,21 @@ template <typename T, int L, bool PARTIAL> __device__ __forceinline__ void param
   }
 }
 
+// scale weight and scale bias of a lane's channels: out = x + a (hat scale weight + scale bias)
+template <typename T, int L, bool PARTIAL>
+__device__ __forceinline__ void block_params(float *sw, float *sb, const float *weight, const float *bias, const float *scale, int lane, int C) {
+  float s[8];
+  param_load<T, L, PARTIAL>(sw, weight, lane, C, 1.f);
+  param_load<T, L, PARTIAL>(sb, bias, lane, C, 0.f);
+  param_load<T, L, PARTIAL>(s, scale, lane, C, 1.f);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) { sw[i] *= s[i]; sb[i] *= s[i]; }
+}
+
+// What was read is in registers of its own from here on: the next rows are requested into those that it was loaded into (without this
+// the compiler requests them first and moves every register).
+__device__ __forceinline__ void unpacked() { __builtin_amdgcn_sched_barrier(0); }
+
 // Sums of two values over a row's lanes.  L > 64: the waves of a row exchange their sums through LDS; the two halves of `slots`
 // take turns, so one barrier per call is enough (a half is rewritten only behind the NEXT call's barrier).  The fences are for LDS
 // alone: loads and stores of rows stay in flight across the barrier.
@@ -290,6 +310,23 @@ template <typename T> __device__ __forceinline__ float norm_sigmoid(float v) {
   return __builtin_amdgcn_rcpf(1.f + (sizeof(T) == 4 ? expf(-v) : __builtin_amdgcn_exp2f(v * -1.44269504f)));
 }
 
+template <typename T> __device__ __forceinline__ void gate_act(float *g, int sigmoid) {
+  if (!sigmoid) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) g[i] = norm_sigmoid<T>(g[i]);
+}
+// the gate that all rows of a group share, behind its activation (one without such a gate)
+template <typename T, int L> __device__ __forceinline__ void shared_gate(float *g, const T *row, int lane, int C, int sigmoid) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) g[i] = 1.f;
+  if (!row) return;
+  RowRaw<T, L> raw;
+  single_load<T, L>(raw, row, lane, C);
+  row_unpack(raw, g);
+  gate_act<T>(g, sigmoid);
+  arrived(g);
+}
+
 // ---------------------------------------------------------------- how the rows are split over workgroups (host)
 // the number of lanes for a row of C channels
 static inline int norm_lanes(int C) {
@@ -327,7 +364,7 @@ static inline NormSplit norm_split(long long P, int C, long long gate_rows, long
   }
   return s;
 }
-template <typename T> static inline NormMode norm_mode(long long P, int C, long long gate_rows) {
+template <typename T> static inline NormMode norm_mode(long long P, int C) {
   if (C % cpfn_piece<T>::N == 0) return WHOLE;
   return P * C * (long long)sizeof(T) < 16 ? EACH : RAGGED;
 }

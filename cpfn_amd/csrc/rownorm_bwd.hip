@@ -11,6 +11,15 @@
 //   d_weight = scale S1,  d_bias = scale S2,  d_scale = weight S1 + bias S2,  d_next_weight = S3,  d_next_bias = S4
 // (hat2 = y without a post-norm).  A lane owns its eight channels for every row of its workgroup, so a column sum is a register until
 // the workgroup ends; the workgroups' sums are added by a second small launch in a fixed order: no atomics, bit-reproducible.
+// d_gate of rows that share one: the factor of the sigmoid is the same for all of them and comes after the sum.
+//
+// Memory bound up to 512 channels; above, the barriers of the row sums (up to six a row) and the workgroups' sums (16 MB) show.
+// Measured (bf16, both launches):
+//   131072 x 128, layer, sigmoid gate for each row    57 us   4.7 TB/s      262144 x 64, rms, no gate      45 us   4.5 TB/s
+//   65536 x 512, rms, gate for each row              111 us   4.8 TB/s      100003 x 131, rms, no gate     51 us   3.1 TB/s
+//   32768 x 1024, layer, gate for 2048 rows          100 us   4.0 TB/s      fp32 20528 x 259, shared gate  36 us   3.5 TB/s
+// The kernels of the whole block without branches, against the one with them: 32768 x 1024 110 -> 100 us, 8192 x 4096 134 -> 109,
+// fp32 20528 x 259 44 -> 36; of the norm in front: 32768 x 1024 57 -> 52.
 #include "rownorm.h"
 
 namespace {
@@ -55,7 +64,7 @@ template <typename T, int L, typename F> __device__ __forceinline__ void slots_s
   }
 }
 
-template <typename T, int L, NormMode MODE>
+template <typename T, int L, NormMode MODE, NormForm FORM>
 __global__ __launch_bounds__((NormShape<T, L>::THREADS)) void norm_residual_bwd_kernel(const NormBwd<T> a) {
   constexpr int ROWS = NormShape<T, L>::ROWS, THREADS = NormShape<T, L>::THREADS, NP = NormShape<T, L>::NP;
   __shared__ float2 slots[16];
@@ -63,11 +72,11 @@ __global__ __launch_bounds__((NormShape<T, L>::THREADS)) void norm_residual_bwd_
   int turn = 0;
   const int lane = threadIdx.x & (L - 1), slot = threadIdx.x / L, C = a.C;
   const float inv_c = 1.f / (float)C;
-  const bool layer = a.layer != 0, post = a.weight != nullptr, has_y = a.y != nullptr, next = a.d_normed != nullptr, has_gate = a.gate != nullptr;
-  float w[8], b[8], s[8], nw[8], s1[8], s2[8], s3[8], s4[8], sg[8];
-  param_load<T, L, MODE != WHOLE>(w, a.weight, lane, C, 1.f);
-  param_load<T, L, MODE != WHOLE>(b, a.bias, lane, C, 0.f);
-  param_load<T, L, MODE != WHOLE>(s, a.scale, lane, C, 1.f);
+  const bool layer = a.layer != 0, post = FORM != ANY || a.weight != nullptr, has_y = FORM == FRONT ? false : FORM != ANY || a.y != nullptr, next = FORM != ANY || a.d_normed != nullptr;
+  constexpr bool may_y = FORM != FRONT, may_own = FORM == ANY || FORM == BLOCK_OWN;       // rows that may be there
+  const bool own = FORM == ANY ? a.gate != nullptr && !a.shared_gate : FORM == BLOCK_OWN;
+  float sw[8], sb[8], nw[8], s1[8], s2[8], s3[8], s4[8], sg[8];
+  block_params<T, L, MODE != WHOLE>(sw, sb, a.weight, a.bias, a.scale, lane, C);
   param_load<T, L, MODE != WHOLE>(nw, a.next_weight, lane, C, 1.f);
 #pragma unroll
   for (int i = 0; i < 8; ++i) { s1[i] = s2[i] = s3[i] = s4[i] = sg[i] = 0.f; }
@@ -84,68 +93,66 @@ __global__ __launch_bounds__((NormShape<T, L>::THREADS)) void norm_residual_bwd_
     }
     RowChunk<T, L, MODE> ch;
     ch.begin(row0, row1, a.P, C, lane, slot);
-    const T *own_gate = a.shared_gate ? nullptr : a.gate;
-    T *d_own_gate = a.shared_gate ? nullptr : a.d_gate;
+    const T *own_gate = own ? a.gate : nullptr;
+    T *d_own_gate = own ? a.d_gate : nullptr;
     const auto bx = ch.source(next ? a.x : nullptr), by = ch.source(a.y), bg = ch.source(own_gate), bd = ch.source(a.d_out), bn = ch.source(a.d_normed);
     const auto tx = ch.target(a.d_x), ty = ch.target(a.d_y), tg = ch.target(d_own_gate);
-    RowRaw<T, L> rx, ry, rg, rd, rn, shared;
+    RowRaw<T, L> rx, ry, rg, rd, rn;
     unsigned o[NP], sh[NP];
     const auto request = [&](unsigned step, long long r) {
       if (MODE == EACH) {
         each_load(rx, next ? a.x : nullptr, r, lane, C, r < row1);
-        each_load(ry, a.y, r, lane, C, r < row1);
-        each_load(rg, own_gate, r, lane, C, r < row1);
+        if (may_y) each_load(ry, a.y, r, lane, C, r < row1);
+        if (may_own) each_load(rg, own_gate, r, lane, C, r < row1);
         each_load(rd, a.d_out, r, lane, C, r < row1);
         each_load(rn, a.d_normed, r, lane, C, r < row1);
       } else {
         ch.at(o, sh, step, r < row1);
         ch.template load<true>(rx, bx, o);
-        ch.template load<true>(ry, by, o);
-        ch.template load<true>(rg, bg, o);
+        if (may_y) ch.template load<true>(ry, by, o);
+        if (may_own) ch.template load<true>(rg, bg, o);
         ch.template load<true>(rd, bd, o);
         ch.template load<true>(rn, bn, o);
       }
     };
+    const auto requested = [&] {
+      arrived(rx);
+      if (may_y) arrived(ry);
+      if (may_own) arrived(rg);
+      arrived(rd); arrived(rn);
+    };
     float gs[8];
-    if (a.shared_gate) {
-      single_load<T, L>(shared, a.gate + g * C, lane, C);
-      row_unpack(shared, gs);
-      arrived(gs);
-    }
-    arrived(w); arrived(b); arrived(s); arrived(nw);
+    shared_gate<T, L>(gs, a.shared_gate ? a.gate + g * C : nullptr, lane, C, a.sigmoid);
+    arrived(sw); arrived(sb); arrived(nw);
     request(0, row0 + slot);
-    arrived(rx); arrived(ry); arrived(rg); arrived(rd); arrived(rn);
+    requested();
     unsigned step = 0;
     for (long long base = row0; base < row1; base += ROWS, step += set_bytes) {
       const long long r = base + slot;
       const bool there = r < row1;
       const float eps = there ? a.eps : 1.f;
-      RowRaw<T, L> cx = rx, cy = ry, cg = rg, cd = rd, cn = rn;
-      unsigned csh[NP];
-#pragma unroll
-      for (int q = 0; q < NP; ++q) csh[q] = MODE == RAGGED ? sh[q] : 0u;
-      request(step + set_bytes, r + ROWS);
-      ch.settle(cx, csh); ch.settle(cy, csh); ch.settle(cg, csh); ch.settle(cd, csh); ch.settle(cn, csh);
-      float hat2[8], ga[8], r2 = 0.f;
-      if (has_y) {
-        row_unpack(cy, hat2);
-        if (post) r2 = row_normalise<T, L, MODE>(hat2, lane, C, inv_c, layer, eps, slots, turn);
-        row_unpack(cg, ga);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float t = a.shared_gate ? gs[i] : ga[i];
-          ga[i] = !has_gate ? 1.f : a.sigmoid ? norm_sigmoid<T>(t) : t;
-        }
+      float h[8], hat2[8], ga[8], D[8], dn[8], r2 = 0.f;
+      ch.settle(rx, sh); ch.settle(rd, sh); ch.settle(rn, sh);
+      row_unpack(rx, h);
+      row_unpack(rd, D);
+      row_unpack(rn, dn);
+      if (may_y) {
+        ch.settle(ry, sh);
+        row_unpack(ry, hat2);
       }
-      float D[8];
-      row_unpack(cd, D);
+      if (may_own) {
+        ch.settle(rg, sh);
+        row_unpack(rg, ga);
+      }
+      unpacked();
+      request(step + set_bytes, r + ROWS);
+      if (has_y && post) r2 = row_normalise<T, L, MODE>(hat2, lane, C, inv_c, layer, eps, slots, turn);
+      if (own) gate_act<T>(ga, a.sigmoid);
+      const auto gate = [&](int i) { return own ? ga[i] : gs[i]; };
       if (next) {
-        float h[8], dn[8];
-        row_unpack(cx, h);
-        row_unpack(cn, dn);
         if (has_y) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) h[i] = fmaf(s[i], ga[i] * fmaf(hat2[i], w[i], b[i]), h[i]);
+          for (int i = 0; i < 8; ++i) h[i] = fmaf(gate(i), fmaf(hat2[i], sw[i], sb[i]), h[i]);
         }
         const float r1 = row_normalise<T, L, MODE>(h, lane, C, inv_c, layer, eps, slots, turn);
         float m1 = 0.f, m2 = 0.f;
@@ -167,23 +174,23 @@ __global__ __launch_bounds__((NormShape<T, L>::THREADS)) void norm_residual_bwd_
       else ch.store(tx, step, D);
       float e[8], dg[8];
       if (has_y) {
-        float m1 = 0.f, m2 = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float da = D[i] * ga[i];
-          s1[i] = fmaf(da, hat2[i], s1[i]);
-          s2[i] += da;
-          e[i] = da * s[i] * w[i];                       // (w = 1 without a post-norm: e = du)
-          m1 += e[i];
-          m2 = fmaf(e[i], hat2[i], m2);
-        }
         if (a.d_gate) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            dg[i] = D[i] * s[i] * fmaf(hat2[i], w[i], b[i]);
-            if (a.sigmoid) dg[i] *= ga[i] * (1.f - ga[i]);
-            sg[i] += dg[i];
+            dg[i] = D[i] * fmaf(hat2[i], sw[i], sb[i]);
+            if (own) dg[i] *= a.sigmoid ? ga[i] * (1.f - ga[i]) : 1.f;
+            else sg[i] += dg[i];
           }
+        }
+        float m1 = 0.f, m2 = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float da = D[i] * gate(i);
+          s1[i] = fmaf(da, hat2[i], s1[i]);
+          s2[i] += da;
+          e[i] = da * sw[i];                             // (sw = scale without a post-norm: e = du)
+          m1 += e[i];
+          m2 = fmaf(e[i], hat2[i], m2);
         }
         if (post) {
           row_sum2<L>(m1, m2, slots, turn);
@@ -194,18 +201,24 @@ __global__ __launch_bounds__((NormShape<T, L>::THREADS)) void norm_residual_bwd_
         }
       }
       if (MODE == EACH) {
-        each_store<T, L>(d_own_gate, r, lane, C, there, dg);
-        each_store<T, L>(a.d_y, r, lane, C, there, e);
+        if (may_own) each_store<T, L>(d_own_gate, r, lane, C, there, dg);
+        if (may_y) each_store<T, L>(a.d_y, r, lane, C, there, e);
       } else {
-        ch.store(tg, step, dg);
-        ch.store(ty, step, e);
+        if (may_own) ch.store(tg, step, dg);
+        if (may_y) ch.store(ty, step, e);
       }
-      arrived(rx); arrived(ry); arrived(rg); arrived(rd); arrived(rn);
+      requested();
     }
-    if (a.shared_gate && a.d_gate && a.blocks_per_group == 1) {        // this workgroup has seen all rows of the gate's row
-      slots_sum<T, L>(sg, comb, C, [&](int c, float v) { a.d_gate[g * C + c] = cpfn_from_f32<T>(v); });
+    if (a.shared_gate && a.d_gate) {
+      if (a.sigmoid) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sg[i] = 0.f;
+        for (int i = 0; i < 8; ++i) sg[i] *= gs[i] * (1.f - gs[i]);
+      }
+      if (a.blocks_per_group == 1) {                     // this workgroup has seen all rows of the gate's row
+        slots_sum<T, L>(sg, comb, C, [&](int c, float v) { a.d_gate[g * C + c] = cpfn_from_f32<T>(v); });
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sg[i] = 0.f;
+      }
     }
   }
   float *part = a.part + (size_t)blockIdx.x * nsums * C;
@@ -266,14 +279,20 @@ template <typename T> __global__ __launch_bounds__(1024) void norm_residual_redu
   }
 }
 
-// two waves for each SIMD are resident together; at least four row sets for each workgroup, or its sums cost as much as its rows
+// Two waves on each SIMD run at once; at least four row sets for each workgroup, or its sums cost as much as its rows.  (Where three fit
+// the registers they measured 0 to 30 % slower: more workgroups' sums, and two keep enough rows in flight.)
 NormSplit split(long long P, int C, long long gate_rows) { return norm_split(P, C, gate_rows, 2048, 4); }
 
-template <typename T, int L> void launch(const NormBwd<T> &a, int nblk, NormMode mode, hipStream_t st) {
+template <typename T, int L, NormForm FORM> void launch_form(const NormBwd<T> &a, int nblk, NormMode mode, hipStream_t st) {
   constexpr int THREADS = NormShape<T, L>::THREADS;
-  if (mode == WHOLE) norm_residual_bwd_kernel<T, L, WHOLE><<<nblk, THREADS, 0, st>>>(a);
-  // (ragged fp32 rows of more than 2048 channels: the registers of 512 lanes do not hold what the piecewise form needs)
-  else norm_residual_bwd_kernel<T, L, L == 512 && sizeof(T) == 4 ? EACH : RAGGED><<<nblk, THREADS, 0, st>>>(a);
+  if (mode == WHOLE) norm_residual_bwd_kernel<T, L, WHOLE, FORM><<<nblk, THREADS, 0, st>>>(a);
+  else norm_residual_bwd_kernel<T, L, RAGGED, FORM><<<nblk, THREADS, 0, st>>>(a);
+}
+template <typename T, int L> void launch(const NormBwd<T> &a, int nblk, NormMode mode, hipStream_t st) {
+  if (!a.d_normed || (a.y && !a.weight)) launch_form<T, L, ANY>(a, nblk, mode, st);
+  else if (!a.y) launch_form<T, L, FRONT>(a, nblk, mode, st);
+  else if (a.gate && !a.shared_gate) launch_form<T, L, BLOCK_OWN>(a, nblk, mode, st);
+  else launch_form<T, L, BLOCK>(a, nblk, mode, st);
 }
 
 struct Grads { float *d_weight, *d_bias, *d_scale, *d_next_weight, *d_next_bias; };
@@ -294,9 +313,9 @@ int backward(const void *x, const void *y, const void *gate, const float *weight
   a.shared_gate = gate && gate_rows < P;
   a.sums12 = d.d_weight || d.d_bias || d.d_scale;
   a.sums34 = d.d_next_weight || d.d_next_bias;
-  const NormMode mode = norm_mode<T>(P, C, gate_rows);
+  const NormMode mode = norm_mode<T>(P, C);
   if (mode == EACH) {
-    norm_residual_bwd_kernel<T, 8, EACH><<<s.nblk, 256, 0, st>>>(a);
+    norm_residual_bwd_kernel<T, 8, EACH, ANY><<<s.nblk, 256, 0, st>>>(a);
   } else {
     switch (norm_lanes(C)) {
       case 8: launch<T, 8>(a, s.nblk, mode, st); break;

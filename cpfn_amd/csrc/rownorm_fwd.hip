@@ -1,6 +1,10 @@
 // Norms before and after a residual block, its gate and its residual scale in one pass over the rows (forward; the formulas are in
 // rownorm.h).  Memory bound: x, y and the gate are read once, out and normed written once; the op-by-op form moves each of the ~12
-// intermediate tensors through memory.
+// intermediate tensors through memory.  Measured (bf16; a copy of gigabytes reaches 4.9 TB/s, one that fits the last-level cache 8.6):
+//   131072 x 128, layer, sigmoid gate for each row    33 us   5.1 TB/s      262144 x 64, rms, no gate      21 us   6.3 TB/s
+//   65536 x 512, rms, gate for each row               64 us   5.2 TB/s      100003 x 131, rms, no gate     25 us   4.2 TB/s
+//   32768 x 1024, layer, gate for 2048 rows           55 us   4.9 TB/s      fp32 20528 x 259, shared gate  18 us   4.8 TB/s
+// Ragged rows cost instructions (masks of the last piece, three more stores).
 #include "rownorm.h"
 
 namespace {
@@ -15,18 +19,17 @@ template <typename T> struct NormFwd {
   T *out, *normed;
 };
 
-template <typename T, int L, NormMode MODE>
+template <typename T, int L, NormMode MODE, NormForm FORM>
 __global__ __launch_bounds__((NormShape<T, L>::THREADS)) void norm_residual_fwd_kernel(const NormFwd<T> a) {
   constexpr int ROWS = NormShape<T, L>::ROWS, NP = NormShape<T, L>::NP;
   __shared__ float2 slots[16];
   int turn = 0;
   const int lane = threadIdx.x & (L - 1), slot = threadIdx.x / L, C = a.C;
   const float inv_c = 1.f / (float)C;
-  const bool layer = a.layer != 0, post = a.weight != nullptr, has_y = a.y != nullptr, has_gate = a.gate != nullptr;
-  float w[8], b[8], s[8], nw[8], nb[8];
-  param_load<T, L, MODE != WHOLE>(w, a.weight, lane, C, 1.f);
-  param_load<T, L, MODE != WHOLE>(b, a.bias, lane, C, 0.f);
-  param_load<T, L, MODE != WHOLE>(s, a.scale, lane, C, 1.f);
+  const bool layer = a.layer != 0, post = FORM != ANY || a.weight != nullptr, has_y = FORM != ANY || a.y != nullptr, next = FORM != ANY || a.normed != nullptr;
+  const bool own = FORM == ANY ? a.gate != nullptr && !a.shared_gate : FORM == BLOCK_OWN;
+  float sw[8], sb[8], nw[8], nb[8];
+  block_params<T, L, MODE != WHOLE>(sw, sb, a.weight, a.bias, a.scale, lane, C);
   param_load<T, L, MODE != WHOLE>(nw, a.next_weight, lane, C, 1.f);
   param_load<T, L, MODE != WHOLE>(nb, a.next_bias, lane, C, 0.f);
   const long long g0 = a.blocks_per_group > 1 ? blockIdx.x / a.blocks_per_group : (long long)blockIdx.x * a.groups_per_block;
@@ -41,67 +44,55 @@ __global__ __launch_bounds__((NormShape<T, L>::THREADS)) void norm_residual_fwd_
     }
     RowChunk<T, L, MODE> ch;
     ch.begin(row0, row1, a.P, C, lane, slot);
-    const auto sx = ch.source(a.x), sy = ch.source(a.y), sg = ch.source(a.shared_gate ? nullptr : a.gate);
+    const T *own_gate = own ? a.gate : nullptr;
+    const auto sx = ch.source(a.x), sy = ch.source(a.y), sg = ch.source(own_gate);
     const auto to = ch.target(a.out), tn = ch.target(a.normed);
-    RowRaw<T, L> rx, ry, rg, shared;
+    RowRaw<T, L> rx, ry, rg;
     unsigned o[NP], sh[NP];
     const auto request = [&](unsigned step, long long r) {
       if (MODE == EACH) {
         each_load(rx, a.x, r, lane, C, r < row1);
         each_load(ry, a.y, r, lane, C, r < row1);
-        each_load(rg, a.shared_gate ? nullptr : a.gate, r, lane, C, r < row1);
+        if (FORM != BLOCK) each_load(rg, own_gate, r, lane, C, r < row1);
       } else {
         ch.at(o, sh, step, r < row1);
         ch.load(rx, sx, o);
         ch.load(ry, sy, o);
-        ch.load(rg, sg, o);
+        if (FORM != BLOCK) ch.load(rg, sg, o);
       }
     };
-    if (a.shared_gate) single_load<T, L>(shared, a.gate + g * C, lane, C);
     float gs[8];
-    if (a.shared_gate) row_unpack(shared, gs);
-    if (a.shared_gate) arrived(gs);
-    arrived(w); arrived(b); arrived(s); arrived(nw); arrived(nb);
+    shared_gate<T, L>(gs, a.shared_gate ? a.gate + g * C : nullptr, lane, C, a.sigmoid);
+    arrived(sw); arrived(sb); arrived(nw); arrived(nb);
     request(0, row0 + slot);
-    arrived(rx); arrived(ry); arrived(rg);
+    arrived(rx); arrived(ry);
+    if (FORM != BLOCK) arrived(rg);
     unsigned step = 0;
     // (every row slot of a workgroup takes part in the barriers of row_sum: the loop runs over whole row sets)
     for (long long base = row0; base < row1; base += ROWS, step += set_bytes) {
       const long long r = base + slot;
       const bool there = r < row1;
       const float eps = there ? a.eps : 1.f;
-      RowRaw<T, L> cx = rx, cy = ry, cg = rg;
-      unsigned csh[NP];
-#pragma unroll
-      for (int q = 0; q < NP; ++q) csh[q] = MODE == RAGGED ? sh[q] : 0u;
+      float v[8], u[8], ga[8];
+      ch.settle(rx, sh);
+      row_unpack(rx, v);
+      ch.settle(ry, sh);
+      row_unpack(ry, u);
+      if (FORM != BLOCK) {
+        ch.settle(rg, sh);
+        row_unpack(rg, ga);
+      }
+      unpacked();
       request(step + set_bytes, r + ROWS);
-      ch.settle(cx, csh);
-      float v[8], u[8];
-      row_unpack(cx, v);
       if (has_y) {
-        ch.settle(cy, csh);
-        row_unpack(cy, u);
-        if (post) {
-          row_normalise<T, L, MODE>(u, lane, C, inv_c, layer, eps, slots, turn);
+        if (post) row_normalise<T, L, MODE>(u, lane, C, inv_c, layer, eps, slots, turn);
+        if (own) gate_act<T>(ga, a.sigmoid);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) u[i] = fmaf(u[i], w[i], b[i]);
-        }
-        if (has_gate) {
-          float gv[8];
-          ch.settle(cg, csh);
-          row_unpack(cg, gv);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float t = a.shared_gate ? gs[i] : gv[i];
-            u[i] *= a.sigmoid ? norm_sigmoid<T>(t) : t;
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = fmaf(s[i], u[i], v[i]);
+        for (int i = 0; i < 8; ++i) v[i] = fmaf(own ? ga[i] : gs[i], fmaf(u[i], sw[i], sb[i]), v[i]);
       }
       if (MODE == EACH) each_store<T, L>(a.out, r, lane, C, there, v);
       else ch.store(to, step, v);
-      if (a.normed) {
+      if (next) {
         // (of the fp32 sum, not of its rounded copy in `out`)
         row_normalise<T, L, MODE>(v, lane, C, inv_c, layer, eps, slots, turn);
 #pragma unroll
@@ -109,16 +100,21 @@ __global__ __launch_bounds__((NormShape<T, L>::THREADS)) void norm_residual_fwd_
       }
       if (MODE == EACH) each_store<T, L>(a.normed, r, lane, C, there, v);
       else ch.store(tn, step, v);
-      arrived(rx); arrived(ry); arrived(rg);
+      arrived(rx); arrived(ry);
+      if (FORM != BLOCK) arrived(rg);
     }
   }
 }
 
-
-template <typename T, int L> void launch(const NormFwd<T> &a, int nblk, NormMode mode, hipStream_t st) {
+template <typename T, int L, NormForm FORM> void launch_form(const NormFwd<T> &a, int nblk, NormMode mode, hipStream_t st) {
   constexpr int THREADS = NormShape<T, L>::THREADS;
-  if (mode == WHOLE) norm_residual_fwd_kernel<T, L, WHOLE><<<nblk, THREADS, 0, st>>>(a);
-  else norm_residual_fwd_kernel<T, L, RAGGED><<<nblk, THREADS, 0, st>>>(a);
+  if (mode == WHOLE) norm_residual_fwd_kernel<T, L, WHOLE, FORM><<<nblk, THREADS, 0, st>>>(a);
+  else norm_residual_fwd_kernel<T, L, RAGGED, FORM><<<nblk, THREADS, 0, st>>>(a);
+}
+template <typename T, int L> void launch(const NormFwd<T> &a, int nblk, NormMode mode, hipStream_t st) {
+  if (!(a.y && a.weight && a.normed)) launch_form<T, L, ANY>(a, nblk, mode, st);
+  else if (a.gate && !a.shared_gate) launch_form<T, L, BLOCK_OWN>(a, nblk, mode, st);
+  else launch_form<T, L, BLOCK>(a, nblk, mode, st);
 }
 
 template <typename T>
@@ -126,8 +122,8 @@ int forward(const void *x, const void *y, const void *gate, const float *weight,
             const float *next_weight, const float *next_bias, long long P, int C, long long gate_rows, int layer, int sigmoid, float eps,
             void *out, void *normed, hipStream_t st) {
   if (!gate) gate_rows = 0;
-  const NormSplit s = norm_split(P, C, gate_rows, sizeof(T) == 4 ? 3072 : 4096, 1);       // waves that are resident together: three (fp32:
-                                                                                              // 130 to 154 registers) or four for each SIMD
+  // four waves on each of the 1024 SIMDs run at once (87 to 129 registers; five, where they fit, measured 0 to 10 % slower)
+  const NormSplit s = norm_split(P, C, gate_rows, 4 * 1024, 1);
   NormFwd<T> a;
   a.x = (const T *)x; a.y = (const T *)y; a.gate = (const T *)gate;
   a.weight = weight; a.bias = bias; a.scale = scale; a.next_weight = next_weight; a.next_bias = next_bias;
@@ -135,9 +131,9 @@ int forward(const void *x, const void *y, const void *gate, const float *weight,
   a.blocks_per_group = s.blocks_per_group; a.groups_per_block = s.groups_per_block; a.shared_gate = gate && gate_rows < P;
   a.C = C; a.layer = layer; a.sigmoid = sigmoid; a.eps = eps;
   a.out = (T *)out; a.normed = (T *)normed;
-  const NormMode mode = norm_mode<T>(P, C, gate_rows);
+  const NormMode mode = norm_mode<T>(P, C);
   if (mode == EACH) {
-    norm_residual_fwd_kernel<T, 8, EACH><<<s.nblk, 256, 0, st>>>(a);
+    norm_residual_fwd_kernel<T, 8, EACH, ANY><<<s.nblk, 256, 0, st>>>(a);
     return cpfn_launch_status();
   }
   switch (norm_lanes(C)) {

@@ -168,6 +168,15 @@ def test_a_gate_shared_by_groups_of_rows(groups, each, C):
         check(*_args(groups * each, C, dtype, groups, seed=groups), kind="rms", act=act)
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("C", [40, 63, 104, 127, 240, 251, 472, 509, 936, 1021, 1928, 2045, 3080, 4091])
+def test_every_form_at_every_number_of_lanes(C, dtype):
+    """Rows of one to eight waves, whole and ragged: the whole block with its own gate, a shared one and none, the norm in front, and what
+    has no kernel of its own (no norm of y)."""
+    for P, groups, kw in ((10, 10, {}), (10, 5, {}), (10, 0, {"bias": False}), (10, 0, {"y": False}), (10, 10, {"post": False}), (10, 0, {"nxt": False})):
+        check(*_args(P, C, dtype, groups, seed=C, **kw), kind="layer", act="sigmoid")
+
+
 @pytest.mark.parametrize("missing", ["out", "normed"])
 @pytest.mark.parametrize("gate", [0, 30, 3])
 def test_a_result_without_a_gradient(missing, gate):
