@@ -1,4 +1,4 @@
-// The norm over all gradients of a model, and their clipping, in two launches for each LIST_MAX tensors of mixed types and lengths.
+// The norm over all gradients of a model, and their clipping, in two launches (lists of up to 130 tensors, of mixed types and lengths).
 //
 //   norm = (sum |g|^p)^(1/p), p = 1, 2 or infinity (the largest |g|);   coef = min(1, max_norm / (norm + 1e-6));   out = coef g
 //
@@ -15,7 +15,7 @@
 
 namespace {
 
-constexpr int LIST_MAX = 104, GN_THREADS = 256;        // (4 KB of kernel arguments)
+constexpr int GN_THREADS = 256;
 // Elements of a workgroup before the workgroups are limited (1.4M values in 60 tensors, both launches: 4096 10.8 us, 16384 13.1) ...
 constexpr int SHARE = 4096;
 // ... to about so many in a call, one more for a tensor's last share: up to 48 long tensors stay within the 2048 that run at once, 8 on
@@ -24,19 +24,32 @@ constexpr int MOST_BLOCKS = 2000;
 constexpr long long KEPT = 48ll << 20;     // elements at the end of the list that pass 1 leaves in the last-level cache (96 or 192 of its 256 MB)
 // partial sums that the scaling workgroups add themselves (above, in lists of hundreds of tensors, one launch in between does): 2000 of
 // them cost a workgroup less than that launch (33.5 -> 32.2 us where nothing is left to scale)
-constexpr int DIRECT_PARTS = MOST_BLOCKS + 2 * LIST_MAX;
+constexpr int DIRECT_PARTS = MOST_BLOCKS + 256;
 
-struct List {
-  const void *src[LIST_MAX];
-  void *dst[LIST_MAX];
-  long long n[LIST_MAX];
-  long long from_end[LIST_MAX];            // elements of the whole call from the tensor's first one to the end of the list
-  int block0[LIST_MAX + 1];                // first workgroup of each tensor
-  unsigned char from[LIST_MAX], to[LIST_MAX];
+// What a launch's arguments hold of a list.  Pass 1 takes more tensors (301 short ones: 23.7 -> 20.4 us).
+struct Sources {
+  enum { MAX = 186 };
+  const void *src[MAX];
+  long long n[MAX];
+  int block0[MAX + 1];                     // first workgroup of each tensor
+  unsigned char from[MAX];
   int count;
 };
+struct Moves {
+  enum { MAX = 130 };
+  const void *src[MAX];
+  long long n[MAX];
+  int block0[MAX + 1];
+  unsigned char from[MAX];
+  int count;
+  void *dst[MAX];
+  unsigned char to[MAX];
+};
+static_assert(sizeof(Sources) <= 4032 && sizeof(Moves) <= 4032, "4 KB of kernel arguments");
+// Where the elements begin that pass 1 leaves in the last-level cache: element `at` of the launch's tensor `tensor`
+struct Kept { int tensor; long long at; };
 
-__device__ __forceinline__ int list_find(const List &a, int blk) {              // the last tensor with block0 <= blk
+template <typename List> __device__ __forceinline__ int list_find(const List &a, int blk) {              // the last tensor with block0 <= blk
   int lo = 0, hi = a.count - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
@@ -109,13 +122,12 @@ template <int P, typename T> __device__ __forceinline__ double gn_share(const T 
   return gn_join<P>(gn_join<P>(acc[0], acc[1]), gn_join<P>(acc[2], acc[3]));
 }
 
-template <int P> __global__ __launch_bounds__(GN_THREADS, 8) void grad_norm_kernel(const List a, long long kept, double *__restrict__ part) {
+template <int P> __global__ __launch_bounds__(GN_THREADS, 8) void grad_norm_kernel(const Sources a, const Kept kept, double *__restrict__ part) {
   __shared__ double lds[GN_THREADS / 64];
   const int d = list_find(a, blockIdx.x);
   const long long first = (long long)(blockIdx.x - a.block0[d]) * GN_THREADS + threadIdx.x;
   const long long step = (long long)(a.block0[d + 1] - a.block0[d]) * GN_THREADS;
-  // the last `kept` elements of this launch's list are the ones that the scaling pass begins with
-  const long long n = a.n[d], behind = a.from_end[d] - kept, keep = behind <= 0 ? 0 : behind < n ? behind : n;
+  const long long n = a.n[d], keep = d < kept.tensor ? n : d > kept.tensor ? 0 : kept.at;
   double v = 0.0;
   if (a.from[d] == CPFN_F32) v = gn_share<P>((const float *)a.src[d], n, keep, first, step);
   else if (a.from[d] == CPFN_BF16) v = gn_share<P>((const cpfn_bf16 *)a.src[d], n, keep, first, step);
@@ -183,7 +195,7 @@ __device__ __forceinline__ void scale_share(const T *__restrict__ p, U *__restri
 // parts == 0: `part` is the norm itself.  elsewhere: the results go to other tensors (always written); in place nothing is to be done
 // where the factor is 1.
 template <int P>
-__global__ __launch_bounds__(GN_THREADS) void grad_scale_kernel(const List a, const double *__restrict__ part, int parts, double max_norm,
+__global__ __launch_bounds__(GN_THREADS) void grad_scale_kernel(const Moves a, const double *__restrict__ part, int parts, double max_norm,
                                                                 int elsewhere, float *__restrict__ norm) {
   __shared__ double lds[GN_THREADS / 64];
   const double total = parts ? gn_total<P>(part, parts, lds) : *part;
@@ -244,44 +256,44 @@ bool overlapping(const void *const *src, void *const *dst, const long long *n, c
   return false;
 }
 
+void set_target(Sources &, int, void *, int) {}
+void set_target(Moves &a, int c, void *dst, int to) { a.dst[c] = dst; a.to[c] = (unsigned char)to; }
+
 // tensors base.. of the list into `a`; returns the index behind the last one taken.  Empty tensors take no place.
-// left: elements from tensor `base` on; taken down by what was put into `a`.
-int fill(List &a, int base, const void *const *src, void *const *dst, const long long *n, const int *from, const int *to, int count, long long share,
-         long long &left) {
+template <typename List>
+int fill(List &a, int base, const void *const *src, void *const *dst, const long long *n, const int *from, const int *to, int count, long long share) {
   a.count = 0;
   a.block0[0] = 0;
   int i = base;
-  for (; i < count && a.count < LIST_MAX; ++i) {
+  for (; i < count && a.count < List::MAX; ++i) {
     if (n[i] == 0) continue;
     const int c = a.count++;
     a.src[c] = src[i];
-    a.dst[c] = dst ? dst[i] : nullptr;
     a.n[c] = n[i];
-    a.from_end[c] = left;
-    left -= n[i];
     a.from[c] = (unsigned char)from[i];
-    a.to[c] = (unsigned char)(to ? to[i] : from[i]);
     a.block0[c + 1] = a.block0[c] + blocks_of(n[i], share);
+    set_target(a, c, dst ? dst[i] : nullptr, to ? to[i] : from[i]);
   }
   return i;
-}
-
-long long sum_of(const long long *n, int count) {
-  long long sum = 0;
-  for (int i = 0; i < count; ++i) sum += n[i];
-  return sum;
 }
 
 // kept: so many elements from the list's end are read again soon
 template <int P>
 int norm_pass(const void *const *src, const long long *n, const int *type, int count, long long share, long long kept, double *part, hipStream_t st) {
   int parts = 0;
-  long long left = sum_of(n, count);
+  long long streamed = -kept;                           // elements in front of those
+  for (int i = 0; i < count; ++i) streamed += n[i];
   for (int base = 0; base < count;) {
-    List a;
-    base = fill(a, base, src, nullptr, n, type, nullptr, count, share, left);
+    Sources a;
+    base = fill(a, base, src, nullptr, n, type, nullptr, count, share);
     if (a.count == 0) break;
-    grad_norm_kernel<P><<<a.block0[a.count], GN_THREADS, 0, st>>>(a, kept, part + parts);
+    Kept k = {0, 0};
+    for (; k.tensor < a.count && streamed >= a.n[k.tensor]; ++k.tensor) streamed -= a.n[k.tensor];
+    if (k.tensor < a.count && streamed > 0) {
+      k.at = streamed;
+      streamed = 0;
+    }
+    grad_norm_kernel<P><<<a.block0[a.count], GN_THREADS, 0, st>>>(a, k, part + parts);
     parts += a.block0[a.count];
   }
   return parts;
@@ -300,10 +312,9 @@ int run(const void *const *src, void *const *dst, const long long *n, const int 
     if (!clip || parts == 0) return cpfn_launch_status();
     parts = 0;
   }
-  long long left = sum_of(n, count);
   for (int base = 0; base < count;) {
-    List a;
-    base = fill(a, base, src, dst, n, from, to, count, share, left);
+    Moves a;
+    base = fill(a, base, src, dst, n, from, to, count, share);
     if (a.count == 0) break;
     grad_scale_kernel<P><<<a.block0[a.count], GN_THREADS, 0, st>>>(a, part, parts, max_norm, elsewhere ? 1 : 0, norm);
     norm = nullptr;

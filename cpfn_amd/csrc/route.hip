@@ -18,13 +18,17 @@ namespace {
 // counter of that expert: no atomics, so the order is the input's order by construction.
 // ITEMS: 64-choice steps of a wave.  4 up to RANK_SMALL choices (more workgroups: 60000 choices, 28 experts 10.6 -> 8.3 us), 8 above (fewer
 // counts to scan: 4000000 choices, 2000 experts 57 -> 44 us; 4194304, 128: 30.9 -> 30.5).
+//
+// Measured: 4194304 choices, 128 experts 26 us, 1.9 TB/s of choices and places (a choice is read twice; without the ranks' arithmetic 22);
+// 4000000, 2000 experts 38 us; 60000, 28 experts 7.6 us, two launches.
 constexpr int RANK_WAVES = 8;
 constexpr long long RANK_SMALL = 1 << 19;
 constexpr int rank_tile(int items) { return RANK_WAVES * items * 64; }
 int rank_items(long long n) { return n <= RANK_SMALL ? 4 : 8; }
 constexpr int ROUTE_MAX_E = 2048;                 // a 16-bit counter for each wave (a tile has 4096 choices at most) and a base: 40 KB of LDS
-// up to so many tiles and experts every workgroup sums the tiles' counts by itself, instead of a launch that does it once
-constexpr int DIRECT_TILES = 64, DIRECT_E = 256;
+// Every workgroup sums the tiles' counts by itself, instead of a launch that does it once, where a wave loads up to 8 times for it (64
+// tiles of an expert each time; of 8 waves): 262144 choices, 8 experts 7.5 us (launch: 9.6), 64 experts 11.0 (10.2); 130000, 128 11.7 (10.0)
+constexpr int DIRECT_LOADS = 64;
 
 template <typename I> __device__ __forceinline__ int expert_of(const I *__restrict__ choice, long long i, long long n, int E) {
   if (i >= n) return -1;
@@ -80,12 +84,15 @@ __global__ __launch_bounds__(RANK_WAVES * 64) void route_count_kernel(const I *_
   for (int x = threadIdx.x; x < E; x += RANK_WAVES * 64) counts[(long long)blockIdx.x * E + x] = (int)lds[x];
 }
 
-__device__ __forceinline__ int wave_scan(int v, int lane) {                       // inclusive
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int u = __shfl_up(v, d, 64);
-    if (lane >= d) v += u;
-  }
+// inclusive sums over a wave (in registers: six exchanges through LDS cost 0.5 to 3 us of a list's order): inside rows of 16 lanes, then each row's last sum into the rows behind it
+template <int CTRL, int ROWS> __device__ __forceinline__ int moved_up(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false); }
+__device__ __forceinline__ int wave_scan(int v) {
+  v += moved_up<0x111, 0xf>(v);                   // row_shr 1, 2, 4, 8
+  v += moved_up<0x112, 0xf>(v);
+  v += moved_up<0x114, 0xf>(v);
+  v += moved_up<0x118, 0xf>(v);
+  v += moved_up<0x142, 0xa>(v);                   // lane 15 to row 1, lane 47 to row 3
+  v += moved_up<0x143, 0xc>(v);                   // lane 31 to rows 2 and 3
   return v;
 }
 
@@ -103,7 +110,7 @@ __global__ __launch_bounds__(1024) void route_scan_kernel(int *__restrict__ coun
   __syncthreads();
   {                                                // a wave for each expert: the stretches' sums -> exclusive
     const int lane = threadIdx.x & 63, wx = threadIdx.x >> 6;
-    const int v = part[lane][wx], up_to = wave_scan(v, lane);
+    const int v = part[lane][wx], up_to = wave_scan(v);
     part[lane][wx] = up_to - v;
     if (lane == 63 && blockIdx.x * 16 + wx < E) totals[blockIdx.x * 16 + wx] = up_to;
   }
@@ -129,7 +136,7 @@ __global__ __launch_bounds__(RANK_WAVES * 64) void route_rank_kernel(const I *__
                                                                      const int *__restrict__ totals, int *__restrict__ offsets,
                                                                      int *__restrict__ place) {
   extern __shared__ unsigned lds[];               // [waves][E] 16-bit counters | [E] first position of this tile's
-  __shared__ int wsum[RANK_WAVES], d_before[DIRECT_E], d_total[DIRECT_E];
+  __shared__ int wsum[RANK_WAVES], d_before[DIRECT_LOADS], d_total[DIRECT_LOADS];
   constexpr int THREADS = RANK_WAVES * 64;
   unsigned short *cnt = (unsigned short *)lds;
   int *base = (int *)(lds + RANK_WAVES * E / 2);
@@ -139,12 +146,18 @@ __global__ __launch_bounds__(RANK_WAVES * 64) void route_rank_kernel(const I *__
   int e[RANK_ITEMS], rank[RANK_ITEMS];
 #pragma unroll
   for (int t = 0; t < RANK_ITEMS; ++t) e[t] = expert_of(choice, i0 + t * 64, n, E);
-  if (mode == 1) {                                // tiles <= 64: a lane for each tile, a wave for each expert
+  if (mode == 1) {                                // a wave for each expert, its lanes share out the tiles
     for (int x = wave; x < E; x += RANK_WAVES) {
-      const int v = lane < tiles ? counts[lane * E + x] : 0;
-      const int s = wave_scan(v, lane);
-      if (lane == (int)blockIdx.x) d_before[x] = s - v;
-      if (lane == 63) d_total[x] = s;
+      int before = 0, total = 0;
+#pragma unroll 4
+      for (int t = lane; t < tiles; t += 64) {
+        const int v = counts[t * E + x];
+        total += v;
+        before += t < (int)blockIdx.x ? v : 0;
+      }
+      total = wave_scan(total);
+      before = wave_scan(before);
+      if (lane == 63) { d_total[x] = total; d_before[x] = before; }
     }
   }
   zero_counters(cnt, E);
@@ -167,7 +180,7 @@ __global__ __launch_bounds__(RANK_WAVES * 64) void route_rank_kernel(const I *__
       total = mode == 0 ? s : mode == 1 ? d_total[x] : totals[x];
       before = mode == 0 ? 0 : mode == 1 ? d_before[x] : counts[(long long)blockIdx.x * E + x];
     }
-    const int s = wave_scan(total, lane);
+    const int s = wave_scan(total);
     if (lane == 63) wsum[wave] = s;
     __syncthreads();
     int pre = carry;
@@ -409,7 +422,7 @@ int plan(const I *choice, long long n, int E, int *offsets, int *place, int *ws,
   int bits = 0;
   while ((1 << bits) < E) ++bits;
   const size_t lds_rank = (size_t)RANK_WAVES * E * 2 + (size_t)E * 4;
-  const int mode = tiles == 1 ? 0 : tiles <= DIRECT_TILES && E <= DIRECT_E ? 1 : 2;
+  const int mode = tiles == 1 ? 0 : (long long)E * ((tiles + 63) / 64) <= DIRECT_LOADS ? 1 : 2;
   int *counts = ws, *totals = ws + (size_t)tiles * E;
   if (mode) route_count_kernel<I, ITEMS><<<tiles, RANK_WAVES * 64, (size_t)E * 4, st>>>(choice, n, E, counts);
   if (mode == 2) route_scan_kernel<<<cpfn_cdiv(E, 16), 1024, 0, st>>>(counts, totals, E, tiles);

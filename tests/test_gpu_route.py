@@ -55,6 +55,13 @@ def test_order_is_a_stable_sort(R, k, E, wide):
         check_plan(choices(R, k, E, seed=R + E, out_of=out_of, skew=skew, dtype=torch.int64 if wide else torch.int32), E)
 
 
+@pytest.mark.parametrize("R,k,E", [(300000, 2, 8), (300000, 2, 21), (300000, 2, 22), (524288, 1, 16), (524289, 1, 7), (600007, 1, 1), (64 * 2048, 1, 64),
+                                   (64 * 2048 + 1, 1, 32), (64 * 2048 + 1, 1, 33), (2049, 1, 65)])
+def test_order_at_the_borders_of_its_forms(R, k, E):
+    """Longer lists, whose waves take more choices, and as many loads for the sums as a workgroup makes by itself, and one more."""
+    check_plan(choices(R, k, E, seed=E, out_of=0.1), E)
+
+
 def test_order_where_nothing_is_routed_and_where_all_go_to_one():
     for R, E in ((5000, 9), (5, 9), (300000, 300)):
         check_plan(torch.full((R, 2), -1, dtype=torch.int32, device=DEV), E)
