@@ -36,6 +36,7 @@ __global__ __launch_bounds__(64) void adam_prepare_kernel(const float *__restric
   unsigned bad = 0;
   if (CLIP) {
     double s = 0.0;
+#pragma unroll 8
     for (int i = threadIdx.x; i < cl.count; i += 64) s += cl.parts[i];
 #pragma unroll
     for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d, 64);
