@@ -5,8 +5,8 @@
 // The tensors travel as a table in the kernel's arguments (nothing is copied to the device, so a captured graph replays it as it is).
 // Pass 1: a workgroup takes a share of ONE tensor and leaves one partial sum.  Sums are fp64: the squares of fp32 values cover
 // 1e-90 .. 1e77, and one lane adds thousands of them.  Pass 2: every workgroup of the scaling launch adds the partial sums itself (in
-// one fixed order: all agree, and runs repeat bit for bit), forms the factor and scales its share, from the list's end backwards: the
-// values that pass 1 read last are the ones that are still in the last-level cache.  A NaN in any gradient makes the norm NaN, an
+// one fixed order: all agree, and runs repeat bit for bit; long lists: one workgroup does, in a launch in between), forms the factor and
+// scales its share, from the list's end backwards: the values that pass 1 read last are still in the last-level cache.  A NaN in any gradient makes the norm NaN, an
 // infinity makes it infinite; the factor follows by the formula (0 for an infinite norm, NaN for NaN).
 #include "gradnorm.h"
 
@@ -19,12 +19,16 @@ constexpr int GN_THREADS = 256;
 // Elements of a workgroup before the workgroups are limited (1.4M values in 60 tensors, both launches: 4096 10.8 us, 16384 13.1) ...
 constexpr int SHARE = 4096;
 // ... to about so many in a call, one more for a tensor's last share: up to 48 long tensors stay within the 2048 that run at once, 8 on
-// each of 256 CUs (67M fp32 elements, to other tensors: 111.6 us; 2048: 114.1; 1536: 112.8; 271M bf16 to fp32: 443.6, 453.7, 459.7)
+// each of 256 CUs (67M fp32 elements 38.2 us, 5.5 TB/s, 2048: 39.8; 271M bf16 elements 86.3, 6.3 TB/s, 2048: 90.2)
 constexpr int MOST_BLOCKS = 2000;
 constexpr long long KEPT = 48ll << 20;     // elements at the end of the list that pass 1 leaves in the last-level cache (96 or 192 of its 256 MB)
-// partial sums that the scaling workgroups add themselves (above, in lists of hundreds of tensors, one launch in between does): 2000 of
-// them cost a workgroup less than that launch (33.5 -> 32.2 us where nothing is left to scale)
-constexpr int DIRECT_PARTS = MOST_BLOCKS + 256;
+// The scaling launch has many short workgroups, whose stretches of memory follow each other closely: 271M values bf16 to fp32 in 284 us,
+// 5.7 TB/s; 2000 workgroups with strides through whole tensors took 357, shares of 4096 292, of 1024 397.  In place a workgroup that finds
+// nothing to do should not be one of too many: 200M bf16 scaled, 35M fp32 left alone: 8192 157 and 4.9 us (4096: 153, 6; 16384: 161, 5).
+constexpr int SCALE_SHARE = 2048, SCALE_SHARE_IN_PLACE = 8192;
+constexpr long long MOST_SCALE_BLOCKS = 1 << 22;         // (a launch has fewer than 2^32 lanes)
+// The partial sums are added by every scaling workgroup, or, where that would be more loads than these, by one launch in between
+constexpr long long DIRECT_LOADS = 1 << 20;
 
 // What a launch's arguments hold of a list.  Pass 1 takes more tensors (301 short ones: 23.7 -> 20.4 us).
 struct Sources {
@@ -153,16 +157,16 @@ template <int P> __global__ __launch_bounds__(GN_THREADS) void grad_norm_finish_
   }
 }
 
-// Elements of a lane and step: 16 bytes on the wider side, so that the lanes of an access lie next to each other on both.  Four steps
-// in flight, from the tensor's end backwards (in place: T = U, every element is read before it is written).
+// Elements [begin, end) of a tensor (begin: a multiple of 16).  Of a lane and step: 16 bytes on the wider side, so that the lanes of an
+// access lie next to each other on both; two steps in flight, from the end (in place: T = U, every element is read before it is written).
 template <typename T, typename U>
-__device__ __forceinline__ void scale_share(const T *__restrict__ p, U *__restrict__ o, long long n, float coef, long long first, long long step) {
-  constexpr int N = cpfn_piece<T>::N < cpfn_piece<U>::N ? cpfn_piece<T>::N : cpfn_piece<U>::N, AHEAD = 4;
+__device__ __forceinline__ void scale_share(const T *__restrict__ p, U *__restrict__ o, long long begin, long long end, float coef) {
+  constexpr int N = cpfn_piece<T>::N < cpfn_piece<U>::N ? cpfn_piece<T>::N : cpfn_piece<U>::N, AHEAD = 2;
   constexpr bool narrow = N * sizeof(T) == 8;                        // 8 bytes in, 16 out
   typedef unsigned half __attribute__((ext_vector_type(2), aligned(2)));
   typedef typename cpfn_piece<T>::vec V;
   typedef typename cpfn_piece<U>::vec W;
-  const long long whole = n / N;
+  const long long whole = end / N, first = begin / N;
   const auto one = [&](const V &v, long long i) {
     float f[8];
     cpfn_unpack(v, f, (T *)nullptr);
@@ -173,30 +177,31 @@ __device__ __forceinline__ void scale_share(const T *__restrict__ p, U *__restri
   const auto get = [&](long long i) {
     V v = {};
     if (narrow) {
-      const half h = *(const half *)(p + i * N);
+      const half h = __builtin_nontemporal_load((const half *)(p + i * N));
       v.x = h.x; v.y = h.y;
     } else {
-      v = *(const V *)(p + i * N);
+      v = __builtin_nontemporal_load((const V *)(p + i * N));
     }
     return v;
   };
-  long long i = whole - 1 - first;
-  for (; i - (AHEAD - 1) * step >= 0; i -= AHEAD * step) {
+  long long i = whole - 1 - threadIdx.x;
+  for (; i - (AHEAD - 1) * GN_THREADS >= first; i -= AHEAD * GN_THREADS) {
     V v[AHEAD];
 #pragma unroll
-    for (int k = 0; k < AHEAD; ++k) v[k] = get(i - k * step);
+    for (int k = 0; k < AHEAD; ++k) v[k] = get(i - k * GN_THREADS);
 #pragma unroll
-    for (int k = 0; k < AHEAD; ++k) one(v[k], i - k * step);
+    for (int k = 0; k < AHEAD; ++k) one(v[k], i - k * GN_THREADS);
   }
-  for (; i >= 0; i -= step) one(get(i), i);
-  if (first < n - whole * N) o[whole * N + first] = cpfn_from_f32<U>(cpfn_to_f32(p[whole * N + first]) * coef);
+  for (; i >= first; i -= GN_THREADS) one(get(i), i);
+  const long long last = whole * N + threadIdx.x;                    // (the tensor's last end % N: no other workgroup has them)
+  if (last < end) o[last] = cpfn_from_f32<U>(cpfn_to_f32(p[last]) * coef);
 }
 
 // parts == 0: `part` is the norm itself.  elsewhere: the results go to other tensors (always written); in place nothing is to be done
 // where the factor is 1.
 template <int P>
 __global__ __launch_bounds__(GN_THREADS) void grad_scale_kernel(const Moves a, const double *__restrict__ part, int parts, double max_norm,
-                                                                int elsewhere, float *__restrict__ norm) {
+                                                                int elsewhere, int share, float *__restrict__ norm) {
   __shared__ double lds[GN_THREADS / 64];
   const double total = parts ? gn_total<P>(part, parts, lds) : *part;
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)total;
@@ -204,13 +209,12 @@ __global__ __launch_bounds__(GN_THREADS) void grad_scale_kernel(const Moves a, c
   if (coef == 1.f && !elsewhere) return;
   const int blk = a.block0[a.count] - 1 - (int)blockIdx.x;                       // (backwards, see above)
   const int d = list_find(a, blk);
-  const long long first = (long long)(blk - a.block0[d]) * GN_THREADS + threadIdx.x;
-  const long long step = (long long)(a.block0[d + 1] - a.block0[d]) * GN_THREADS, n = a.n[d];
-  if (a.from[d] == CPFN_F32) scale_share((const float *)a.src[d], (float *)a.dst[d], n, coef, first, step);
-  else if (a.from[d] == CPFN_BF16 && a.to[d] == CPFN_BF16) scale_share((const cpfn_bf16 *)a.src[d], (cpfn_bf16 *)a.dst[d], n, coef, first, step);
-  else if (a.from[d] == CPFN_BF16) scale_share((const cpfn_bf16 *)a.src[d], (float *)a.dst[d], n, coef, first, step);
-  else if (a.to[d] == CPFN_F16) scale_share((const cpfn_f16 *)a.src[d], (cpfn_f16 *)a.dst[d], n, coef, first, step);
-  else scale_share((const cpfn_f16 *)a.src[d], (float *)a.dst[d], n, coef, first, step);
+  const long long begin = (long long)(blk - a.block0[d]) * share, end = begin + share < a.n[d] ? begin + share : a.n[d];
+  if (a.from[d] == CPFN_F32) scale_share((const float *)a.src[d], (float *)a.dst[d], begin, end, coef);
+  else if (a.from[d] == CPFN_BF16 && a.to[d] == CPFN_BF16) scale_share((const cpfn_bf16 *)a.src[d], (cpfn_bf16 *)a.dst[d], begin, end, coef);
+  else if (a.from[d] == CPFN_BF16) scale_share((const cpfn_bf16 *)a.src[d], (float *)a.dst[d], begin, end, coef);
+  else if (a.to[d] == CPFN_F16) scale_share((const cpfn_f16 *)a.src[d], (cpfn_f16 *)a.dst[d], begin, end, coef);
+  else scale_share((const cpfn_f16 *)a.src[d], (float *)a.dst[d], begin, end, coef);
 }
 
 // workgroups of a tensor: one for each `share` elements
@@ -303,9 +307,15 @@ template <int P>
 int run(const void *const *src, void *const *dst, const long long *n, const int *from, const int *to, int count, double max_norm,
         bool clip, bool elsewhere, float *norm, double *ws, hipStream_t st) {
   const long long share = share_of(n, count);
+  int scale_share = elsewhere ? SCALE_SHARE : SCALE_SHARE_IN_PLACE;
+  long long sum = 0;
+  for (int i = 0; i < count; ++i) sum += n[i];
+  while (sum / scale_share > MOST_SCALE_BLOCKS) scale_share *= 2;
   double *part = ws + 1;
   int parts = norm_pass<P>(src, n, from, count, share, clip ? KEPT : 0, part, st);
-  if (!clip || parts > DIRECT_PARTS || parts == 0) {
+  long long scale_blocks = 0;
+  for (int i = 0; i < count; ++i) scale_blocks += (n[i] + scale_share - 1) / scale_share;
+  if (!clip || parts == 0 || parts * scale_blocks > DIRECT_LOADS) {
     grad_norm_finish_kernel<P><<<1, GN_THREADS, 0, st>>>(part, parts, ws, norm);
     norm = nullptr;                                     // (written)
     part = ws;
@@ -314,9 +324,9 @@ int run(const void *const *src, void *const *dst, const long long *n, const int 
   }
   for (int base = 0; base < count;) {
     Moves a;
-    base = fill(a, base, src, dst, n, from, to, count, share);
+    base = fill(a, base, src, dst, n, from, to, count, scale_share);
     if (a.count == 0) break;
-    grad_scale_kernel<P><<<a.block0[a.count], GN_THREADS, 0, st>>>(a, part, parts, max_norm, elsewhere ? 1 : 0, norm);
+    grad_scale_kernel<P><<<a.block0[a.count], GN_THREADS, 0, st>>>(a, part, parts, max_norm, elsewhere ? 1 : 0, scale_share, norm);
     norm = nullptr;
   }
   return cpfn_launch_status();

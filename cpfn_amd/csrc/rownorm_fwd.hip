@@ -1,8 +1,8 @@
 // Norms before and after a residual block, its gate and its residual scale in one pass over the rows (forward; the formulas are in
 // rownorm.h).  Memory bound: x, y and the gate are read once, out and normed written once; the op-by-op form moves each of the ~12
 // intermediate tensors through memory.  Measured (bf16; a copy of gigabytes reaches 4.9 TB/s, one that fits the last-level cache 8.6):
-//   131072 x 128, layer, sigmoid gate for each row    33 us   5.1 TB/s      262144 x 64, rms, no gate      21 us   6.3 TB/s
-//   65536 x 512, rms, gate for each row               64 us   5.2 TB/s      100003 x 131, rms, no gate     25 us   4.2 TB/s
+//   131072 x 128, layer, sigmoid gate for each row    32 us   5.2 TB/s      262144 x 64, rms, no gate      21 us   6.3 TB/s
+//   65536 x 512, rms, gate for each row               61 us   5.5 TB/s      100003 x 131, rms, no gate     24 us   4.4 TB/s
 //   32768 x 1024, layer, gate for 2048 rows           55 us   4.9 TB/s      fp32 20528 x 259, shared gate  18 us   4.8 TB/s
 // Ragged rows cost instructions (masks of the last piece, three more stores).
 #include "rownorm.h"
@@ -122,8 +122,10 @@ int forward(const void *x, const void *y, const void *gate, const float *weight,
             const float *next_weight, const float *next_bias, long long P, int C, long long gate_rows, int layer, int sigmoid, float eps,
             void *out, void *normed, hipStream_t st) {
   if (!gate) gate_rows = 0;
-  // four waves on each of the 1024 SIMDs run at once (87 to 129 registers; five, where they fit, measured 0 to 10 % slower)
-  const NormSplit s = norm_split(P, C, gate_rows, 4 * 1024, 1);
+  // Four waves on each of the 1024 SIMDs run at once (87 to 129 registers); twice as many are launched, and those that come second start
+  // as the first end: 65536 x 512 64 -> 61 us, fp32 65536 x 256 65 -> 60, 8192 x 4096 56 -> 53.  Four and more times as many load the
+  // parameters too often: 131072 x 128 31 to 35 (33), 100003 x 131 26 to 44 (24), 8192 x 4096 52 to 87.
+  const NormSplit s = norm_split(P, C, gate_rows, 8 * 1024, 1);
   NormFwd<T> a;
   a.x = (const T *)x; a.y = (const T *)y; a.gate = (const T *)gate;
   a.weight = weight; a.bias = bias; a.scale = scale; a.next_weight = next_weight; a.next_bias = next_bias;
