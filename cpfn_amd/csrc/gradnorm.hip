@@ -21,7 +21,9 @@ constexpr int SHARE = 4096;
 // ... to about so many in a call, one more for a tensor's last share: up to 48 long tensors stay within the 2048 that run at once, 8 on
 // each of 256 CUs (67M fp32 elements 38.2 us, 5.5 TB/s, 2048: 39.8; 271M bf16 elements 86.3, 6.3 TB/s, 2048: 90.2)
 constexpr int MOST_BLOCKS = 2000;
-constexpr long long KEPT = 48ll << 20;     // elements at the end of the list that pass 1 leaves in the last-level cache (96 or 192 of its 256 MB)
+// Bytes at the list's end that pass 1 leaves in the last-level cache (of 256 MB; the rest is not kept): 271M bf16 to fp32, both passes, none
+// 383 us, 96 MB 375, 240 MB 360
+constexpr long long KEPT = 240ll << 20;
 // The scaling launch has many short workgroups, whose stretches of memory follow each other closely: 271M values bf16 to fp32 in 284 us,
 // 5.7 TB/s; 2000 workgroups with strides through whole tensors took 357, shares of 4096 292, of 1024 397.  In place a workgroup that finds
 // nothing to do should not be one of too many: 200M bf16 scaled, 35M fp32 left alone: 8192 157 and 4.9 us (4096: 153, 6; 16384: 161, 5).
@@ -281,20 +283,21 @@ int fill(List &a, int base, const void *const *src, void *const *dst, const long
   return i;
 }
 
-// kept: so many elements from the list's end are read again soon
+// kept: so many bytes from the list's end are read again soon
 template <int P>
 int norm_pass(const void *const *src, const long long *n, const int *type, int count, long long share, long long kept, double *part, hipStream_t st) {
   int parts = 0;
-  long long streamed = -kept;                           // elements in front of those
-  for (int i = 0; i < count; ++i) streamed += n[i];
+  const auto size = [](int t) { return t == CPFN_F32 ? 4 : 2; };
+  long long streamed = -kept;                           // bytes in front of those
+  for (int i = 0; i < count; ++i) streamed += n[i] * size(type[i]);
   for (int base = 0; base < count;) {
     Sources a;
     base = fill(a, base, src, nullptr, n, type, nullptr, count, share);
     if (a.count == 0) break;
     Kept k = {0, 0};
-    for (; k.tensor < a.count && streamed >= a.n[k.tensor]; ++k.tensor) streamed -= a.n[k.tensor];
+    for (; k.tensor < a.count && streamed >= a.n[k.tensor] * size(a.from[k.tensor]); ++k.tensor) streamed -= a.n[k.tensor] * size(a.from[k.tensor]);
     if (k.tensor < a.count && streamed > 0) {
-      k.at = streamed;
+      k.at = streamed / size(a.from[k.tensor]);
       streamed = 0;
     }
     grad_norm_kernel<P><<<a.block0[a.count], GN_THREADS, 0, st>>>(a, k, part + parts);
@@ -382,6 +385,6 @@ extern "C" int cpfn_grad_sumsq(const float *g, long long n, double *parts, void 
   if (n < 0 || n > (1ll << 48) || (n > 0 && (!g || !parts)) || ((uintptr_t)parts & 7)) return CPFN_EINVAL;
   const void *src = g;
   const int type = CPFN_F32;
-  norm_pass<2>(&src, &n, &type, 1, share_of(&n, 1), n, parts, (hipStream_t)stream);
+  norm_pass<2>(&src, &n, &type, 1, share_of(&n, 1), 4 * n, parts, (hipStream_t)stream);
   return cpfn_launch_status();
 }
