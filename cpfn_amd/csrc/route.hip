@@ -408,6 +408,15 @@ int lanes_log2_for(int C, int per_lane, int most) {
   while (l < most && (per_lane << l) < C) ++l;
   return l;
 }
+// The same for the sums over a row's choices, whose lanes hold several pieces at once: fewer lanes and more steps where a last, nearly
+// empty step would leave half of the lanes idle (fp32 259 channels 40 -> 29 us, bf16 520 21 -> 18, fp32 131 12.3 -> 11.3).  The copies are
+// slower for it (fp32 131 11 -> 16 us), the adjoints as fast or slower.
+int lanes_log2_sparing(int C, int per_lane, int most) {
+  const int l = lanes_log2_for(C, per_lane, most), pieces = (C + per_lane - 1) / per_lane;
+  for (int m = l; m >= 4; --m)
+    if (((long long)(pieces + (1 << m) - 1) >> m << m) * 2 <= 3ll * pieces) return m;
+  return l;
+}
 unsigned move_blocks(long long R, int lanes_log2) {
   const long long rows = MOVE_THREADS >> lanes_log2, b = (R + rows - 1) / rows;
   return (unsigned)(b < MOVE_BLOCKS ? b : MOVE_BLOCKS);
@@ -444,7 +453,7 @@ template <typename T> int gather(const void *rows, const int *place, const int *
   return cpfn_launch_status();
 }
 template <typename T> int combine(const void *sorted, const float *weights, const int *place, long long R, int k, int C, void *out, hipStream_t st) {
-  const int l = lanes_log2_for(C, cpfn_piece<T>::N, 8);
+  const int l = lanes_log2_sparing(C, cpfn_piece<T>::N, 8);
   const unsigned b = move_blocks(R, l);
   if (k == 1) route_combine_kernel<T, 1><<<b, MOVE_THREADS, 0, st>>>((const T *)sorted, weights, place, R, k, C, l, (T *)out);
   else if (k == 2) route_combine_kernel<T, 2><<<b, MOVE_THREADS, 0, st>>>((const T *)sorted, weights, place, R, k, C, l, (T *)out);
