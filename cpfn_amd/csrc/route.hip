@@ -210,8 +210,8 @@ __global__ __launch_bounds__(RANK_WAVES * 64) void route_rank_kernel(const I *__
 // workgroups, measured 0 to 40 % slower at 131072 x 128 .. 50000 x 1024 rows: the chip holds enough groups).  A row is walked in
 // 16-byte pieces; the last piece of a row whose length is no multiple of one ENDS with the row and overlaps the piece before it: its
 // lane moves (or computes) a few elements that another lane moves too, to the same value.  Rows shorter than a piece go element by element.
-// Memory bound.  Measured (bf16): 131072 x 128 to 2 of 8: gather 20 us, combine 20, its adjoint 30 (5.0, 5.0, 5.7 TB/s); 50000 x 1024 to 4
-// of 64: 90, 90, 173 us (5.7, 5.5, 5.2); 100000 x 131 to 2 of 8, half of them left out: 25, 21, 37.
+// Memory bound.  Measured (bf16): 131072 x 128 to 2 of 8: gather 16.5 us, combine 17.4, its adjoint 30 (6.1, 5.8, 5.5 TB/s); 50000 x 1024 to 4
+// of 64: 97, 88, 175 us (5.3, 5.6, 5.1); fp32 30000 x 259 to 3 of 64: 29, 30, 56 (4.3, 4.2, 3.9).
 constexpr int MOVE_THREADS = 256;
 constexpr long long MOVE_BLOCKS = 1 << 20;
 constexpr int MOVE_MAX_C = 1 << 30;               // (a row is walked with 32-bit steps of up to 2048 elements)
@@ -335,7 +335,10 @@ __global__ __launch_bounds__(MOVE_THREADS) void route_combine_kernel(const T *__
   }
 }
 
-// LANES <= 64: the products of a row meet inside a wave
+// LANES <= 64: the products of a row meet inside a wave.  A lane has two pieces of a row in flight: against one, with twice the lanes,
+// fp32 30000 x 259 to 3 of 64 69 -> 56 us, fp32 8000 x 1100 48 -> 43, 262144 x 256 to one 77 -> 73, 131072 x 128 31.9 -> 30.2 (30000 x 512
+// to 8 of 64 105.5 -> 107.6).
+constexpr int STEPS = 2;
 template <typename T, int LANES, int KT>
 __global__ __launch_bounds__(MOVE_THREADS) void route_combine_bwd_kernel(const T *__restrict__ g, const T *__restrict__ sorted,
                                                                          const float *__restrict__ weights, const int *__restrict__ place,
@@ -360,34 +363,38 @@ __global__ __launch_bounds__(MOVE_THREADS) void route_combine_bwd_kernel(const T
         w[t] = weights ? weights[at] : 1.f;
         dot[t] = 0.f;
       }
-      for (int c = lane * N; c < C; c += LANES * N) {
-        const int here = C >= N ? piece_at<T>(c, C) : 0, twice = c - here;        // elements that the lane before has too
-        V gv, v[KT];
-        piece_get(g + (row ? r : 0) * C, here, C, gv);
-        if (d_weights) {
+      for (int c0 = lane * N; c0 < C; c0 += STEPS * LANES * N) {
+        int here[STEPS], skip[STEPS];                     // skip: first elements, which the lane before has too (all: a step behind the row)
+        V gv[STEPS], v[STEPS][KT];
 #pragma unroll
-          for (int t = 0; t < KT; ++t) piece_get(sorted + (long long)(p[t] < 0 ? 0 : p[t]) * C, here, C, v[t]);
-        }
-        float gf[N];
-        cpfn_unpack(gv, gf, (T *)nullptr);
+        for (int u = 0; u < STEPS; ++u) {
+          const int c = c0 + u * LANES * N;
+          here[u] = C >= N ? piece_at<T>(c, C) : 0;
+          skip[u] = c < C ? c - here[u] : N;
+          piece_get(g + (row ? r : 0) * C, here[u], C, gv[u]);
+          if (d_weights) {
 #pragma unroll
-        for (int t = 0; t < KT; ++t) {
-          if (d_weights) {                              // (of a choice that is not there the sum is not used)
-            float f[N];
-            cpfn_unpack(v[t], f, (T *)nullptr);
-            if (C % N && C >= N) {
-#pragma unroll
-              for (int i = 0; i < N; ++i) dot[t] = i >= twice ? fmaf(gf[i], f[i], dot[t]) : dot[t];
-            } else {
-#pragma unroll
-              for (int i = 0; i < N; ++i) dot[t] = fmaf(gf[i], f[i], dot[t]);
-            }
+            for (int t = 0; t < KT; ++t) piece_get(sorted + (long long)(p[t] < 0 ? 0 : p[t]) * C, here[u], C, v[u][t]);
           }
-          if (d_sorted && p[t] >= 0) {
-            float f[N];
+        }
 #pragma unroll
-            for (int i = 0; i < N; ++i) f[i] = w[t] * gf[i];
-            piece_put(d_sorted + (long long)p[t] * C, here, C, f);
+        for (int u = 0; u < STEPS; ++u) {
+          float gf[N];
+          cpfn_unpack(gv[u], gf, (T *)nullptr);
+#pragma unroll
+          for (int t = 0; t < KT; ++t) {
+            if (d_weights) {                              // (of a choice that is not there the sum is not used)
+              float f[N];
+              cpfn_unpack(v[u][t], f, (T *)nullptr);
+#pragma unroll
+              for (int i = 0; i < N; ++i) dot[t] = i >= skip[u] ? fmaf(gf[i], f[i], dot[t]) : dot[t];
+            }
+            if (d_sorted && p[t] >= 0 && skip[u] < N) {
+              float f[N];
+#pragma unroll
+              for (int i = 0; i < N; ++i) f[i] = w[t] * gf[i];
+              piece_put(d_sorted + (long long)p[t] * C, here[u], C, f);
+            }
           }
         }
       }
@@ -472,7 +479,7 @@ void combine_bwd_launch(const void *g, const void *sorted, const float *weights,
 template <typename T>
 int combine_bwd(const void *g, const void *sorted, const float *weights, const int *place, const int *offsets, long long R, int k, int E, int C,
                 void *d_sorted, float *d_weights, hipStream_t st) {
-  const int l = lanes_log2_for(C, cpfn_piece<T>::N, 6);
+  const int l = lanes_log2_for(C, cpfn_piece<T>::N * STEPS, 6);
   const int *end = offsets + E;
   switch (l < 2 ? 2 : l) {
     case 2: combine_bwd_launch<T, 4>(g, sorted, weights, place, end, R, k, C, d_sorted, d_weights, 2, st); break;
