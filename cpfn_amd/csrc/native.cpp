@@ -216,6 +216,9 @@ void check_capture(const Tensor &on) {
   }
 }
 
+// Does autograd record this call?  (A node costs a call of 5 us another one where nobody asks for it.)
+template <typename... A> bool recorded(const A &...tensors) { return at::GradMode::is_enabled() && (or_none(tensors).requires_grad() || ...); }
+
 Tensor contiguous(const Tensor &t) { return t.defined() ? t.contiguous() : t; }
 
 // The end of a residual block and the norm of the next one as one node.  Only the inputs are kept: out, the normalised rows and both
@@ -259,6 +262,11 @@ struct NormResidual : public torch::autograd::Function<NormResidual> {
 
 std::tuple<Maybe, Maybe> norm_residual(const Tensor &x, const Maybe &y, const Maybe &weight, const Maybe &bias, const Maybe &gate, bool sigmoid,
                                        const Maybe &scale, const Maybe &next_weight, const Maybe &next_bias, bool layer, double eps) {
+  if (!recorded(x, y, weight, bias, gate, scale, next_weight, next_bias)) {
+    const auto r = Norm{x.contiguous(), contiguous(or_none(y)), or_none(weight), or_none(bias), contiguous(or_none(gate)), or_none(scale), or_none(next_weight),
+                        or_none(next_bias), sigmoid, layer, eps}.forward();
+    return pair_of(r.first, r.second);
+  }
   const auto r = NormResidual::apply(x, y, weight, bias, gate, scale, next_weight, next_bias, sigmoid, layer, eps);
   return pair_of(y.has_value() ? r[0] : Tensor(), next_weight.has_value() ? r.back() : Tensor());
 }
@@ -471,8 +479,11 @@ PYBIND11_MODULE(_native, m) {
     const auto r = combine_rows_bwd(g, or_none(sorted), or_none(weights), Plan{offsets, place, E}, need_rows, need_weights);
     return pair_of(r.first, r.second);
   }, free_gil());
-  m.def("route_gather", [](const Tensor &rows, const Tensor &offsets, const Tensor &place, int64_t E) { return RouteGather::apply(rows, offsets, place, E); }, free_gil());
+  m.def("route_gather", [](const Tensor &rows, const Tensor &offsets, const Tensor &place, int64_t E) {
+    return recorded(rows) ? RouteGather::apply(rows, offsets, place, E) : gather_rows(rows.contiguous(), Plan{offsets, place, E});
+  }, free_gil());
   m.def("route_combine", [](const Tensor &sorted, const Maybe &weights, const Tensor &offsets, const Tensor &place, int64_t E) {
+    if (!recorded(sorted, weights)) return combine_rows(sorted.contiguous(), contiguous(or_none(weights)), Plan{offsets, place, E});
     return RouteCombine::apply(sorted, weights, offsets, place, E);
   }, free_gil());
   m.def("grad_norm", &grad_norm);
