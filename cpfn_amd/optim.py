@@ -29,8 +29,8 @@ def _norm_code(norm_type):
 
 
 def grad_norm(grads, norm_type=2.0):
-    """The norm over all values of a list of tensors (fp32, bf16 and fp16 together; any lengths) -> 0-dim fp32 tensor on their device,
-    without a host synchronisation.  norm_type 1, 2 or inf; fp64 sums in a fixed order (bit-reproducible); NaN if any value is NaN.
+    """The norm over all values of a list of tensors (fp32, bf16 and fp16 together; any lengths; dense, in any order of their dimensions,
+    on one device) -> 0-dim fp32 tensor on that device, without a host synchronisation.  norm_type 1, 2 or inf; fp64 sums in a fixed order (bit-reproducible); NaN if any value is NaN.
     An empty list: a zero on the CPU."""
     return _native_call("grad_norm", _list_of(grads), _norm_code(norm_type), None, None)
 
