@@ -352,3 +352,20 @@ def test_what_is_clipped_counts_as_changed():
         x = torch.randn(100, device=DEV)
         norm = optim.clip_grads_([x], 0.5)
     assert abs(float(x.double().norm()) - 0.5) < 1e-5 and abs(float(norm)) > 0.5
+
+
+@pytest.mark.parametrize("p", [2.0, 1.0, INF])
+def test_the_smallest_and_the_largest_bound_and_out_in_place(p):
+    from cpfn_amd import optim
+    for kind in ("mixed", "many"):
+        keep = lists(kind)
+        for bound in (0.0, INF):
+            g = [t.clone() for t in keep]
+            norm = optim.clip_grads_(g, bound, norm_type=p)
+            assert abs(float(norm) - exact_norm(keep, p)) <= 2 * U * exact_norm(keep, p)          # (its one rounding, and 1e-16s)
+            for a, b in zip(g, keep):
+                assert torch.equal(a, b if bound else torch.zeros_like(b))
+        ours, theirs = [t.clone() for t in keep], [t.clone() for t in keep]
+        optim.clip_grads_(ours, 0.1, norm_type=p, out=ours)
+        optim.clip_grads_(theirs, 0.1, norm_type=p)
+        assert all(torch.equal(a, b) for a, b in zip(ours, theirs))

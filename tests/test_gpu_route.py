@@ -285,3 +285,27 @@ def test_places_that_no_plan_left_are_choices_that_are_not_there(C, dtype):
         assert_within(out, (Approx(picked) * Approx(w.detach().double()[:, :, None])).sum(1).view(R, C), "out")
         assert_within(d_w, (Approx(picked) * Approx(g.double()[:, None, :])).sum(2).view(R, k), "d_weights")
         assert not bool(d_w[~there].any())
+
+
+def test_only_one_of_rows_and_weights_is_differentiated_and_a_graph_is_walked_twice():
+    from cpfn_amd import autograd_ops, ops
+    c, rows, mid, w, d_sorted, d_out = problem(90, 3, 5, 44, torch.float32, 0.2)
+    plan = ops.route_plan(c, 5)
+    both = torch.autograd.grad(autograd_ops.route_combine(mid, w, plan), [mid, w], [d_out])
+    only_w = torch.autograd.grad(autograd_ops.route_combine(mid.detach(), w, plan), [w], [d_out])
+    only_mid = torch.autograd.grad(autograd_ops.route_combine(mid, w.detach(), plan), [mid], [d_out])
+    assert torch.equal(only_w[0], both[1]) and torch.equal(only_mid[0], both[0])
+    wt = w.detach().t().contiguous().t().requires_grad_()               # (weights in another order of memory)
+    assert not wt.is_contiguous()
+    turned = torch.autograd.grad(autograd_ops.route_combine(mid, wt, plan), [mid, wt], [d_out])
+    assert all(torch.equal(a, b) for a, b in zip(turned, both))
+    out = autograd_ops.route_combine(mid, w, plan)
+    for _ in range(2):
+        again = torch.autograd.grad(out, [mid, w], [d_out], retain_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(again, both))
+    with torch.no_grad():
+        assert torch.equal(autograd_ops.route_combine(mid, w, plan), out)
+        assert torch.equal(autograd_ops.route_gather(rows, plan), autograd_ops.route_gather(rows.detach(), plan))
+    plan.place[0, 0] = -1                                               # (a plan that changed under a recorded call)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(out, [mid], [d_out])

@@ -344,3 +344,23 @@ def test_a_long_tensor_whose_offsets_pass_32_bits():
     out, normed = ops.norm_residual_fwd(x, y, weight=w, next_weight=w)
     a, b = ops.norm_residual_fwd(tail[0].contiguous(), tail[1].contiguous(), weight=w, next_weight=w)
     assert torch.equal(out[-4:], a) and torch.equal(normed[-4:], b) and not bool(out[:-4].any())
+
+
+def test_a_graph_is_walked_twice_and_nothing_is_recorded_without_gradients():
+    from cpfn_amd import autograd_ops
+    t, d_out, d_normed = inputs(50, 88, torch.bfloat16, 5, seed=9)
+    out, normed = call(t, "rms", "sigmoid")
+    leaves = [v for v in t.values() if v is not None]
+    first = torch.autograd.grad([out, normed], leaves, [d_out, d_normed], retain_graph=True)
+    again = torch.autograd.grad([out, normed], leaves, [d_out, d_normed])
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+    detached = {n: None if v is None else v.detach() for n, v in t.items()}
+    for grad_mode, u in ((False, t), (True, detached)):
+        with torch.set_grad_enabled(grad_mode):
+            o, n = call(u, "rms", "sigmoid")
+        assert not o.requires_grad and not n.requires_grad and torch.equal(o, out) and torch.equal(n, normed)
+    with torch.inference_mode():
+        assert torch.equal(call(t, "rms", "sigmoid")[1], normed)
+        turned = t["x"].detach().t().contiguous().t()
+        assert not turned.is_contiguous()
+        assert torch.equal(autograd_ops.row_norm(turned, t["next_weight"]), autograd_ops.row_norm(t["x"], t["next_weight"]))
