@@ -369,3 +369,20 @@ def test_the_smallest_and_the_largest_bound_and_out_in_place(p):
         optim.clip_grads_(ours, 0.1, norm_type=p, out=ours)
         optim.clip_grads_(theirs, 0.1, norm_type=p)
         assert all(torch.equal(a, b) for a, b in zip(ours, theirs))
+
+
+def test_adam_on_the_clipped_gradients_of_a_long_bucket():
+    """As many partial sums as a call leaves, and their sum by the one wave that prepares the step."""
+    from cpfn_amd import lib, training
+    from cpfn_amd.optim import FlatAdam
+    torch.manual_seed(1)
+    m = torch.nn.Linear(4001, 3001).to(DEV)
+    bucket = training.FlatGradBucket(m)
+    opt = FlatAdam(bucket, lr=1e-2)
+    assert lib.lib().cpfn_grad_sumsq_blocks(bucket.flat.numel()) >= 1999
+    bucket.flat.normal_()
+    flat = bucket.flat.clone()
+    state = [t.clone() for t in (opt.flat_p, opt.exp_avg, opt.exp_avg_sq)]
+    opt.step(max_grad_norm=0.5)
+    assert torch.equal(bucket.flat, flat)
+    assert check_adam_step(opt, state, flat, 1, 0.5, 1e-2) < 1e-3
