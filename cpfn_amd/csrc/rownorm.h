@@ -4,7 +4,7 @@
 //   u = n(y; weight, bias)  (y itself without a weight),   a = gate | sigmoid(gate) | 1
 //   out = x + scale a u   (x itself without y),            normed = n(out; next_weight, next_bias)
 //
-// A row is held by L lanes, eight channels each, from its one load to its one store: L = 8 .. 64 lanes inside a wave (row sums by
+// A row is held by L lanes, W = 8 channels each (or 16), from its one load to its one store: L = 8 .. 64 lanes inside a wave (row sums by
 // DPP and lane swaps), 128 .. 512 lanes = several waves (sums through LDS, one barrier each).  All arithmetic is fp32.
 //
 // Loads run one row set ahead of the arithmetic, and no branch stands around a load or a store: then the compiler can count what is
@@ -25,12 +25,12 @@ enum NormMode { WHOLE, RAGGED, EACH };
 enum NormForm { ANY, BLOCK, BLOCK_OWN, FRONT };
 
 // (rows of several waves have a workgroup of their own: its barriers then wait for nobody else)
-template <typename T, int L> struct NormShape {
-  enum { THREADS = L <= 64 ? 256 : L, ROWS = THREADS / L, VN = cpfn_piece<T>::N, NP = 8 / VN };
+template <typename T, int L, int W> struct NormShape {
+  enum { THREADS = L <= 64 ? 256 : L, ROWS = THREADS / L, VN = cpfn_piece<T>::N, NP = W / VN };
 };
 
-// channel of element i (0..7) of lane `lane` of its row
-template <typename T, int L> __device__ __forceinline__ int norm_col(int lane, int i) {
+// channel of element i (0..W-1) of lane `lane` of its row
+template <typename T, int L, int W> __device__ __forceinline__ int norm_col(int lane, int i) {
   constexpr int VN = cpfn_piece<T>::N;
   return ((i / VN) * L + lane) * VN + i % VN;
 }
@@ -38,11 +38,11 @@ template <typename T, int L> __device__ __forceinline__ int norm_col(int lane, i
 typedef unsigned cpfn_u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned cpfn_u32x2 __attribute__((ext_vector_type(2)));
 
-template <typename T, int L> struct RowRaw { cpfn_u32x4 p[8 / cpfn_piece<T>::N]; };
+template <typename T, int L, int W> struct RowRaw { cpfn_u32x4 p[W / cpfn_piece<T>::N]; };
 
-template <typename T, int L> __device__ __forceinline__ void row_unpack(const RowRaw<T, L> &raw, float *f) {
+template <typename T, int L, int W> __device__ __forceinline__ void row_unpack(const RowRaw<T, L, W> &raw, float *f) {
 #pragma unroll
-  for (int q = 0; q < 8 / cpfn_piece<T>::N; ++q) {
+  for (int q = 0; q < W / cpfn_piece<T>::N; ++q) {
     const unsigned u[4] = {raw.p[q].x, raw.p[q].y, raw.p[q].z, raw.p[q].w};
     float *o = f + q * cpfn_piece<T>::N;
 #pragma unroll
@@ -68,8 +68,8 @@ template <typename T> __device__ __forceinline__ cpfn_u32x4 piece_pack(const flo
 
 // Where a lane finds its pieces in a chunk of rows [row0, row1) of tensors [P, C].  Offsets are bytes from the chunk's start.
 constexpr unsigned OUTSIDE = 0xC0000000u;            // (chunks stay below 2^30 bytes: every step from here is outside too)
-template <typename T, int L, NormMode MODE> struct RowChunk {
-  static constexpr int VN = cpfn_piece<T>::N, NP = 8 / VN;
+template <typename T, int L, int W, NormMode MODE> struct RowChunk {
+  static constexpr int VN = cpfn_piece<T>::N, NP = W / VN;
   int lane, C;
   long long row0, row1, P;
   unsigned off[NP];                  // first row set
@@ -136,12 +136,12 @@ template <typename T, int L, NormMode MODE> struct RowChunk {
     }
   }
   // STREAM: the values are not kept in the caches (the last reader of whole rows; ragged rows share their cache lines)
-  template <bool STREAM = false> __device__ __forceinline__ void load(RowRaw<T, L> &raw, __amdgpu_buffer_rsrc_t rs, const unsigned *o) const {
+  template <bool STREAM = false> __device__ __forceinline__ void load(RowRaw<T, L, W> &raw, __amdgpu_buffer_rsrc_t rs, const unsigned *o) const {
 #pragma unroll
     for (int q = 0; q < NP; ++q) raw.p[q] = __builtin_amdgcn_raw_buffer_load_b128(rs, o[q], 0, STREAM && MODE == WHOLE ? 2 : 0);
   }
   // what was loaded -> the row's values, zero behind its end
-  __device__ __forceinline__ void settle(RowRaw<T, L> &raw, const unsigned *shift) const {
+  __device__ __forceinline__ void settle(RowRaw<T, L, W> &raw, const unsigned *shift) const {
     if (MODE != RAGGED) return;
 #pragma unroll
     for (int q = 0; q < NP; ++q) {
@@ -179,23 +179,23 @@ template <typename T, int L, NormMode MODE> struct RowChunk {
 };
 
 // EACH: every element an access of its own
-template <typename T, int L> __device__ __forceinline__ void each_load(RowRaw<T, L> &raw, const T *p, long long r, int lane, int C, bool there) {
-  float f[8];
+template <typename T, int L, int W> __device__ __forceinline__ void each_load(RowRaw<T, L, W> &raw, const T *p, long long r, int lane, int C, bool there) {
+  float f[W];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = p && there && norm_col<T, L>(lane, i) < C ? cpfn_to_f32(p[r * C + norm_col<T, L>(lane, i)]) : 0.f;
+  for (int i = 0; i < W; ++i) f[i] = p && there && norm_col<T, L, W>(lane, i) < C ? cpfn_to_f32(p[r * C + norm_col<T, L, W>(lane, i)]) : 0.f;
 #pragma unroll
-  for (int q = 0; q < 8 / cpfn_piece<T>::N; ++q) raw.p[q] = piece_pack<T>(f + q * cpfn_piece<T>::N);
+  for (int q = 0; q < W / cpfn_piece<T>::N; ++q) raw.p[q] = piece_pack<T>(f + q * cpfn_piece<T>::N);
 }
-template <typename T, int L> __device__ __forceinline__ void each_store(T *p, long long r, int lane, int C, bool there, const float *f) {
+template <typename T, int L, int W> __device__ __forceinline__ void each_store(T *p, long long r, int lane, int C, bool there, const float *f) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (p && there && norm_col<T, L>(lane, i) < C) p[r * C + norm_col<T, L>(lane, i)] = cpfn_from_f32<T>(f[i]);
+  for (int i = 0; i < W; ++i)
+    if (p && there && norm_col<T, L, W>(lane, i) < C) p[r * C + norm_col<T, L, W>(lane, i)] = cpfn_from_f32<T>(f[i]);
 }
 
 // one row of a tensor by itself (a gate that a group of rows shares), element by element where its end is not whole
-template <typename T, int L> __device__ __forceinline__ void single_load(RowRaw<T, L> &raw, const T *__restrict__ row, int lane, int C) {
+template <typename T, int L, int W> __device__ __forceinline__ void single_load(RowRaw<T, L, W> &raw, const T *__restrict__ row, int lane, int C) {
 #pragma unroll
-  for (int q = 0; q < 8 / cpfn_piece<T>::N; ++q) {
+  for (int q = 0; q < W / cpfn_piece<T>::N; ++q) {
     const auto v = cpfn_load_piece(row, (q * L + lane) * cpfn_piece<T>::N, C);
     raw.p[q] = cpfn_u32x4{cpfn_word(v.x), cpfn_word(v.y), cpfn_word(v.z), cpfn_word(v.w)};
   }
@@ -204,27 +204,27 @@ template <typename T, int L> __device__ __forceinline__ void single_load(RowRaw<
 // A value has arrived where this stands.  In front of a loop: without it every step of the loop waits for whatever was requested last,
 // which is the next step's rows.  At the end of a step, on the next step's rows: there the number of stores behind them is known (where
 // the loop begins it is not: with or without a step before it), and only the loads are waited for.
-__device__ __forceinline__ void arrived(float *f) {
+template <int W> __device__ __forceinline__ void arrived(float (&f)[W]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(f[i]));
+  for (int i = 0; i < W; ++i) asm volatile("" : "+v"(f[i]));
 }
 
-template <typename T, int L> __device__ __forceinline__ void arrived(RowRaw<T, L> &raw) {
+template <typename T, int L, int W> __device__ __forceinline__ void arrived(RowRaw<T, L, W> &raw) {
 #pragma unroll
-  for (int q = 0; q < 8 / cpfn_piece<T>::N; ++q) asm volatile("" : "+v"(raw.p[q]));
+  for (int q = 0; q < W / cpfn_piece<T>::N; ++q) asm volatile("" : "+v"(raw.p[q]));
 }
 
 // a parameter vector (fp32, any 4-byte alignment: parameters live inside a flat buffer), `fill` where there is none.  16 bytes a load:
 // word by word the five vectors cost a launch over 131072 x 128 rows 15 of its 50 us
-template <typename T, int L, bool PARTIAL> __device__ __forceinline__ void param_load(float *f, const float *__restrict__ p, int lane, int C, float fill) {
+template <typename T, int L, int W, bool PARTIAL> __device__ __forceinline__ void param_load(float *f, const float *__restrict__ p, int lane, int C, float fill) {
   if (!p) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = fill;
+    for (int i = 0; i < W; ++i) f[i] = fill;
     return;
   }
 #pragma unroll
-  for (int i = 0; i < 8; i += 4) {
-    const int c = norm_col<T, L>(lane, i);
+  for (int i = 0; i < W; i += 4) {
+    const int c = norm_col<T, L, W>(lane, i);
     cpfn_piece<float>::vec v = {};
     if (c + 4 <= C) {
       v = *(const cpfn_piece<float>::vec *)(p + c);
@@ -238,14 +238,14 @@ template <typename T, int L, bool PARTIAL> __device__ __forceinline__ void param
 }
 
 // scale weight and scale bias of a lane's channels: out = x + a (hat scale weight + scale bias)
-template <typename T, int L, bool PARTIAL>
+template <typename T, int L, int W, bool PARTIAL>
 __device__ __forceinline__ void block_params(float *sw, float *sb, const float *weight, const float *bias, const float *scale, int lane, int C) {
-  float s[8];
-  param_load<T, L, PARTIAL>(sw, weight, lane, C, 1.f);
-  param_load<T, L, PARTIAL>(sb, bias, lane, C, 0.f);
-  param_load<T, L, PARTIAL>(s, scale, lane, C, 1.f);
+  float s[W];
+  param_load<T, L, W, PARTIAL>(sw, weight, lane, C, 1.f);
+  param_load<T, L, W, PARTIAL>(sb, bias, lane, C, 0.f);
+  param_load<T, L, W, PARTIAL>(s, scale, lane, C, 1.f);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) { sw[i] *= s[i]; sb[i] *= s[i]; }
+  for (int i = 0; i < W; ++i) { sw[i] *= s[i]; sb[i] *= s[i]; }
 }
 
 // What was read is in registers of its own from here on: the next rows are requested into those that it was loaded into (without this
@@ -260,9 +260,9 @@ template <int L> __device__ __forceinline__ void row_sum2(float &a, float &b, fl
   a = cpfn_lanes_sum<LW>(a);
   b = cpfn_lanes_sum<LW>(b);
   if (L > 64) {
-    constexpr int W = L / 64;
+    constexpr int WAVES = L / 64;
     const int wave = threadIdx.x >> 6;
-    float2 *s = slots + turn * W;
+    float2 *s = slots + turn * WAVES;
     turn ^= 1;
     if ((threadIdx.x & 63) == 0) s[wave] = make_float2(a, b);
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
@@ -270,7 +270,7 @@ template <int L> __device__ __forceinline__ void row_sum2(float &a, float &b, fl
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
     a = 0.f; b = 0.f;
 #pragma unroll
-    for (int i = 0; i < W; ++i) {
+    for (int i = 0; i < WAVES; ++i) {
       const float2 v = s[i];
       a += v.x; b += v.y;
     }
@@ -285,22 +285,22 @@ template <int L> __device__ __forceinline__ float row_sum(float a, float2 *slots
 // v -> its normalised form (v - mu) r; returns r.  Two passes over the registers for `layer` (mean, then centred squares): no
 // cancellation.  Channels behind C hold zero and stay out of the centred squares; a row slot without a row is called with a positive
 // eps, so that its zeros stay zeros.
-template <typename T, int L, NormMode MODE>
+template <typename T, int L, int W, NormMode MODE>
 __device__ __forceinline__ float row_normalise(float *v, int lane, int C, float inv_c, bool layer, float eps, float2 *slots, int &turn) {
   if (layer) {
     float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s += v[i];
+    for (int i = 0; i < W; ++i) s += v[i];
     const float mu = row_sum<L>(s, slots, turn) * inv_c;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = norm_col<T, L>(lane, MODE == WHOLE ? i & -cpfn_piece<T>::N : i) < C ? v[i] - mu : 0.f;
+    for (int i = 0; i < W; ++i) v[i] = norm_col<T, L, W>(lane, MODE == WHOLE ? i & -cpfn_piece<T>::N : i) < C ? v[i] - mu : 0.f;
   }
   float q = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) q = fmaf(v[i], v[i], q);
+  for (int i = 0; i < W; ++i) q = fmaf(v[i], v[i], q);
   const float r = rsqrtf(fmaf(row_sum<L>(q, slots, turn), inv_c, eps));
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] *= r;
+  for (int i = 0; i < W; ++i) v[i] *= r;
   return r;
 }
 
@@ -310,36 +310,41 @@ template <typename T> __device__ __forceinline__ float norm_sigmoid(float v) {
   return __builtin_amdgcn_rcpf(1.f + (sizeof(T) == 4 ? expf(-v) : __builtin_amdgcn_exp2f(v * -1.44269504f)));
 }
 
-template <typename T> __device__ __forceinline__ void gate_act(float *g, int sigmoid) {
+template <typename T, int W> __device__ __forceinline__ void gate_act(float (&g)[W], int sigmoid) {
   if (!sigmoid) return;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) g[i] = norm_sigmoid<T>(g[i]);
+  for (int i = 0; i < W; ++i) g[i] = norm_sigmoid<T>(g[i]);
 }
 // the gate that all rows of a group share, behind its activation (one without such a gate)
-template <typename T, int L> __device__ __forceinline__ void shared_gate(float *g, const T *row, int lane, int C, int sigmoid) {
+template <typename T, int L, int W> __device__ __forceinline__ void shared_gate(float (&g)[W], const T *row, int lane, int C, int sigmoid) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) g[i] = 1.f;
+  for (int i = 0; i < W; ++i) g[i] = 1.f;
   if (!row) return;
-  RowRaw<T, L> raw;
-  single_load<T, L>(raw, row, lane, C);
+  RowRaw<T, L, W> raw;
+  single_load<T, L, W>(raw, row, lane, C);
   row_unpack(raw, g);
-  gate_act<T>(g, sigmoid);
+  gate_act<T, W>(g, sigmoid);
   arrived(g);
 }
 
 // ---------------------------------------------------------------- how the rows are split over workgroups (host)
-// the number of lanes for a row of C channels
-static inline int norm_lanes(int C) {
+// Channels of a lane: 8, and 16 where that keeps a whole row of 16-bit values in one wave (32768 x 1024, layer, shared gate: forward 56 ->
+// 51 us, backward 101 -> 94; norm in front 24 -> 22, 52 -> 48; 50000 x 520 54 -> 45, 110 -> 90).  Elsewhere 16 are slower, for their
+// registers (131072 x 128 backward 56 -> 64, 16384 x 2048 94 -> 107), for idle lanes (fp32 20528 x 259 36 -> 47) or for the masks of
+// ragged rows (40000 x 601 forward 45 -> 47).
+static inline int norm_width(int C, size_t element) { return element == 2 && C % 8 == 0 && C > 512 && C <= 1024 ? 16 : 8; }
+// lanes for a row of C channels
+static inline int norm_lanes(int C, int W) {
   int L = 8;
-  while (L * 8 < C) L *= 2;
+  while (L * W < C) L *= 2;
   return L;
 }
 // Rows are cut at the borders of gate groups (rows that share a gate row; one group without such a gate), then into chunks: a
 // workgroup has one chunk of a group (blocks_per_group > 1) or whole groups.
 struct NormSplit { long long groups, rows_per_gate, chunk; int nblk, blocks_per_group, groups_per_block; };
 // waves: as many as are resident together; sets: row sets that a workgroup should have at least
-static inline NormSplit norm_split(long long P, int C, long long gate_rows, long long waves, int sets_at_least) {
-  const int L = norm_lanes(C), threads = L <= 64 ? 256 : L, rows = threads / L;
+static inline NormSplit norm_split(long long P, int C, int W, long long gate_rows, long long waves, int sets_at_least) {
+  const int L = norm_lanes(C, W), threads = L <= 64 ? 256 : L, rows = threads / L;
   const bool shared = gate_rows > 0 && gate_rows < P;
   NormSplit s;
   s.groups = shared ? gate_rows : 1;

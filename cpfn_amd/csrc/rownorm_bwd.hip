@@ -9,15 +9,16 @@
 // [..] for layer norms only.  The parameters' gradients are column sums of four products:
 //   S1 = sum D a hat2,  S2 = sum D a,  S3 = sum d_normed hat1,  S4 = sum d_normed
 //   d_weight = scale S1,  d_bias = scale S2,  d_scale = weight S1 + bias S2,  d_next_weight = S3,  d_next_bias = S4
-// (hat2 = y without a post-norm).  A lane owns its eight channels for every row of its workgroup, so a column sum is a register until
+// (hat2 = y without a post-norm).  A lane owns its channels for every row of its workgroup, so a column sum is a register until
 // the workgroup ends; the workgroups' sums are added by a second small launch in a fixed order: no atomics, bit-reproducible.
 // d_gate of rows that share one: the factor of the sigmoid is the same for all of them and comes after the sum.
 //
-// Memory bound up to 512 channels; above, the barriers of the row sums (up to six a row) and the workgroups' sums (16 MB) show.
+// Memory bound up to 512 channels; above, registers (1024: one wave on a SIMD), the barriers of the row sums (up to six a row) and the
+// workgroups' sums (16 MB) show.
 // Measured (bf16, both launches):
 //   131072 x 128, layer, sigmoid gate for each row    57 us   4.7 TB/s      262144 x 64, rms, no gate      45 us   4.5 TB/s
 //   65536 x 512, rms, gate for each row              111 us   4.8 TB/s      100003 x 131, rms, no gate     51 us   3.1 TB/s
-//   32768 x 1024, layer, gate for 2048 rows          100 us   4.0 TB/s      fp32 20528 x 259, shared gate  36 us   3.5 TB/s
+//   32768 x 1024, layer, gate for 2048 rows           94 us   4.3 TB/s      fp32 20528 x 259, shared gate  36 us   3.5 TB/s
 // The kernels of the whole block without branches, against the one with them: 32768 x 1024 110 -> 100 us, 8192 x 4096 134 -> 109,
 // fp32 20528 x 259 44 -> 36; of the norm in front: 32768 x 1024 57 -> 52.
 #include "rownorm.h"
@@ -40,46 +41,47 @@ template <typename T> struct NormBwd {
 };
 
 // sum over the row slots of a workgroup, element by element; lane `i` order of the registers -> dst[channel]
-template <typename T, int L, typename F> __device__ __forceinline__ void slots_sum(const float *v, float *lds, int C, F store) {
-  constexpr int THREADS = NormShape<T, L>::THREADS, ROWS = NormShape<T, L>::ROWS;
+template <typename T, int L, int W, typename F> __device__ __forceinline__ void slots_sum(const float *v, float *lds, int C, F store) {
+  constexpr int THREADS = NormShape<T, L, W>::THREADS, ROWS = NormShape<T, L, W>::ROWS;
   const int lane = threadIdx.x & (L - 1), slot = threadIdx.x / L;
   if (ROWS == 1) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int c = norm_col<T, L>(lane, i);
+    for (int i = 0; i < W; ++i) {
+      const int c = norm_col<T, L, W>(lane, i);
       if (c < C) store(c, v[i]);
     }
     return;
   }
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 8; ++i) lds[slot * (L * 8) + i * L + lane] = v[i];
+  for (int i = 0; i < W; ++i) lds[slot * (L * W) + i * L + lane] = v[i];
   __syncthreads();
-  for (int e = threadIdx.x; e < L * 8; e += THREADS) {
+  for (int e = threadIdx.x; e < L * W; e += THREADS) {
     float t = 0.f;
 #pragma unroll
-    for (int q = 0; q < ROWS; ++q) t += lds[q * (L * 8) + e];
-    const int c = norm_col<T, L>(e & (L - 1), e / L);
+    for (int q = 0; q < ROWS; ++q) t += lds[q * (L * W) + e];
+    const int c = norm_col<T, L, W>(e & (L - 1), e / L);
     if (c < C) store(c, t);
   }
 }
 
-template <typename T, int L, NormMode MODE, NormForm FORM>
-__global__ __launch_bounds__((NormShape<T, L>::THREADS)) void norm_residual_bwd_kernel(const NormBwd<T> a) {
-  constexpr int ROWS = NormShape<T, L>::ROWS, THREADS = NormShape<T, L>::THREADS, NP = NormShape<T, L>::NP;
+template <typename T, int L, int W, NormMode MODE, NormForm FORM>
+__global__ __launch_bounds__((NormShape<T, L, W>::THREADS)) void norm_residual_bwd_kernel(const NormBwd<T> a) {
+  constexpr int ROWS = NormShape<T, L, W>::ROWS, THREADS = NormShape<T, L, W>::THREADS, NP = NormShape<T, L, W>::NP;
   __shared__ float2 slots[16];
-  __shared__ float comb[ROWS > 1 ? THREADS * 8 : 1];
+  __shared__ float comb[ROWS > 1 ? THREADS * W : 1];
   int turn = 0;
   const int lane = threadIdx.x & (L - 1), slot = threadIdx.x / L, C = a.C;
   const float inv_c = 1.f / (float)C;
-  const bool layer = a.layer != 0, post = FORM != ANY || a.weight != nullptr, has_y = FORM == FRONT ? false : FORM != ANY || a.y != nullptr, next = FORM != ANY || a.d_normed != nullptr;
+  const bool layer = a.layer != 0, post = FORM != ANY || a.weight != nullptr, next = FORM != ANY || a.d_normed != nullptr;
+  const bool has_y = FORM == FRONT ? false : FORM != ANY || a.y != nullptr;
   constexpr bool may_y = FORM != FRONT, may_own = FORM == ANY || FORM == BLOCK_OWN;       // rows that may be there
   const bool own = FORM == ANY ? a.gate != nullptr && !a.shared_gate : FORM == BLOCK_OWN;
-  float sw[8], sb[8], nw[8], s1[8], s2[8], s3[8], s4[8], sg[8];
-  block_params<T, L, MODE != WHOLE>(sw, sb, a.weight, a.bias, a.scale, lane, C);
-  param_load<T, L, MODE != WHOLE>(nw, a.next_weight, lane, C, 1.f);
+  float sw[W], sb[W], nw[W], s1[W], s2[W], s3[W], s4[W], sg[W];
+  block_params<T, L, W, MODE != WHOLE>(sw, sb, a.weight, a.bias, a.scale, lane, C);
+  param_load<T, L, W, MODE != WHOLE>(nw, a.next_weight, lane, C, 1.f);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) { s1[i] = s2[i] = s3[i] = s4[i] = sg[i] = 0.f; }
+  for (int i = 0; i < W; ++i) { s1[i] = s2[i] = s3[i] = s4[i] = sg[i] = 0.f; }
   const long long g0 = a.blocks_per_group > 1 ? blockIdx.x / a.blocks_per_group : (long long)blockIdx.x * a.groups_per_block;
   long long g1 = a.blocks_per_group > 1 ? g0 + 1 : g0 + a.groups_per_block;
   if (g1 > a.groups) g1 = a.groups;
@@ -91,13 +93,13 @@ __global__ __launch_bounds__((NormShape<T, L>::THREADS)) void norm_residual_bwd_
       row0 += (long long)(blockIdx.x % a.blocks_per_group) * a.chunk;
       if (row0 + a.chunk < row1) row1 = row0 + a.chunk;
     }
-    RowChunk<T, L, MODE> ch;
+    RowChunk<T, L, W, MODE> ch;
     ch.begin(row0, row1, a.P, C, lane, slot);
     const T *own_gate = own ? a.gate : nullptr;
     T *d_own_gate = own ? a.d_gate : nullptr;
     const auto bx = ch.source(next ? a.x : nullptr), by = ch.source(a.y), bg = ch.source(own_gate), bd = ch.source(a.d_out), bn = ch.source(a.d_normed);
     const auto tx = ch.target(a.d_x), ty = ch.target(a.d_y), tg = ch.target(d_own_gate);
-    RowRaw<T, L> rx, ry, rg, rd, rn;
+    RowRaw<T, L, W> rx, ry, rg, rd, rn;
     unsigned o[NP], sh[NP];
     const auto request = [&](unsigned step, long long r) {
       if (MODE == EACH) {
@@ -121,8 +123,8 @@ __global__ __launch_bounds__((NormShape<T, L>::THREADS)) void norm_residual_bwd_
       if (may_own) arrived(rg);
       arrived(rd); arrived(rn);
     };
-    float gs[8];
-    shared_gate<T, L>(gs, a.shared_gate ? a.gate + g * C : nullptr, lane, C, a.sigmoid);
+    float gs[W];
+    shared_gate<T, L, W>(gs, a.shared_gate ? a.gate + g * C : nullptr, lane, C, a.sigmoid);
     arrived(sw); arrived(sb); arrived(nw);
     request(0, row0 + slot);
     requested();
@@ -131,7 +133,7 @@ __global__ __launch_bounds__((NormShape<T, L>::THREADS)) void norm_residual_bwd_
       const long long r = base + slot;
       const bool there = r < row1;
       const float eps = there ? a.eps : 1.f;
-      float h[8], hat2[8], ga[8], D[8], dn[8], r2 = 0.f;
+      float h[W], hat2[W], ga[W], D[W], dn[W], r2 = 0.f;
       ch.settle(rx, sh); ch.settle(rd, sh); ch.settle(rn, sh);
       row_unpack(rx, h);
       row_unpack(rd, D);
@@ -146,18 +148,18 @@ __global__ __launch_bounds__((NormShape<T, L>::THREADS)) void norm_residual_bwd_
       }
       unpacked();
       request(step + set_bytes, r + ROWS);
-      if (has_y && post) r2 = row_normalise<T, L, MODE>(hat2, lane, C, inv_c, layer, eps, slots, turn);
-      if (own) gate_act<T>(ga, a.sigmoid);
+      if (has_y && post) r2 = row_normalise<T, L, W, MODE>(hat2, lane, C, inv_c, layer, eps, slots, turn);
+      if (own) gate_act<T, W>(ga, a.sigmoid);
       const auto gate = [&](int i) { return own ? ga[i] : gs[i]; };
       if (next) {
         if (has_y) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) h[i] = fmaf(gate(i), fmaf(hat2[i], sw[i], sb[i]), h[i]);
+          for (int i = 0; i < W; ++i) h[i] = fmaf(gate(i), fmaf(hat2[i], sw[i], sb[i]), h[i]);
         }
-        const float r1 = row_normalise<T, L, MODE>(h, lane, C, inv_c, layer, eps, slots, turn);
+        const float r1 = row_normalise<T, L, W, MODE>(h, lane, C, inv_c, layer, eps, slots, turn);
         float m1 = 0.f, m2 = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < W; ++i) {
           s3[i] = fmaf(dn[i], h[i], s3[i]);
           s4[i] += dn[i];
           dn[i] *= nw[i];
@@ -168,15 +170,15 @@ __global__ __launch_bounds__((NormShape<T, L>::THREADS)) void norm_residual_bwd_
         m1 = layer ? m1 * inv_c : 0.f;
         m2 *= inv_c;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) D[i] = fmaf(r1, dn[i] - m1 - h[i] * m2, D[i]);
+        for (int i = 0; i < W; ++i) D[i] = fmaf(r1, dn[i] - m1 - h[i] * m2, D[i]);
       }
-      if (MODE == EACH) each_store<T, L>(a.d_x, r, lane, C, there, D);
+      if (MODE == EACH) each_store<T, L, W>(a.d_x, r, lane, C, there, D);
       else ch.store(tx, step, D);
-      float e[8], dg[8];
+      float e[W], dg[W];
       if (has_y) {
         if (a.d_gate) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
+          for (int i = 0; i < W; ++i) {
             dg[i] = D[i] * fmaf(hat2[i], sw[i], sb[i]);
             if (own) dg[i] *= a.sigmoid ? ga[i] * (1.f - ga[i]) : 1.f;
             else sg[i] += dg[i];
@@ -184,7 +186,7 @@ __global__ __launch_bounds__((NormShape<T, L>::THREADS)) void norm_residual_bwd_
         }
         float m1 = 0.f, m2 = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < W; ++i) {
           const float da = D[i] * gate(i);
           s1[i] = fmaf(da, hat2[i], s1[i]);
           s2[i] += da;
@@ -197,12 +199,12 @@ __global__ __launch_bounds__((NormShape<T, L>::THREADS)) void norm_residual_bwd_
           m1 = layer ? m1 * inv_c : 0.f;
           m2 *= inv_c;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) e[i] = r2 * (e[i] - m1 - hat2[i] * m2);
+          for (int i = 0; i < W; ++i) e[i] = r2 * (e[i] - m1 - hat2[i] * m2);
         }
       }
       if (MODE == EACH) {
-        if (may_own) each_store<T, L>(d_own_gate, r, lane, C, there, dg);
-        if (may_y) each_store<T, L>(a.d_y, r, lane, C, there, e);
+        if (may_own) each_store<T, L, W>(d_own_gate, r, lane, C, there, dg);
+        if (may_y) each_store<T, L, W>(a.d_y, r, lane, C, there, e);
       } else {
         if (may_own) ch.store(tg, step, dg);
         if (may_y) ch.store(ty, step, e);
@@ -212,25 +214,25 @@ __global__ __launch_bounds__((NormShape<T, L>::THREADS)) void norm_residual_bwd_
     if (a.shared_gate && a.d_gate) {
       if (a.sigmoid) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sg[i] *= gs[i] * (1.f - gs[i]);
+        for (int i = 0; i < W; ++i) sg[i] *= gs[i] * (1.f - gs[i]);
       }
       if (a.blocks_per_group == 1) {                     // this workgroup has seen all rows of the gate's row
-        slots_sum<T, L>(sg, comb, C, [&](int c, float v) { a.d_gate[g * C + c] = cpfn_from_f32<T>(v); });
+        slots_sum<T, L, W>(sg, comb, C, [&](int c, float v) { a.d_gate[g * C + c] = cpfn_from_f32<T>(v); });
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sg[i] = 0.f;
+        for (int i = 0; i < W; ++i) sg[i] = 0.f;
       }
     }
   }
   float *part = a.part + (size_t)blockIdx.x * nsums * C;
   if (a.sums12) {
-    slots_sum<T, L>(s1, comb, C, [&](int c, float v) { part[c] = v; });
-    slots_sum<T, L>(s2, comb, C, [&](int c, float v) { part[C + c] = v; });
+    slots_sum<T, L, W>(s1, comb, C, [&](int c, float v) { part[c] = v; });
+    slots_sum<T, L, W>(s2, comb, C, [&](int c, float v) { part[C + c] = v; });
   }
   if (a.sums34) {
-    slots_sum<T, L>(s3, comb, C, [&](int c, float v) { part[2 * C + c] = v; });
-    slots_sum<T, L>(s4, comb, C, [&](int c, float v) { part[3 * C + c] = v; });
+    slots_sum<T, L, W>(s3, comb, C, [&](int c, float v) { part[2 * C + c] = v; });
+    slots_sum<T, L, W>(s4, comb, C, [&](int c, float v) { part[3 * C + c] = v; });
   }
-  if (nsums == 5) slots_sum<T, L>(sg, comb, C, [&](int c, float v) { part[4 * C + c] = v; });
+  if (nsums == 5) slots_sum<T, L, W>(sg, comb, C, [&](int c, float v) { part[4 * C + c] = v; });
 }
 
 // The workgroups' sums -> gradients of the parameters (grid.y 0: S1, S2; 1: S3, S4) and of a shared gate (grid.y 2 + group).
@@ -279,20 +281,21 @@ template <typename T> __global__ __launch_bounds__(1024) void norm_residual_redu
   }
 }
 
-// Two waves on each SIMD run at once; at least four row sets for each workgroup, or its sums cost as much as its rows.  (Where three fit
-// the registers they measured 0 to 30 % slower: more workgroups' sums, and two keep enough rows in flight.)
-NormSplit split(long long P, int C, long long gate_rows) { return norm_split(P, C, gate_rows, 2048, 4); }
+// Two waves on each SIMD run at once (one with 16 channels a lane); at least four row sets for each workgroup, or its sums cost as much
+// as its rows.  (Where three waves fit the registers they measured 0 to 30 % slower: more workgroups' sums, and two keep enough rows in
+// flight.)
+NormSplit split(long long P, int C, int W, long long gate_rows) { return norm_split(P, C, W, gate_rows, 2048, 4); }
 
-template <typename T, int L, NormForm FORM> void launch_form(const NormBwd<T> &a, int nblk, NormMode mode, hipStream_t st) {
-  constexpr int THREADS = NormShape<T, L>::THREADS;
-  if (mode == WHOLE) norm_residual_bwd_kernel<T, L, WHOLE, FORM><<<nblk, THREADS, 0, st>>>(a);
-  else norm_residual_bwd_kernel<T, L, RAGGED, FORM><<<nblk, THREADS, 0, st>>>(a);
+template <typename T, int L, int W, NormForm FORM> void launch_form(const NormBwd<T> &a, int nblk, NormMode mode, hipStream_t st) {
+  constexpr int THREADS = NormShape<T, L, W>::THREADS;
+  if (W == 16 || mode == WHOLE) norm_residual_bwd_kernel<T, L, W, WHOLE, FORM><<<nblk, THREADS, 0, st>>>(a);
+  else if constexpr (W == 8) norm_residual_bwd_kernel<T, L, W, RAGGED, FORM><<<nblk, THREADS, 0, st>>>(a);
 }
-template <typename T, int L> void launch(const NormBwd<T> &a, int nblk, NormMode mode, hipStream_t st) {
-  if (!a.d_normed || (a.y && !a.weight)) launch_form<T, L, ANY>(a, nblk, mode, st);
-  else if (!a.y) launch_form<T, L, FRONT>(a, nblk, mode, st);
-  else if (a.gate && !a.shared_gate) launch_form<T, L, BLOCK_OWN>(a, nblk, mode, st);
-  else launch_form<T, L, BLOCK>(a, nblk, mode, st);
+template <typename T, int L, int W> void launch(const NormBwd<T> &a, int nblk, NormMode mode, hipStream_t st) {
+  if (!a.d_normed || (a.y && !a.weight)) launch_form<T, L, W, ANY>(a, nblk, mode, st);
+  else if (!a.y) launch_form<T, L, W, FRONT>(a, nblk, mode, st);
+  else if (a.gate && !a.shared_gate) launch_form<T, L, W, BLOCK_OWN>(a, nblk, mode, st);
+  else launch_form<T, L, W, BLOCK>(a, nblk, mode, st);
 }
 
 struct Grads { float *d_weight, *d_bias, *d_scale, *d_next_weight, *d_next_bias; };
@@ -301,7 +304,8 @@ template <typename T>
 int backward(const void *x, const void *y, const void *gate, const float *weight, const float *bias, const float *scale,
              const float *next_weight, const void *d_out, const void *d_normed, long long P, int C, long long gate_rows, int layer,
              int sigmoid, float eps, void *d_x, void *d_y, void *d_gate, const Grads &d, float *workspace, hipStream_t st) {
-  const NormSplit s = split(P, C, gate_rows);
+  const int W = norm_width(C, sizeof(T));
+  const NormSplit s = split(P, C, W, gate_rows);
   NormBwd<T> a;
   a.x = (const T *)x; a.y = (const T *)y; a.gate = (const T *)gate; a.d_out = (const T *)d_out; a.d_normed = (const T *)d_normed;
   a.weight = weight; a.bias = bias; a.scale = scale; a.next_weight = next_weight;
@@ -315,16 +319,18 @@ int backward(const void *x, const void *y, const void *gate, const float *weight
   a.sums34 = d.d_next_weight || d.d_next_bias;
   const NormMode mode = norm_mode<T>(P, C);
   if (mode == EACH) {
-    norm_residual_bwd_kernel<T, 8, EACH, ANY><<<s.nblk, 256, 0, st>>>(a);
+    norm_residual_bwd_kernel<T, 8, 8, EACH, ANY><<<s.nblk, 256, 0, st>>>(a);
+  } else if (W == 16) {
+    if constexpr (sizeof(T) == 2) launch<T, 64, 16>(a, s.nblk, mode, st);
   } else {
-    switch (norm_lanes(C)) {
-      case 8: launch<T, 8>(a, s.nblk, mode, st); break;
-      case 16: launch<T, 16>(a, s.nblk, mode, st); break;
-      case 32: launch<T, 32>(a, s.nblk, mode, st); break;
-      case 64: launch<T, 64>(a, s.nblk, mode, st); break;
-      case 128: launch<T, 128>(a, s.nblk, mode, st); break;
-      case 256: launch<T, 256>(a, s.nblk, mode, st); break;
-      default: launch<T, 512>(a, s.nblk, mode, st); break;
+    switch (norm_lanes(C, W)) {
+      case 8: launch<T, 8, 8>(a, s.nblk, mode, st); break;
+      case 16: launch<T, 16, 8>(a, s.nblk, mode, st); break;
+      case 32: launch<T, 32, 8>(a, s.nblk, mode, st); break;
+      case 64: launch<T, 64, 8>(a, s.nblk, mode, st); break;
+      case 128: launch<T, 128, 8>(a, s.nblk, mode, st); break;
+      case 256: launch<T, 256, 8>(a, s.nblk, mode, st); break;
+      default: launch<T, 512, 8>(a, s.nblk, mode, st); break;
     }
   }
   const bool gate_part = a.shared_gate && d_gate && s.blocks_per_group > 1;
@@ -345,7 +351,8 @@ int backward(const void *x, const void *y, const void *gate, const float *weight
 extern "C" long long cpfn_norm_residual_workspace(long long P, int C, long long gate_rows) {
   if (P < 0 || C < 1 || C > CPFN_NORM_MAX_C || gate_rows < 0 || (gate_rows > 0 && P % gate_rows != 0)) return -1;
   if (P == 0) return 0;
-  return (long long)split(P, C, gate_rows).nblk * 5 * C * (long long)sizeof(float);
+  const int a = split(P, C, norm_width(C, 2), gate_rows).nblk, b = split(P, C, norm_width(C, 4), gate_rows).nblk;
+  return (long long)(a > b ? a : b) * 5 * C * (long long)sizeof(float);
 }
 
 extern "C" int cpfn_norm_residual_bwd(const void *x, const void *y, const void *gate, const float *weight, const float *bias,

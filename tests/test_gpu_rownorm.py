@@ -169,7 +169,7 @@ def test_a_gate_shared_by_groups_of_rows(groups, each, C):
 
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
-@pytest.mark.parametrize("C", [40, 63, 104, 127, 240, 251, 472, 509, 936, 1021, 1928, 2045, 3080, 4091])
+@pytest.mark.parametrize("C", [40, 63, 104, 127, 240, 251, 472, 509, 520, 936, 1021, 1024, 1032, 1928, 2045, 3080, 4091])
 def test_every_form_at_every_number_of_lanes(C, dtype):
     """Rows of one to eight waves, whole and ragged: the whole block with its own gate, a shared one and none, the norm in front, and what
     has no kernel of its own (no norm of y)."""
