@@ -287,7 +287,8 @@ gather_rows = GatherRows.apply
 
 # ----------------------------------------------------------- a routed residual block's row operators
 # (the autograd nodes: csrc/native.cpp; rows that are not contiguous are copied, as by the nodes above.  Forward and backward passes can be
-#  captured; a captured backward pass is refused while an eager graph of the same leaves is alive on the default stream)
+#  captured; a captured backward pass is refused while an eager graph of the same leaves is alive on the default stream; a forward-mode
+#  tangent on an input, or on the gradient of a backward pass, is refused)
 def norm_residual(x, y, weight=None, bias=None, gate=None, gate_act="none", scale=None, next_weight=None, next_bias=None, kind="rms",
                   eps=1e-5):
     """The rows x [P, C] that run past a residual block and the block's result y [P, C] (fp32, bf16 or fp16) -> (out, normed):

@@ -199,6 +199,14 @@ void not_again(variable_list &grads, const char *what) {
     if (g.defined()) g = out[k++];
 }
 
+// Forward-mode derivatives (torch.autograd.forward_ad) are refused: a kernel reads an input's value alone, and its result would stand for
+// one whose derivative is zero.  Also where autograd records nothing: neither requires_grad nor no_grad says anything about them.
+bool tangent(const Tensor &t) { return t.defined() && t._fw_grad(0).defined(); }
+bool tangent(const Maybe &t) { return t.has_value() && tangent(*t); }
+template <typename... A> void refuse_tangents(const char *what, const A &...tensors) {
+  REQUIRE(!(tangent(tensors) || ...), what, " has no forward-mode derivative (a tensor carries a tangent: torch.autograd.forward_ad.unpack_dual gives its value)");
+}
+
 // A backward pass that is captured must not reach a leaf whose gradient is accumulated on the default stream, which cannot take part in a
 // capture.  It is where an eager graph of the same leaf, built on that stream, is still alive: the leaf has one accumulating node, which
 // keeps the stream that it was made on.
@@ -241,6 +249,7 @@ struct NormResidual : public torch::autograd::Function<NormResidual> {
   static variable_list backward(AutogradContext *ctx, const variable_list &d) {
     const auto saved = ctx->get_saved_variables();
     check_capture(saved[0]);
+    for (const Tensor &t : d) refuse_tangents("norm_residual", t);
     const int64_t how = ctx->saved_data["how"].toInt();
     const Norm n{saved[0], saved[1], saved[2], saved[3], saved[4], saved[5], saved[6], Tensor(), (how & 1) != 0, (how & 2) != 0, ctx->saved_data["eps"].toDouble()};
     const bool given[8] = {true, n.y.defined(), n.weight.defined(), n.bias.defined(), n.gate.defined(), n.scale.defined(), n.next_weight.defined(), (how & 4) != 0};
@@ -262,6 +271,7 @@ struct NormResidual : public torch::autograd::Function<NormResidual> {
 
 std::tuple<Maybe, Maybe> norm_residual(const Tensor &x, const Maybe &y, const Maybe &weight, const Maybe &bias, const Maybe &gate, bool sigmoid,
                                        const Maybe &scale, const Maybe &next_weight, const Maybe &next_bias, bool layer, double eps) {
+  refuse_tangents("norm_residual", x, y, weight, bias, gate, scale, next_weight, next_bias);
   if (!recorded(x, y, weight, bias, gate, scale, next_weight, next_bias)) {
     const auto r = Norm{x.contiguous(), contiguous(or_none(y)), or_none(weight), or_none(bias), contiguous(or_none(gate)), or_none(scale), or_none(next_weight),
                         or_none(next_bias), sigmoid, layer, eps}.forward();
@@ -369,6 +379,7 @@ struct RouteGather : public torch::autograd::Function<RouteGather> {
   static variable_list backward(AutogradContext *ctx, const variable_list &d) {
     const auto saved = ctx->get_saved_variables();
     check_capture(saved[1]);
+    refuse_tangents("route_gather", d[0]);
     variable_list grads(4);
     grads[0] = combine_rows(d[0].contiguous(), Tensor(), Plan{saved[0], saved[1], ctx->saved_data["E"].toInt()});
     not_again(grads, "route_gather");
@@ -385,6 +396,7 @@ struct RouteCombine : public torch::autograd::Function<RouteCombine> {
   static variable_list backward(AutogradContext *ctx, const variable_list &d) {
     const auto saved = ctx->get_saved_variables();
     check_capture(saved[3]);
+    refuse_tangents("route_combine", d[0]);
     const bool weighted = saved[1].defined();
     const auto g = combine_rows_bwd(d[0].contiguous(), saved[0], saved[1], Plan{saved[2], saved[3], ctx->saved_data["E"].toInt()}, ctx->needs_input_grad(0),
                                     weighted && ctx->needs_input_grad(1));
@@ -480,9 +492,11 @@ PYBIND11_MODULE(_native, m) {
     return pair_of(r.first, r.second);
   }, free_gil());
   m.def("route_gather", [](const Tensor &rows, const Tensor &offsets, const Tensor &place, int64_t E) {
+    refuse_tangents("route_gather", rows);
     return recorded(rows) ? RouteGather::apply(rows, offsets, place, E) : gather_rows(rows.contiguous(), Plan{offsets, place, E});
   }, free_gil());
   m.def("route_combine", [](const Tensor &sorted, const Maybe &weights, const Tensor &offsets, const Tensor &place, int64_t E) {
+    refuse_tangents("route_combine", sorted, weights);
     if (!recorded(sorted, weights)) return combine_rows(sorted.contiguous(), contiguous(or_none(weights)), Plan{offsets, place, E});
     return RouteCombine::apply(sorted, weights, offsets, place, E);
   }, free_gil());
