@@ -182,21 +182,24 @@ std::vector<Maybe> norm_residual_bwd(const Tensor &x, const Maybe &y, const Mayb
   return r;
 }
 
-// The gradients of a backward pass that is itself recorded (create_graph) can be used, but not differentiated again.
-void not_again(variable_list &grads, const char *what) {
-  if (!at::GradMode::is_enabled()) return;
+// Results that can be used, but not differentiated: autograd raises `error` where it comes to them.
+void not_differentiable(variable_list &results, std::string error) {
   variable_list in;
-  for (Tensor &g : grads)
+  for (Tensor &g : results)
     if (g.defined()) {
       in.push_back(g.detach());
       in.back().set_requires_grad(true);
     }
   if (in.empty()) return;
-  auto node = std::make_shared<torch::autograd::DelayedError>(c10::str(what, " is differentiable once: its gradients cannot be differentiated"), (int64_t)in.size());
+  auto node = std::make_shared<torch::autograd::DelayedError>(std::move(error), (int64_t)in.size());
   auto out = (*node)(std::move(in));
   size_t k = 0;
-  for (Tensor &g : grads)
+  for (Tensor &g : results)
     if (g.defined()) g = out[k++];
+}
+// The gradients of a backward pass that is itself recorded (create_graph).
+void not_again(variable_list &grads, const char *what) {
+  if (at::GradMode::is_enabled()) not_differentiable(grads, c10::str(what, " is differentiable once: its gradients cannot be differentiated"));
 }
 
 // Forward-mode derivatives (torch.autograd.forward_ad) are refused: a kernel reads an input's value alone, and its result would stand for
@@ -417,10 +420,13 @@ struct Table {
   std::vector<long long> n;
   std::vector<int> type;
   int64_t bytes = 0;
+  bool recorded = false;                     // a tensor that autograd follows
 
   const Tensor &add(PyObject *o, const char *name, c10::Device &device) {
     REQUIRE(THPVariable_Check(o), name, " must be tensors");
     const Tensor &t = THPVariable_Unpack(o);
+    refuse_tangents(name, t);
+    recorded |= t.requires_grad();
     REQUIRE(t.is_cuda(), name, " must be CUDA(HIP) tensors: CPU not supported");
     if (device.is_cpu()) device = t.device();
     REQUIRE(t.device() == device, name, " must be on one device (got ", device, " and ", t.device(), ")");
@@ -435,7 +441,8 @@ struct Table {
   }
 };
 
-// the norm over all gradients; max_norm: clipped to it, in place or into `out`
+// the norm over all gradients; max_norm: clipped to it, in place or into `out`.  The norm of tensors that autograd follows (gradients of
+// create_graph, parameters) has a value and no derivative: differentiating it raises.  Clipping works on values, as under no_grad.
 Tensor grad_norm(const py::list &grads, int p, std::optional<double> max_norm, const std::optional<py::list> &out) {
   const size_t count_ = grads.size();
   REQUIRE(!out || out->size() == count_, "out must have a tensor for each gradient (got ", out ? out->size() : 0, " for ", count_, ")");
@@ -469,6 +476,11 @@ Tensor grad_norm(const py::list &grads, int p, std::optional<double> max_norm, c
   } else {
     check_status(cpfn_grad_norm(src.at.data(), src.n.data(), src.type.data(), (int)count_, p, fptr(norm), ptr(ws), stream), "cpfn_grad_norm");
     count("cpfn_grad_norm", src.bytes);
+    if (src.recorded && at::GradMode::is_enabled()) {
+      variable_list r{norm};
+      not_differentiable(r, "grad_norm has no derivative: under torch.no_grad(), or of detached tensors, it is a plain value");
+      return r[0];
+    }
   }
   return norm;
 }

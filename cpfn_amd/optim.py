@@ -30,8 +30,11 @@ def _norm_code(norm_type):
 
 def grad_norm(grads, norm_type=2.0):
     """The norm over all values of a list of tensors (fp32, bf16 and fp16 together; any lengths; dense, in any order of their dimensions,
-    on one device) -> 0-dim fp32 tensor on that device, without a host synchronisation.  norm_type 1, 2 or inf; fp64 sums in a fixed order (bit-reproducible); NaN if any value is NaN.
-    An empty list: a zero on the CPU."""
+    on one device) -> 0-dim fp32 tensor on that device, without a host synchronisation.  norm_type 1, 2 or inf; fp64 sums in a fixed order
+    (bit-reproducible); NaN if any value is NaN.  An empty list: a zero on the CPU.
+    A value, not a differentiable function (no gradient penalty): of tensors that autograd follows (gradients of create_graph=True,
+    parameters) the result requires a gradient and raises where one is asked of it; under torch.no_grad() it is a plain tensor.
+    Forward-mode tangents are refused."""
     return _native_call("grad_norm", _list_of(grads), _norm_code(norm_type), None, None)
 
 
@@ -39,7 +42,8 @@ def clip_grads_(grads, max_norm, norm_type=2.0, out=None):
     """grads *= min(1, max_norm / (norm + 1e-6)) with the norm of grad_norm -> that norm (before clipping, on the device).  Nothing is
     synchronised, and in place nothing is written where the factor is 1.  out: tensors of the same shapes, of the gradients' types or
     fp32 (master gradients), that take the result instead; a gradient listed twice, or memory shared with a tensor that is written, is
-    refused.  An infinite norm gives the factor 0 and a NaN one NaN, as the formula has it."""
+    refused.  It works on values, as under torch.no_grad(), whatever autograd follows; forward-mode tangents are refused.  An infinite norm
+    gives the factor 0 and a NaN one NaN, as the formula has it."""
     return _native_call("grad_norm", _list_of(grads), _norm_code(norm_type), float(max_norm), None if out is None else _list_of(out))
 
 
@@ -51,7 +55,8 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     if error_if_nonfinite and grads:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("error_if_nonfinite reads the norm on the host: not inside a stream capture")
-        norm = float(grad_norm(grads, norm_type))
+        with torch.no_grad():
+            norm = float(grad_norm(grads, norm_type))
         if not norm < float("inf"):
             raise RuntimeError("the norm of the gradients is %r: not clipped" % norm)
     return clip_grads_(grads, max_norm, norm_type)

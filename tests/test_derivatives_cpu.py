@@ -1,10 +1,11 @@
-"""CPU: derivatives that the routed residual block's operators do not have are refused, not lost: a forward-mode tangent on any input.
+"""CPU: derivatives that the routed residual block's operators do not have are refused, not lost: a forward-mode tangent on any input, or on a
+tensor of a gradient list.
 (The refusal comes before the check of the device, so that it shows without a GPU.)"""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
 
-from cpfn_amd import autograd_ops, ops
+from cpfn_amd import autograd_ops, ops, optim
 
 
 def _plan(rows, k, E):
@@ -34,3 +35,11 @@ def test_forward_mode_tangents_are_refused(trained, grad_mode):
                 t[n] = fwd.make_dual(t[n], torch.ones_like(t[n]))
                 with pytest.raises(RuntimeError, match="forward-mode"):
                     call(t)
+
+
+def test_forward_mode_tangents_in_a_gradient_list_are_refused():
+    with fwd.dual_level(), torch.no_grad():
+        dual = fwd.make_dual(torch.ones(5), torch.ones(5))
+        for call in (lambda: optim.grad_norm([dual]), lambda: optim.clip_grads_([dual], 1.0)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()

@@ -1,5 +1,5 @@
 """Derivatives that the routed residual block's operators do not have are refused on the device, not lost: forward-mode tangents on an
-input or on the gradient that a backward pass is given."""
+input or on the gradient that a backward pass is given; the norm of gradients that are themselves recorded."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
@@ -49,3 +49,35 @@ def test_a_tangent_of_the_gradient_is_refused():
                 torch.autograd.grad(out, list(t.values()), d, retain_graph=True, allow_unused=True)
         got = torch.autograd.grad(out, list(t.values()), torch.ones_like(out), allow_unused=True)
         assert any(v is not None and bool(torch.isfinite(v).all()) for v in got), name
+
+
+def test_the_norm_of_recorded_gradients_raises_where_it_is_differentiated():
+    """A gradient penalty on optim.grad_norm would otherwise train as if the penalty were not there."""
+    from cpfn_amd import optim
+    torch.manual_seed(0)
+    w = torch.nn.Parameter(torch.randn(7, 5, device=DEV))
+    x = torch.randn(9, 7, device=DEV)
+    loss = ((x @ w) ** 3).sum()
+    (g,) = torch.autograd.grad(loss, [w], create_graph=True)
+    for recorded in (g, w):
+        plain = recorded.detach()
+        for p in (1.0, 2.0, float("inf")):
+            want = optim.grad_norm([plain], p)
+            got = optim.grad_norm([recorded], p)
+            assert not want.requires_grad and got.requires_grad and torch.equal(got.detach(), want)
+            with pytest.raises(RuntimeError, match="grad_norm"):
+                (loss + got ** 2).backward(retain_graph=True)
+            with torch.no_grad():
+                assert not optim.grad_norm([recorded], p).requires_grad
+    w.grad = None
+    loss.backward(create_graph=True)                       # clipping works on values, as torch.nn.utils.clip_grad_norm_ does
+    before = w.grad.detach().clone()
+    norm = optim.clip_grad_norm_([w], 1.0, error_if_nonfinite=True)
+    assert not norm.requires_grad and torch.equal(norm, optim.grad_norm([before]))
+    torch.testing.assert_close(w.grad.detach(), before / (norm + 1e-6), rtol=1e-6, atol=0.0)     # (three roundings)
+    w.grad = None
+    with fwd.dual_level():
+        dual = fwd.make_dual(before.clone(), torch.ones_like(before))
+        for call in (lambda: optim.grad_norm([dual]), lambda: optim.clip_grads_([dual], 1.0), lambda: optim.clip_grads_([before], 1.0, out=[dual])):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
