@@ -340,12 +340,13 @@ class SPFNTrainer:
         return self.optimizer.grad_norm if isinstance(self.optimizer, FlatAdam) else self._grad_norm
 
     def _clip_bucket(self):
-        """Clip the flat bucket in place for an optimizer that is not FlatAdam (which clips what it reads)."""
+        """Clip the gradients in the flat bucket in place for an optimizer that is not FlatAdam (which clips what it reads)."""
         if self.max_grad_norm is None:
             return
         if self.bucket.flat.is_cuda:
             from .optim import clip_grads_
-            self._grad_norm = clip_grads_(self.bucket.flat, self.max_grad_norm)
+            # (the gradients, not the whole bucket: a NaN factor would stay in the slices of parameters without one)
+            self._grad_norm = clip_grads_([p.grad for p in self.bucket.params if p.grad is not None], self.max_grad_norm)
         else:
             self._grad_norm = torch.nn.utils.clip_grad_norm_(self.bucket.params, self.max_grad_norm)
 
