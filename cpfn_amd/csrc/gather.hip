@@ -41,6 +41,10 @@ __global__ __launch_bounds__(TPB) void group_bwd_kernel(const float *__restrict_
     atomicAdd(grad_points + ((size_t)b * C + c) * N + ii, grad_out[((size_t)b * C + c) * J + j]);
 }
 
+// An index outside [0, M) is the nearest row that there is, as in the gathers above: three_nn leaves M where there is no neighbour (a
+// query that is not finite, fewer than three known points), and row M of the last cloud is behind the tensor's end.
+__device__ __forceinline__ int in_cloud(int i, int M) { return i < 0 ? 0 : (i >= M ? M - 1 : i); }
+
 // out[b,c,n] = Σ_t feats[b,c,idx[b,n,t]] * w[b,n,t]   (products rounded, summed in t order)
 __global__ __launch_bounds__(TPB) void interp_fwd_kernel(const float *__restrict__ feats,
                                                          const int *__restrict__ idx,
@@ -51,7 +55,7 @@ __global__ __launch_bounds__(TPB) void interp_fwd_kernel(const float *__restrict
   if (n >= N) return;
   const int *ii = idx + ((size_t)b * N + n) * 3;
   const float *ww = w + ((size_t)b * N + n) * 3;
-  const int i0 = ii[0], i1 = ii[1], i2 = ii[2];
+  const int i0 = in_cloud(ii[0], M), i1 = in_cloud(ii[1], M), i2 = in_cloud(ii[2], M);
   const float w0 = ww[0], w1 = ww[1], w2 = ww[2];
   const int c0 = blockIdx.y * c_per_block;
   const int c1 = min(C, c0 + c_per_block);
@@ -71,7 +75,7 @@ __global__ __launch_bounds__(TPB) void interp_bwd_kernel(const float *__restrict
   if (n >= N) return;
   const int *ii = idx + ((size_t)b * N + n) * 3;
   const float *ww = w + ((size_t)b * N + n) * 3;
-  const int i0 = ii[0], i1 = ii[1], i2 = ii[2];
+  const int i0 = in_cloud(ii[0], M), i1 = in_cloud(ii[1], M), i2 = in_cloud(ii[2], M);
   const float w0 = ww[0], w1 = ww[1], w2 = ww[2];
   const int c0 = blockIdx.y * c_per_block;
   const int c1 = min(C, c0 + c_per_block);
@@ -142,8 +146,9 @@ __global__ __launch_bounds__(TPB) void interp_rows_fwd_kernel(const float *__res
   const int *ii = idx + ((size_t)b * N + n) * 3;
   const float *ww = w + ((size_t)b * N + n) * 3;
   const float *f = feats + (size_t)b * M * C;
-  const float acc = __fadd_rn(__fmul_rn(f[(size_t)ii[0] * C + c], ww[0]), __fmul_rn(f[(size_t)ii[1] * C + c], ww[1]));
-  out[(size_t)b * N * C + e] = __fadd_rn(acc, __fmul_rn(f[(size_t)ii[2] * C + c], ww[2]));
+  const int i0 = in_cloud(ii[0], M), i1 = in_cloud(ii[1], M), i2 = in_cloud(ii[2], M);
+  const float acc = __fadd_rn(__fmul_rn(f[(size_t)i0 * C + c], ww[0]), __fmul_rn(f[(size_t)i1 * C + c], ww[1]));
+  out[(size_t)b * N * C + e] = __fadd_rn(acc, __fmul_rn(f[(size_t)i2 * C + c], ww[2]));
 }
 
 __global__ __launch_bounds__(TPB) void interp_rows_bwd_kernel(const float *__restrict__ grad_out,
@@ -159,9 +164,9 @@ __global__ __launch_bounds__(TPB) void interp_rows_bwd_kernel(const float *__res
   const float *ww = w + ((size_t)b * N + n) * 3;
   const float g = grad_out[(size_t)b * N * C + e];
   float *o = grad_feats + (size_t)b * M * C;
-  atomicAdd(o + (size_t)ii[0] * C + c, g * ww[0]);
-  atomicAdd(o + (size_t)ii[1] * C + c, g * ww[1]);
-  atomicAdd(o + (size_t)ii[2] * C + c, g * ww[2]);
+  atomicAdd(o + (size_t)in_cloud(ii[0], M) * C + c, g * ww[0]);
+  atomicAdd(o + (size_t)in_cloud(ii[1], M) * C + c, g * ww[1]);
+  atomicAdd(o + (size_t)in_cloud(ii[2], M) * C + c, g * ww[2]);
 }
 
 // ---------------------------------------------------------------- bf16 row movers of the MLP path
@@ -197,7 +202,7 @@ __global__ __launch_bounds__(TPB) void interp_rows_bf16_kernel(const unsigned sh
   float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
   for (int t = 0; t < 3; ++t) {
-    const uint4 r = *(const uint4 *)(feats + ((size_t)b * M + ii[t]) * C + c0);
+    const uint4 r = *(const uint4 *)(feats + ((size_t)b * M + in_cloud(ii[t], M)) * C + c0);
     const unsigned short *h = (const unsigned short *)&r;
     const float wt = ww[t];
 #pragma unroll
@@ -238,7 +243,7 @@ __global__ __launch_bounds__(TPB) void concat_interp_bf16_kernel(const unsigned 
   float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
   for (int t = 0; t < 3; ++t) {
-    const uint4 r = *(const uint4 *)(feats + ((size_t)b * M + ii[t]) * C2 + c0);
+    const uint4 r = *(const uint4 *)(feats + ((size_t)b * M + in_cloud(ii[t], M)) * C2 + c0);
     const unsigned short *h = (const unsigned short *)&r;
     const float wt = ww[t];
 #pragma unroll
