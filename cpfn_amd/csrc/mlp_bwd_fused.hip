@@ -206,7 +206,9 @@ __global__ __launch_bounds__(512) void mlp_bwd_fused_kernel(
       for (int i = 0; i < NA; ++i) {
         const long long p = min(base + arow + i * RPA, p1 - 1);
         if (XT && ap.g_idx) {
-          const long long row = (long long)((int)p / ap.g_rpc) * ap.g_nsrc + gnx[XT ? i : 0];
+          // (an index behind the table — ball_query's n_src of an empty ball — stays inside the cloud; the forward layer's loads are
+          //  bounded by its descriptor)
+          const long long row = (long long)((int)p / ap.g_rpc) * ap.g_nsrc + min((unsigned)gnx[XT ? i : 0], (unsigned)(ap.g_nsrc - 1));
           va[sidx][i] = *(const uint4 *)(A + row * lda + acol);
           gnx[XT ? i : 0] = ap.g_idx[min(base + STEP + arow + i * RPA, p1 - 1)];      // for the next issue (base + STEP)
         } else {

@@ -64,3 +64,27 @@ def test_rows_are_taken_from_the_own_cloud(B, M, N):
         assert torch.equal(out[..., 8:].float(), want) and torch.equal(out[..., :8], skip)
         d = torch.cat([torch.zeros_like(skip), grad.to(torch.bfloat16)], 2)
         assert torch.equal(torch.autograd.grad(out, f, d)[0], back.to(torch.bfloat16))
+
+
+def test_rows_gathered_in_the_backward_pass_are_the_own_cloud_s():
+    """The one-pass backward kernel that gathers its input rows, on indices behind the table (ball_query's N of an empty ball) and on the
+    same indices brought inside: the same bits."""
+    from cpfn_amd import lib as _l
+    from cpfn_amd.ops import _ptr, _stream
+    h = _l.lib()
+    B, n_src, rpc, D = 5, 200, 8192, 128
+    P = B * rpc
+    g = torch.Generator().manual_seed(1)
+    table, gy, y, W = (torch.randn(n, D, generator=g).to(torch.bfloat16).to(DEV) for n in (B * n_src, P, P, D))
+    coef, scale, shift, xyz = (torch.randn(*n, generator=g).to(DEV) for n in ((3, D), (D,), (D,), (P, 3)))
+    idx = torch.randint(0, n_src + 2, (P,), generator=g).to(torch.int32)
+    idx[-64:] = n_src
+    idx[:7] = 2 ** 31 - 1
+    splits = h.cpfn_mlp_wgrad_splits(P, D, D)
+    res = []
+    for i in (idx.to(DEV), idx.clamp(max=n_src - 1).to(DEV)):
+        ws, out, wx = torch.empty(splits * D * D, device=DEV), torch.empty(P, D, dtype=torch.bfloat16, device=DEV), torch.empty(splits * D * 3, device=DEV)
+        _l.check(h.cpfn_mlp_bwd_fused_xt_gather(_ptr(gy), _ptr(table), _ptr(i), rpc, n_src, _ptr(W), P, D, D, _ptr(ws), _ptr(out), _ptr(y), _ptr(coef),
+                                                _ptr(scale), _ptr(shift), _ptr(xyz), _ptr(wx), _stream()), "cpfn_mlp_bwd_fused_xt_gather")
+        res.append((ws, out, wx))
+    assert all(torch.equal(a, b) for a, b in zip(*res)) and bool(res[0][0].any())
