@@ -284,7 +284,7 @@ class SPFNTrainer:
         if max_grad_norm is not None and not float(max_grad_norm) >= 0.0:
             raise RuntimeError("max_grad_norm must not be negative (got %r)" % (max_grad_norm,))
         self.max_grad_norm = None if max_grad_norm is None else float(max_grad_norm)
-        self._grad_norm = None
+        self._grad_norm, self._stepped = None, False
         self.module = module
         self.batch_size = batch_size
         self.init_learning_rate, self.decay_step, self.decay_rate = init_learning_rate, decay_step, decay_rate
@@ -332,12 +332,14 @@ class SPFNTrainer:
 
     @property
     def grad_norm(self):
-        """The 2-norm of the last step's gradients before clipping, a 0-dim tensor (on the device, without a synchronisation); None
-        without max_grad_norm or before the first step."""
+        """The 2-norm of the last step's gradients before clipping, a 0-dim tensor (on the device, without a synchronisation): NaN or
+        infinite if that step was skipped for it; None without max_grad_norm or before the first step."""
         if self.max_grad_norm is None:
             return None
         from .optim import FlatAdam
-        return self.optimizer.grad_norm if isinstance(self.optimizer, FlatAdam) else self._grad_norm
+        if isinstance(self.optimizer, FlatAdam):
+            return self.optimizer.grad_norm if self._stepped else None
+        return self._grad_norm
 
     def _clip_bucket(self):
         """Clip the gradients in the flat bucket in place for an optimizer that is not FlatAdam (which clips what it reads)."""
@@ -349,6 +351,25 @@ class SPFNTrainer:
             self._grad_norm = clip_grads_([p.grad for p in self.bucket.params if p.grad is not None], self.max_grad_norm)
         else:
             self._grad_norm = torch.nn.utils.clip_grad_norm_(self.bucket.params, self.max_grad_norm)
+
+    def _count_step(self):
+        self.global_step += 1
+        self._stepped = True
+
+    def _skip_on_host(self):
+        """A step whose update the host skips: counted; its norm is taken all the same."""
+        self._host_skipped += 1
+        if self.max_grad_norm is None:
+            return
+        if not self.bucket.flat.is_cuda:
+            self._grad_norm = torch.linalg.vector_norm(self.bucket.flat)
+            return
+        from .optim import FlatAdam, grad_norm
+        norm = grad_norm(self.bucket.flat)
+        if isinstance(self.optimizer, FlatAdam):
+            self.optimizer.grad_norm.copy_(norm)
+        else:
+            self._grad_norm = norm
 
     def _skip_counter(self, device):
         if self._skipped_dev is None:
@@ -1028,7 +1049,7 @@ class SPFNTrainer:
                 self._exchange_with_stamps(batch["P"].device)
                 self._checked_optimizer_step(st["skipped"], fault=self.bucket.fault_slot.reshape(()))
                 st["fault_host"].copy_(self.bucket.fault_slot, non_blocking=True)
-            self.global_step += 1
+            self._count_step()
             if st["world"] > 1 and getattr(self, "_fault_raised", None) is not None:
                 # raise_fault(): the replay just issued carries the word through the collective (every rank skips); now stop.
                 # (The peers see the same reduced slot in their pinned word at the head of one of their next steps.)
@@ -1048,7 +1069,7 @@ class SPFNTrainer:
         if st["world"] > 1:
             self.bucket.all_reduce_mean()
             self._checked_optimizer_step(st["skipped"])
-        self.global_step += 1
+        self._count_step()
         return st["out"]
 
     def _exchange_with_stamps(self, dev):
@@ -1185,8 +1206,8 @@ class SPFNTrainer:
         elif bool(self.bucket.finite()) and (reduced_fault is None or float(reduced_fault) == 0.0):   # host sync (reference: 148)
             self._clipped_optimizer_step()
         else:
-            self._host_skipped += 1
-        self.global_step += 1
+            self._skip_on_host()
+        self._count_step()
         if world > 1 and not self.use_graphs:
             self._after_exchange_fault_check()
         return tuple(o.detach() for o in out)     # do not keep the autograd graph alive across steps

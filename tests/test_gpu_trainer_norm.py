@@ -1,6 +1,7 @@
-"""SPFNTrainer(max_grad_norm=): a step that is skipped for its gradients."""
+"""SPFNTrainer(max_grad_norm=): a step that is skipped for its gradients, and the norm that is reported."""
 import contextlib
 import io
+import math
 
 import pytest
 import torch
@@ -42,3 +43,15 @@ def test_training_goes_on_after_a_skipped_step(fused, graphs):
         assert same == (b is bad), step
         assert all(p.grad is not None or not bool(v.any()) for p, v in zip(tr.bucket.params, tr.bucket.views)), step
     assert (tr._graph is not None) == graphs
+
+
+@pytest.mark.parametrize("graphs", [False, True])
+@pytest.mark.parametrize("fused", [True, False])
+def test_the_norm_is_the_last_step_s(fused, graphs):
+    """Nothing before the first step; of a skipped step its own, not the one before."""
+    _, tr, batch, bad = trainer(use_graphs=graphs, require_graphs=graphs, fused_adam=None if fused else False)
+    assert tr.grad_norm is None
+    for step, b in enumerate((batch, bad, batch, batch, bad, batch)):
+        tr.step(b)
+        torch.cuda.synchronize()
+        assert math.isfinite(float(tr.grad_norm)) == (b is batch), step
