@@ -2,6 +2,8 @@
 
     python -m cpfn_amd.build [--force]
 
+and _native.so, the torch extension beside it, with g++ and torch's headers (of the torch that is installed).
+
 One translation unit per kernel family, linked into one shared object whose only
 exported symbols are the `extern "C"` entry points declared in include/cpfn_hip.h.
 Geometry files are compiled with -ffp-contract=off: their index outputs must be
@@ -141,23 +143,33 @@ def _check_isa(src):
             os.remove(os.path.join(OBJ, f))
 
 
-def _build_native(force):
-    """_native.so (csrc/native.cpp): the torch extension over the C ABI; host code only, linked to libcpfn_hip.so beside it."""
+def _native_command():
     import sysconfig
-    src = os.path.join(CSRC, "native.cpp")
-    if not force and not _stale(NATIVE, [src, os.path.join(HERE, "..", "include", "cpfn_hip.h")]):
-        return
     import torch
     from torch.utils.cpp_extension import include_paths
     cmd = ["g++", "-O2", "-fPIC", "-shared", "-std=c++17", "-fvisibility=hidden", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
            "-DTORCH_EXTENSION_NAME=_native", "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI]
     for d in include_paths() + [os.path.join(os.path.dirname(os.path.dirname(_hipcc())), "include"), sysconfig.get_paths()["include"]]:
         cmd += ["-isystem", d]
-    cmd += [src, "-o", NATIVE, "-L" + os.path.join(os.path.dirname(torch.__file__), "lib"), "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip",
-            "-ltorch", "-ltorch_python", "-L" + HERE, "-l:libcpfn_hip.so", "-Wl,-rpath,$ORIGIN"]
+    return cmd + [os.path.join(CSRC, "native.cpp"), "-o", NATIVE, "-L" + os.path.join(os.path.dirname(torch.__file__), "lib"), "-lc10", "-lc10_hip",
+                  "-ltorch_cpu", "-ltorch_hip", "-ltorch", "-ltorch_python", "-L" + HERE, "-l:libcpfn_hip.so", "-Wl,-rpath,$ORIGIN"]
+
+
+def _build_native(force):
+    """_native.so (csrc/native.cpp): the torch extension over the C ABI; host code only, linked to libcpfn_hip.so beside it.  It fits one
+    torch and one Python: what it was built for is kept beside the objects, and it is built again where that has changed."""
+    import torch
+    cmd = _native_command()
+    built_for = "\n".join([torch.__version__, str(torch.version.git_version), sys.version] + cmd)
+    stamp = os.path.join(OBJ, "native.built_for")
+    if not force and os.path.exists(stamp) and open(stamp).read() == built_for and not _stale(
+            NATIVE, [os.path.join(CSRC, "native.cpp"), os.path.join(HERE, "..", "include", "cpfn_hip.h")]):
+        return
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError("g++ failed for native.cpp:\n%s" % r.stderr[-4000:])
+    with open(stamp, "w") as f:
+        f.write(built_for)
 
 
 def build(force=False, verbose=False):
