@@ -10,7 +10,9 @@
 //   S1 = sum D a hat2,  S2 = sum D a,  S3 = sum d_normed hat1,  S4 = sum d_normed
 //   d_weight = scale S1,  d_bias = scale S2,  d_scale = weight S1 + bias S2,  d_next_weight = S3,  d_next_bias = S4
 // (hat2 = y without a post-norm).  A lane owns its channels for every row of its workgroup, so a column sum is a register until
-// the workgroup ends; the workgroups' sums are added by a second small launch in a fixed order: no atomics, bit-reproducible.
+// the workgroup ends, or for SEGMENT row sets: equal terms (a mean's gradient) are rounded the same way at each of n fp32 additions, off by
+// up to n 2^-24, so longer sums go to LDS in between.  The workgroups' sums are added by a second small launch in fp64, in a fixed order:
+// no atomics, bit-reproducible.
 // d_gate of rows that share one: the factor of the sigmoid is the same for all of them and comes after the sum.
 //
 // Memory bound up to 512 channels; above, registers (1024: one wave on a SIMD), the barriers of the row sums (up to six a row) and the
@@ -65,12 +67,16 @@ template <typename T, int L, int W, typename F> __device__ __forceinline__ void 
   }
 }
 
+constexpr int SEGMENT = 128;         // row sets whose sums are added in registers (workgroups of 16 to 32 sets are what the usual sizes give)
+
 template <typename T, int L, int W, NormMode MODE, NormForm FORM>
 __global__ __launch_bounds__((NormShape<T, L, W>::THREADS)) void norm_residual_bwd_kernel(const NormBwd<T> a) {
   constexpr int ROWS = NormShape<T, L, W>::ROWS, THREADS = NormShape<T, L, W>::THREADS, NP = NormShape<T, L, W>::NP;
   __shared__ float2 slots[16];
   __shared__ float comb[ROWS > 1 ? THREADS * W : 1];
-  int turn = 0;
+  __shared__ float held[5][THREADS * W];             // each lane's own: what its sums were before the present ones
+  int turn = 0, summed = 0;                            // summed: row sets in the registers
+  bool holds = false, holds_gate = false;
   const int lane = threadIdx.x & (L - 1), slot = threadIdx.x / L, C = a.C;
   const float inv_c = 1.f / (float)C;
   const bool layer = a.layer != 0, post = FORM != ANY || a.weight != nullptr, next = FORM != ANY || a.d_normed != nullptr;
@@ -87,131 +93,159 @@ __global__ __launch_bounds__((NormShape<T, L, W>::THREADS)) void norm_residual_b
   if (g1 > a.groups) g1 = a.groups;
   const int nsums = 4 + (a.shared_gate && a.blocks_per_group > 1);
   const unsigned set_bytes = (unsigned)(ROWS * C) * (unsigned)sizeof(T);
-  for (long long g = g0; g < g1; ++g) {
-    long long row0 = g * a.rows_per_gate, row1 = row0 + a.rows_per_gate;
-    if (a.blocks_per_group > 1) {
-      row0 += (long long)(blockIdx.x % a.blocks_per_group) * a.chunk;
-      if (row0 + a.chunk < row1) row1 = row0 + a.chunk;
+  const auto hold = [&](int k, float *v, bool more) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      float *h = &held[k][i * THREADS + threadIdx.x];
+      *h = more ? *h + v[i] : v[i];
+      v[i] = 0.f;
     }
-    RowChunk<T, L, W, MODE> ch;
-    ch.begin(row0, row1, a.P, C, lane, slot);
-    const T *own_gate = own ? a.gate : nullptr;
-    T *d_own_gate = own ? a.d_gate : nullptr;
-    const auto bx = ch.source(next ? a.x : nullptr), by = ch.source(a.y), bg = ch.source(own_gate), bd = ch.source(a.d_out), bn = ch.source(a.d_normed);
-    const auto tx = ch.target(a.d_x), ty = ch.target(a.d_y), tg = ch.target(d_own_gate);
-    RowRaw<T, L, W> rx, ry, rg, rd, rn;
-    unsigned o[NP], sh[NP];
-    const auto request = [&](unsigned step, long long r) {
-      if (MODE == EACH) {
-        each_load(rx, next ? a.x : nullptr, r, lane, C, r < row1);
-        if (may_y) each_load(ry, a.y, r, lane, C, r < row1);
-        if (may_own) each_load(rg, own_gate, r, lane, C, r < row1);
-        each_load(rd, a.d_out, r, lane, C, r < row1);
-        each_load(rn, a.d_normed, r, lane, C, r < row1);
-      } else {
-        ch.at(o, sh, step, r < row1);
-        ch.template load<true>(rx, bx, o);
-        if (may_y) ch.template load<true>(ry, by, o);
-        if (may_own) ch.template load<true>(rg, bg, o);
-        ch.template load<true>(rd, bd, o);
-        ch.template load<true>(rn, bn, o);
-      }
-    };
-    const auto requested = [&] {
-      arrived(rx);
-      if (may_y) arrived(ry);
-      if (may_own) arrived(rg);
-      arrived(rd); arrived(rn);
-    };
+  };
+  const auto whole = [&](int k, float *v) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) v[i] += held[k][i * THREADS + threadIdx.x];
+  };
+  for (long long g = g0; g < g1; ++g) {
+    long long first = g * a.rows_per_gate, last = first + a.rows_per_gate;
+    if (a.blocks_per_group > 1) {
+      first += (long long)(blockIdx.x % a.blocks_per_group) * a.chunk;
+      if (first + a.chunk < last) last = first + a.chunk;
+    }
     float gs[W];
     shared_gate<T, L, W>(gs, a.shared_gate ? a.gate + g * C : nullptr, lane, C, a.sigmoid);
-    arrived(sw); arrived(sb); arrived(nw);
-    request(0, row0 + slot);
-    requested();
-    unsigned step = 0;
-    for (long long base = row0; base < row1; base += ROWS, step += set_bytes) {
-      const long long r = base + slot;
-      const bool there = r < row1;
-      const float eps = there ? a.eps : 1.f;
-      float h[W], hat2[W], ga[W], D[W], dn[W], r2 = 0.f;
-      ch.settle(rx, sh); ch.settle(rd, sh); ch.settle(rn, sh);
-      row_unpack(rx, h);
-      row_unpack(rd, D);
-      row_unpack(rn, dn);
-      if (may_y) {
-        ch.settle(ry, sh);
-        row_unpack(ry, hat2);
-      }
-      if (may_own) {
-        ch.settle(rg, sh);
-        row_unpack(rg, ga);
-      }
-      unpacked();
-      request(step + set_bytes, r + ROWS);
-      if (has_y && post) r2 = row_normalise<T, L, W, MODE>(hat2, lane, C, inv_c, layer, eps, slots, turn);
-      if (own) gate_act<T, W>(ga, a.sigmoid);
-      const auto gate = [&](int i) { return own ? ga[i] : gs[i]; };
-      if (next) {
-        if (has_y) {
-#pragma unroll
-          for (int i = 0; i < W; ++i) h[i] = fmaf(gate(i), fmaf(hat2[i], sw[i], sb[i]), h[i]);
+    for (long long row0 = first; row0 < last; row0 += SEGMENT * ROWS) {
+      const long long row1 = row0 + SEGMENT * ROWS < last ? row0 + SEGMENT * ROWS : last;
+      const int sets = (int)((row1 - row0 + ROWS - 1) / ROWS);
+      if (summed + sets > SEGMENT) {
+        hold(0, s1, holds); hold(1, s2, holds); hold(2, s3, holds); hold(3, s4, holds);
+        holds = true;
+        summed = 0;
+        if (row0 > first) {                              // (a gate's sum begins with its group)
+          hold(4, sg, holds_gate);
+          holds_gate = true;
         }
-        const float r1 = row_normalise<T, L, W, MODE>(h, lane, C, inv_c, layer, eps, slots, turn);
-        float m1 = 0.f, m2 = 0.f;
-#pragma unroll
-        for (int i = 0; i < W; ++i) {
-          s3[i] = fmaf(dn[i], h[i], s3[i]);
-          s4[i] += dn[i];
-          dn[i] *= nw[i];
-          m1 += dn[i];
-          m2 = fmaf(dn[i], h[i], m2);
-        }
-        row_sum2<L>(m1, m2, slots, turn);
-        m1 = layer ? m1 * inv_c : 0.f;
-        m2 *= inv_c;
-#pragma unroll
-        for (int i = 0; i < W; ++i) D[i] = fmaf(r1, dn[i] - m1 - h[i] * m2, D[i]);
       }
-      if (MODE == EACH) each_store<T, L, W>(a.d_x, r, lane, C, there, D);
-      else ch.store(tx, step, D);
-      float e[W], dg[W];
-      if (has_y) {
-        if (a.d_gate) {
+      summed += sets;
+      RowChunk<T, L, W, MODE> ch;
+      ch.begin(row0, row1, a.P, C, lane, slot);
+      const T *own_gate = own ? a.gate : nullptr;
+      T *d_own_gate = own ? a.d_gate : nullptr;
+      const auto bx = ch.source(next ? a.x : nullptr), by = ch.source(a.y), bg = ch.source(own_gate), bd = ch.source(a.d_out), bn = ch.source(a.d_normed);
+      const auto tx = ch.target(a.d_x), ty = ch.target(a.d_y), tg = ch.target(d_own_gate);
+      RowRaw<T, L, W> rx, ry, rg, rd, rn;
+      unsigned o[NP], sh[NP];
+      const auto request = [&](unsigned step, long long r) {
+        if (MODE == EACH) {
+          each_load(rx, next ? a.x : nullptr, r, lane, C, r < row1);
+          if (may_y) each_load(ry, a.y, r, lane, C, r < row1);
+          if (may_own) each_load(rg, own_gate, r, lane, C, r < row1);
+          each_load(rd, a.d_out, r, lane, C, r < row1);
+          each_load(rn, a.d_normed, r, lane, C, r < row1);
+        } else {
+          ch.at(o, sh, step, r < row1);
+          ch.template load<true>(rx, bx, o);
+          if (may_y) ch.template load<true>(ry, by, o);
+          if (may_own) ch.template load<true>(rg, bg, o);
+          ch.template load<true>(rd, bd, o);
+          ch.template load<true>(rn, bn, o);
+        }
+      };
+      const auto requested = [&] {
+        arrived(rx);
+        if (may_y) arrived(ry);
+        if (may_own) arrived(rg);
+        arrived(rd); arrived(rn);
+      };
+      arrived(sw); arrived(sb); arrived(nw);
+      request(0, row0 + slot);
+      requested();
+      unsigned step = 0;
+      for (long long base = row0; base < row1; base += ROWS, step += set_bytes) {
+        const long long r = base + slot;
+        const bool there = r < row1;
+        const float eps = there ? a.eps : 1.f;
+        float h[W], hat2[W], ga[W], D[W], dn[W], r2 = 0.f;
+        ch.settle(rx, sh); ch.settle(rd, sh); ch.settle(rn, sh);
+        row_unpack(rx, h);
+        row_unpack(rd, D);
+        row_unpack(rn, dn);
+        if (may_y) {
+          ch.settle(ry, sh);
+          row_unpack(ry, hat2);
+        }
+        if (may_own) {
+          ch.settle(rg, sh);
+          row_unpack(rg, ga);
+        }
+        unpacked();
+        request(step + set_bytes, r + ROWS);
+        if (has_y && post) r2 = row_normalise<T, L, W, MODE>(hat2, lane, C, inv_c, layer, eps, slots, turn);
+        if (own) gate_act<T, W>(ga, a.sigmoid);
+        const auto gate = [&](int i) { return own ? ga[i] : gs[i]; };
+        if (next) {
+          if (has_y) {
+#pragma unroll
+            for (int i = 0; i < W; ++i) h[i] = fmaf(gate(i), fmaf(hat2[i], sw[i], sb[i]), h[i]);
+          }
+          const float r1 = row_normalise<T, L, W, MODE>(h, lane, C, inv_c, layer, eps, slots, turn);
+          float m1 = 0.f, m2 = 0.f;
 #pragma unroll
           for (int i = 0; i < W; ++i) {
-            dg[i] = D[i] * fmaf(hat2[i], sw[i], sb[i]);
-            if (own) dg[i] *= a.sigmoid ? ga[i] * (1.f - ga[i]) : 1.f;
-            else sg[i] += dg[i];
+            s3[i] = fmaf(dn[i], h[i], s3[i]);
+            s4[i] += dn[i];
+            dn[i] *= nw[i];
+            m1 += dn[i];
+            m2 = fmaf(dn[i], h[i], m2);
           }
-        }
-        float m1 = 0.f, m2 = 0.f;
-#pragma unroll
-        for (int i = 0; i < W; ++i) {
-          const float da = D[i] * gate(i);
-          s1[i] = fmaf(da, hat2[i], s1[i]);
-          s2[i] += da;
-          e[i] = da * sw[i];                             // (sw = scale without a post-norm: e = du)
-          m1 += e[i];
-          m2 = fmaf(e[i], hat2[i], m2);
-        }
-        if (post) {
           row_sum2<L>(m1, m2, slots, turn);
           m1 = layer ? m1 * inv_c : 0.f;
           m2 *= inv_c;
 #pragma unroll
-          for (int i = 0; i < W; ++i) e[i] = r2 * (e[i] - m1 - hat2[i] * m2);
+          for (int i = 0; i < W; ++i) D[i] = fmaf(r1, dn[i] - m1 - h[i] * m2, D[i]);
         }
+        if (MODE == EACH) each_store<T, L, W>(a.d_x, r, lane, C, there, D);
+        else ch.store(tx, step, D);
+        float e[W], dg[W];
+        if (has_y) {
+          if (a.d_gate) {
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+              dg[i] = D[i] * fmaf(hat2[i], sw[i], sb[i]);
+              if (own) dg[i] *= a.sigmoid ? ga[i] * (1.f - ga[i]) : 1.f;
+              else sg[i] += dg[i];
+            }
+          }
+          float m1 = 0.f, m2 = 0.f;
+#pragma unroll
+          for (int i = 0; i < W; ++i) {
+            const float da = D[i] * gate(i);
+            s1[i] = fmaf(da, hat2[i], s1[i]);
+            s2[i] += da;
+            e[i] = da * sw[i];                             // (sw = scale without a post-norm: e = du)
+            m1 += e[i];
+            m2 = fmaf(e[i], hat2[i], m2);
+          }
+          if (post) {
+            row_sum2<L>(m1, m2, slots, turn);
+            m1 = layer ? m1 * inv_c : 0.f;
+            m2 *= inv_c;
+#pragma unroll
+            for (int i = 0; i < W; ++i) e[i] = r2 * (e[i] - m1 - hat2[i] * m2);
+          }
+        }
+        if (MODE == EACH) {
+          if (may_own) each_store<T, L, W>(d_own_gate, r, lane, C, there, dg);
+          if (may_y) each_store<T, L, W>(a.d_y, r, lane, C, there, e);
+        } else {
+          if (may_own) ch.store(tg, step, dg);
+          if (may_y) ch.store(ty, step, e);
+        }
+        requested();
       }
-      if (MODE == EACH) {
-        if (may_own) each_store<T, L, W>(d_own_gate, r, lane, C, there, dg);
-        if (may_y) each_store<T, L, W>(a.d_y, r, lane, C, there, e);
-      } else {
-        if (may_own) ch.store(tg, step, dg);
-        if (may_y) ch.store(ty, step, e);
-      }
-      requested();
     }
     if (a.shared_gate && a.d_gate) {
+      if (holds_gate) whole(4, sg);
+      holds_gate = false;
       if (a.sigmoid) {
 #pragma unroll
         for (int i = 0; i < W; ++i) sg[i] *= gs[i] * (1.f - gs[i]);
@@ -223,6 +257,7 @@ __global__ __launch_bounds__((NormShape<T, L, W>::THREADS)) void norm_residual_b
       }
     }
   }
+  if (holds) { whole(0, s1); whole(1, s2); whole(2, s3); whole(3, s4); }
   float *part = a.part + (size_t)blockIdx.x * nsums * C;
   if (a.sums12) {
     slots_sum<T, L, W>(s1, comb, C, [&](int c, float v) { part[c] = v; });

@@ -44,24 +44,23 @@ def test_short_rows_whose_last_chunk_is_shorter_than_a_piece(C, dtype):
             assert_within(normed.detach(), want["normed"], "normed")
 
 
-def signs(g, *shape):
-    return torch.randint(0, 2, shape, generator=g).float() * 2 - 1
-
-
 def integers(P, C, groups, dt, seed, scale):
     """Rows of +-1: their rms norm with eps = 0 is themselves (C times the rounded 1 / C is 1 for these C, and the root of 1 is 1)."""
     assert float(np.float32(np.float64(C) * np.float64(np.float32(1) / np.float32(C)))) == 1.0
-    g = torch.Generator().manual_seed(seed)
-    t = {"x": signs(g, P, C).to(dt), "y": signs(g, P, C).to(dt), "weight": torch.randint(1, 3, (C,), generator=g).float(),
-         "gate": torch.randint(1, 3, (groups, C), generator=g).to(dt) if groups else None, "scale": torch.full((C,), scale),
-         "next_weight": torch.ones(C)}
-    t = {n: None if v is None else v.to(DEV) for n, v in t.items()}
-    return t, torch.randint(-1, 2, (P, C), generator=g).to(dt).to(DEV)
+    g = torch.Generator(device=DEV).manual_seed(seed)
+
+    def draw(low, high, *shape):
+        return torch.randint(low, high, shape, generator=g, device=DEV).to(torch.float32 if len(shape) == 1 else dt)
+    t = {"x": draw(0, 2, P, C) * 2 - 1, "y": draw(0, 2, P, C) * 2 - 1, "weight": draw(1, 3, C), "gate": draw(1, 3, groups, C) if groups else None,
+         "scale": torch.full((C,), scale, device=DEV), "next_weight": torch.ones(C, device=DEV)}
+    return t, draw(-1, 2, P, C)
 
 
+# (the last row: more than 128 row sets for a workgroup, whose sums go to LDS in between, in one group, in parts of one and over several)
 EXACT = [(0, 140003, 24), (0, 140003, 31), (0, 40011, 131), (0, 20003, 259), (0, 9001, 520), (0, 3001, 1283), (0, 2001, 3001), (0, 70000, 64),
          (0, 33, 5), (0, 257, 3), (140003, 1, 31), (20003, 1, 131), (7, 20001, 31), (3, 6007, 131), (11, 819, 520), (16, 1283, 259), (700, 2, 40),
-         (5003, 3, 63), (2503, 9, 131), (3001, 2, 1283), (1200, 70, 24)]
+         (5003, 3, 63), (2503, 9, 131), (3001, 2, 1283), (1200, 70, 24),
+         (0, 2200003, 24), (0, 300007, 520), (0, 40009, 3001), (3, 1500001, 8), (600, 5003, 24), (100003, 33, 40), (1031, 63, 3001), (70, 9001, 131)]
 
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
@@ -92,3 +91,28 @@ def test_column_sums_of_integers_are_exact(groups, each, C, dtype):
     back = ops.norm_residual_bwd(t["x"], None, None, None, None, "none", None, t["next_weight"], None, d, "rms", 0.0)
     assert torch.equal(back["next_weight"].double(), (d.double() * t["x"].double()).sum(0))
     assert torch.equal(back["next_bias"].double(), d.double().sum(0))
+
+
+def test_column_sums_of_many_equal_terms():
+    """Equal terms are rounded the same way at every step, so a long chain of fp32 additions drifts: n 2^-24 of the sum at most.  A lane adds
+    up 128 row sets, then these sums (fewer than 20 here: a workgroup has up to 2344 row sets), then come the 32 row slots of a workgroup;
+    then fp64, and one rounding."""
+    from cpfn_amd import ops
+    c = torch.full((), 0.1, device=DEV)
+    tol = 1.01 * (128 + 20 + 31 + 1) * 2.0 ** -24
+
+    def near(got, n, name):
+        off = float((got.double() / (n * c.double()) - 1.0).abs().max())
+        assert off <= tol, (name, off / 2.0 ** -24)
+    P, C = 2048 * 512 * 32, 8
+    ones, d, w = torch.ones(P, C, device=DEV), c.expand(P, C).contiguous(), torch.ones(C, device=DEV)
+    back = ops.norm_residual_bwd(ones, None, None, None, None, "none", None, w, None, d, "rms", 0.0, needs=("next_weight", "next_bias"))
+    near(back["next_weight"], P, "next_weight")
+    near(back["next_bias"], P, "next_bias")
+    for groups, each in ((600, 65536), (300000, 128)):
+        P = groups * each
+        ones, d, gate = torch.ones(P, C, device=DEV), c.expand(P, C).contiguous(), torch.ones(groups, C, device=DEV)
+        back = ops.norm_residual_bwd(ones, ones, w, torch.zeros_like(w), gate, "none", w, None, d, None, "rms", 0.0, needs=("weight", "bias", "gate", "scale"))
+        near(back["gate"], each, "gate")
+        for n in ("weight", "bias", "scale"):
+            near(back[n], P, n)
