@@ -95,7 +95,7 @@ struct Norm {
     if (gate.defined()) {
       check_rows(gate, "gate", &x);
       const int64_t G = gate.size(0);
-      REQUIRE(gate.size(1) == C && (P > 0 ? G >= 1 && P % G == 0 : G == 0),
+      REQUIRE(gate.size(1) == C && (P == 0 || (G >= 1 && P % G == 0)),
               "gate must be [P, C], or [G, C] for G groups of P / G consecutive rows (got ", gate.sizes(), " for ", x.sizes(), ")");
     }
     check_vector(weight, "weight", x);
@@ -145,7 +145,7 @@ struct Norm {
     if (!any) return g;
     for (int i : {0, 1})
       if (needs[i]) g[i] = at::empty({P, C}, x.options());
-    if (needs[4]) g[4] = at::empty(gate.sizes(), x.options());
+    if (needs[4]) g[4] = P == 0 ? at::zeros(gate.sizes(), x.options()) : at::empty(gate.sizes(), x.options());
     const auto f32 = x.options().dtype(at::kFloat);
     for (int i : {2, 3, 5, 6, 7})
       if (needs[i]) g[i] = P == 0 ? at::zeros({C}, f32) : at::empty({C}, f32);
