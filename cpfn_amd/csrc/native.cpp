@@ -8,6 +8,7 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
@@ -203,11 +204,14 @@ void not_again(variable_list &grads, const char *what) {
 }
 
 // Forward-mode derivatives (torch.autograd.forward_ad) are refused: a kernel reads an input's value alone, and its result would stand for
-// one whose derivative is zero.  Also where autograd records nothing: neither requires_grad nor no_grad says anything about them.
+// one whose derivative is zero.  Also where autograd records nothing: neither requires_grad nor no_grad says anything about them.  There
+// are tangents only while a dual level is open, which is asked first (tensor by tensor a list of 301 cost 2 us more).
+bool tangents_about() { return torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr; }
 bool tangent(const Tensor &t) { return t.defined() && t._fw_grad(0).defined(); }
 bool tangent(const Maybe &t) { return t.has_value() && tangent(*t); }
 template <typename... A> void refuse_tangents(const char *what, const A &...tensors) {
-  REQUIRE(!(tangent(tensors) || ...), what, " has no forward-mode derivative (a tensor carries a tangent: torch.autograd.forward_ad.unpack_dual gives its value)");
+  REQUIRE(!tangents_about() || !(tangent(tensors) || ...), what,
+          " has no forward-mode derivative (a tensor carries a tangent: torch.autograd.forward_ad.unpack_dual gives its value)");
 }
 
 // A backward pass that is captured must not reach a leaf whose gradient is accumulated on the default stream, which cannot take part in a
@@ -421,11 +425,12 @@ struct Table {
   std::vector<int> type;
   int64_t bytes = 0;
   bool recorded = false;                     // a tensor that autograd follows
+  const bool tangents = tangents_about();
 
   const Tensor &add(PyObject *o, const char *name, c10::Device &device) {
     REQUIRE(THPVariable_Check(o), name, " must be tensors");
     const Tensor &t = THPVariable_Unpack(o);
-    refuse_tangents(name, t);
+    if (tangents) refuse_tangents(name, t);
     recorded |= t.requires_grad();
     REQUIRE(t.is_cuda(), name, " must be CUDA(HIP) tensors: CPU not supported");
     if (device.is_cpu()) device = t.device();
