@@ -19,8 +19,8 @@ namespace {
 // ITEMS: 64-choice steps of a wave.  4 up to RANK_SMALL choices (more workgroups: 60000 choices, 28 experts 10.6 -> 8.3 us), 8 above (fewer
 // counts to scan: 4000000 choices, 2000 experts 57 -> 44 us; 4194304, 128: 30.9 -> 30.5).
 //
-// Measured: 4194304 choices, 128 experts 26 us, 1.9 TB/s of choices and places (a choice is read twice; without the ranks' arithmetic 22);
-// 4000000, 2000 experts 38 us; 60000, 28 experts 7.6 us, two launches.
+// Measured: 4194304 choices, 128 experts 28 us (count 8, scan 5.5, ranks 14.5), 1.8 TB/s of choices and places (a choice is read twice; the
+// ranks' arithmetic is 4 of a call's 26); 4000000, 2000 experts 37 us (6, 11, 21); 60000, 28 experts 8.2 us, two launches.
 constexpr int RANK_WAVES = 8;
 constexpr long long RANK_SMALL = 1 << 19;
 constexpr int rank_tile(int items) { return RANK_WAVES * items * 64; }
@@ -210,8 +210,8 @@ __global__ __launch_bounds__(RANK_WAVES * 64) void route_rank_kernel(const I *__
 // workgroups, measured 0 to 40 % slower at 131072 x 128 .. 50000 x 1024 rows: the chip holds enough groups).  A row is walked in
 // 16-byte pieces; the last piece of a row whose length is no multiple of one ENDS with the row and overlaps the piece before it: its
 // lane moves (or computes) a few elements that another lane moves too, to the same value.  Rows shorter than a piece go element by element.
-// Memory bound.  Measured (bf16): 131072 x 128 to 2 of 8: gather 16.5 us, combine 17.4, its adjoint 30 (6.1, 5.8, 5.5 TB/s); 50000 x 1024 to 4
-// of 64: 97, 88, 175 us (5.3, 5.6, 5.1); fp32 30000 x 259 to 3 of 64: 29, 30, 56 (4.3, 4.2, 3.9).
+// Memory bound.  Measured (bf16): 131072 x 128 to 2 of 8: gather 20 us, combine 21, its adjoint 30 (5.2, 5.0, 5.7 TB/s); 50000 x 1024 to 4
+// of 64: 91, 90, 173 us (5.6, 5.7, 5.3); fp32 30000 x 259 to 3 of 64: 33, 32, 47 (3.8, 3.9, 4.6).
 constexpr int MOVE_THREADS = 256;
 constexpr long long MOVE_BLOCKS = 1 << 20;
 constexpr int MOVE_MAX_C = 1 << 30;               // (a row is walked with 32-bit steps of up to 2048 elements)

@@ -18,9 +18,10 @@
 // Memory bound up to 512 channels; above, registers (1024: one wave on a SIMD), the barriers of the row sums (up to six a row) and the
 // workgroups' sums (16 MB) show.
 // Measured (bf16, both launches):
-//   131072 x 128, layer, sigmoid gate for each row    57 us   4.7 TB/s      262144 x 64, rms, no gate      45 us   4.5 TB/s
-//   65536 x 512, rms, gate for each row              111 us   4.8 TB/s      100003 x 131, rms, no gate     51 us   3.1 TB/s
-//   32768 x 1024, layer, gate for 2048 rows           94 us   4.3 TB/s      fp32 20528 x 259, shared gate  36 us   3.5 TB/s
+//   131072 x 128, layer, sigmoid gate for each row    50 us   5.3 TB/s      262144 x 64, rms, no gate      39 us   5.1 TB/s
+//   65536 x 512, rms, gate for each row               90 us   5.9 TB/s      100003 x 131, rms, no gate     49 us   3.2 TB/s
+//   32768 x 1024, layer, gate for 2048 rows           80 us   5.0 TB/s      fp32 20528 x 259, shared gate  36 us   3.5 TB/s
+//   262144 x 128, layer, gate for 32 rows             82 us   4.9 TB/s      8192 x 4096, layer, no gate    93 us   4.4 TB/s
 // The kernels of the whole block without branches, against the one with them: 32768 x 1024 110 -> 100 us, 8192 x 4096 134 -> 109,
 // fp32 20528 x 259 44 -> 36; of the norm in front: 32768 x 1024 57 -> 52.
 #include "rownorm.h"

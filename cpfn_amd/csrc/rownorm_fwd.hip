@@ -1,9 +1,10 @@
 // Norms before and after a residual block, its gate and its residual scale in one pass over the rows (forward; the formulas are in
 // rownorm.h).  Memory bound: x, y and the gate are read once, out and normed written once; the op-by-op form moves each of the ~12
 // intermediate tensors through memory.  Measured (bf16; a copy of gigabytes reaches 4.9 TB/s, one that fits the last-level cache 8.6):
-//   131072 x 128, layer, sigmoid gate for each row    32 us   5.2 TB/s      262144 x 64, rms, no gate      21 us   6.3 TB/s
-//   65536 x 512, rms, gate for each row               61 us   5.5 TB/s      100003 x 131, rms, no gate     24 us   4.4 TB/s
-//   32768 x 1024, layer, gate for 2048 rows           51 us   5.2 TB/s      fp32 20528 x 259, shared gate  18 us   4.8 TB/s
+//   131072 x 128, layer, sigmoid gate for each row    33 us   5.1 TB/s      262144 x 64, rms, no gate      26 us   5.1 TB/s
+//   65536 x 512, rms, gate for each row               61 us   5.5 TB/s      100003 x 131, rms, no gate     30 us   3.5 TB/s
+//   32768 x 1024, layer, gate for 2048 rows           51 us   5.3 TB/s      fp32 20528 x 259, shared gate  20 us   4.2 TB/s
+//   262144 x 128, layer, gate for 32 rows             52 us   5.2 TB/s      8192 x 4096, layer, no gate    51 us   5.3 TB/s
 // Ragged rows cost instructions (masks of the last piece, three more stores).
 #include "rownorm.h"
 

@@ -2,6 +2,9 @@
 // anywhere (norms, routed rows, gradient lists).  The vector types carry the ELEMENT's alignment: the compiler still emits one
 // 16-byte access (the target reads and writes global memory at any alignment), so that an odd number of channels, a slice of a
 // buffer or a parameter inside a flat buffer takes the same path as an aligned tensor.
+//
+// Figures in the comments of these kernels: "measured" are kernel durations of a trace (profiles/block_operators_kernels.txt); "a -> b" and
+// other comparisons of two choices are calls in a row between two events, which hold the launches' gaps too, in one run of both sides.
 #pragma once
 #include "common.h"
 

@@ -8,7 +8,7 @@ tensors.  Capturable: learning rate, step count and `found_inf` (set it before `
 gradients) are device scalars.  GPU only — on CPU the trainer keeps torch.optim.Adam.
 
 `grad_norm`, `clip_grads_` and `clip_grad_norm_` take any list of gradients (csrc/gradnorm.hip): the norm over all of them and their
-clipping, in two launches for up to 130 tensors; `FlatAdam.step(max_grad_norm=...)` clips what it reads from the flat buffer."""
+clipping: two launches for up to 130 tensors of together a few million values, three where they are more; `FlatAdam.step(max_grad_norm=...)` clips what it reads from the flat buffer."""
 import torch
 
 from . import lib as _l

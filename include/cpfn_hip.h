@@ -107,7 +107,7 @@ CPFN_API int cpfn_ball_query(const float *xyz, const float *new_xyz, int B, int 
  * (modules/geometry_utils.py:212-215): the same expanded D as the ball query,
  * ascending, ties to the lower index; returns SQUARED distances (can be < 0).
  * unknown[B,N,3] (queries), known[B,M,3] -> dist2[B,N,3], idx[B,N,3].
- * M < 3 leaves +inf / M in the unused slots. */
+ * M < 3, or a query that is not finite, leaves +inf / M in the unused slots. */
 CPFN_API int cpfn_three_nn(const float *unknown, const float *known, int B, int N, int M,
                   float *dist2, int *idx, void *stream);
 /* cpfn_three_nn (direct == 0) / cpfn_three_nn_direct (direct != 0) and, when w is not NULL, cpfn_three_weights on the distances
@@ -156,7 +156,8 @@ CPFN_API int cpfn_three_weights(const float *dist, int64_t R, float *w, void *st
 /* ------------------------------------------------- channel-major fp32 ops
  * Drop-in layouts of the reference's bound functions (bindings.cpp:6-19). */
 
-/* three_weighted_sum (interpolate_gpu.cu:72-101): feats[B,C,M], idx/w[B,N,3] -> out[B,C,N] */
+/* three_weighted_sum (interpolate_gpu.cu:72-101): feats[B,C,M], idx/w[B,N,3] -> out[B,C,N].  Here and in every interpolation below an
+ * index >= M (cpfn_three_nn's slot without a neighbour) reads row M - 1 of its cloud, one < 0 row 0. */
 CPFN_API int cpfn_three_interp_fwd(const float *feats, const int *idx, const float *w, int B,
                           int C, int M, int N, float *out, void *stream);
 /* three_weighted_sum_grad (interpolate_gpu.cu:116-143): grad_out[B,C,N] -> grad_feats[B,C,M]
