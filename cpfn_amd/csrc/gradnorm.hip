@@ -26,9 +26,10 @@ constexpr int MOST_BLOCKS = 2000;
 // Bytes at the list's end that pass 1 leaves in the last-level cache (of 256 MB; the rest is not kept): 271M bf16 to fp32, both passes, none
 // 383 us, 96 MB 375, 240 MB 360
 constexpr long long KEPT = 240ll << 20;
-// The scaling launch has many short workgroups, whose stretches of memory follow each other closely: 271M values bf16 to fp32 268 us measured,
-// 6.1 TB/s; in a comparison 284, shares of 4096 292, of 1024 397, 2000 workgroups with strides through whole tensors 357.  In place a workgroup that finds
-// nothing to do should not be one of too many: 200M bf16 scaled, 35M fp32 left alone: 8192 157 and 4.9 us (4096: 153, 6; 16384: 161, 5).
+// The scaling launch has many short workgroups, whose stretches of memory follow each other closely: 271M values bf16 to fp32 268 us
+// measured, 6.1 TB/s; in a comparison 284, shares of 4096 292, of 1024 397, 2000 workgroups with strides through whole tensors 357.  In
+// place a workgroup that finds nothing to do should not be one of too many: 200M bf16 scaled, 35M fp32 left alone: 8192 157 and 4.9 us
+// (4096: 153, 6; 16384: 161, 5).
 constexpr int SCALE_SHARE = 2048, SCALE_SHARE_IN_PLACE = 8192;
 constexpr long long MOST_SCALE_BLOCKS = 1 << 22;         // (a launch has fewer than 2^32 lanes)
 // The partial sums are added by every scaling workgroup, or, where that would be more loads than these, by one launch in between
